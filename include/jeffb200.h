@@ -252,6 +252,68 @@ int jb_kv_scatter(const uint16_t* kn, const uint16_t* vn, int b, int n, const in
                   int64_t page_bytes, const int32_t* out_tables, int table_stride, int kv_entry, int attn_layer,
                   int attn_layers, void* stream);
 
+/* ---------------------------------------------------------------- single tokens over the prefix pool
+ *
+ * What a continuation token by token needs beside the decision pass. These entry points have no counterpart in the
+ * reference, which only answers prefill passes. Key/value pages are given as the pool's data, its pages and their
+ * stride in bytes; an entry of a block table outside [0, pages) is taken for no page (its tokens are left out of the
+ * attention, a state in it reads as zeros), and nothing is written outside the pool. */
+
+/* Block tables and slot maps from the requests' lengths, on the device. Row r of b holds lengths[r] tokens and adds
+ * added[r] (negative counts as 0). It takes the pages its new tokens need, off the free list in row order (free_pages,
+ * the first free page first), into its table's entries from kv_entry + ceil(lengths[r] / page_tokens) on; with fixed
+ * != 0 a row that holds none and adds some first takes kv_entry pages into entries 0 .. kv_entry - 1 (a prefix's state
+ * and convolution pages). All other entries stay. The new tokens are packed row after row: for token t of `tokens`
+ * slots[t] = page * page_tokens + place in the page, rows[t] and positions[t]; -1, -1 and 0 past the last one. starts
+ * (b + 1) is each row's first token, taken (b + 1) the pages that the rows before it take. taken[b] > free_count: the
+ * list was too short; the entries past it are 0 (the sink) and their tokens' slots -1. A token past the table's last
+ * entry (width) takes no page and has slot -1; tokens past `tokens` are not listed. */
+int jb_block_tables(const int32_t* lengths, const int32_t* added, int b, const int32_t* free_pages, int free_count,
+                    int32_t* tables, int table_stride, int width, int kv_entry, int page_tokens, int fixed, int tokens,
+                    int64_t* slots, int32_t* rows, int32_t* positions, int32_t* starts, int32_t* taken, void* stream);
+
+/* Attention input side of t tokens with several rotary axes: per query and key head RMSNorm * w1, then the pair
+ * (d, d + 32), d < 32, turned by positions[axis][t] * inv_freq[d], axis = (axes >> 2 d) & 3 (positions (axes, t), an
+ * axis axis_stride entries after the one before); fp32 with one rounding to bf16, the angle in fp64. pr (t, ldpr) as
+ * jb_attn_prep_rows. q (t, 8, 256). Keys and values go to kn and vn (t, 2, 256), into the pages that slots (t) name
+ * (slot = page * 32 + place; a slot outside the pool is written nowhere), or to both. */
+int jb_attn_prep_axes(const uint16_t* pr, int64_t ldpr, int t, const float* q_w1, const float* k_w1,
+                      const float* inv_freq, const int32_t* positions, int64_t axis_stride, int64_t axes, uint16_t* q,
+                      uint16_t* kn, uint16_t* vn, void* kv, int64_t pages, int64_t page_bytes, int attn_layer,
+                      int attn_layers, const int64_t* slots, void* stream);
+
+/* Attention of one new token per row over its cached keys: y (b, heads, dim) = softmax(scale q . k_j) v_j over the
+ * tokens j < lengths[r] of pages tables[r][kv_entry + j / 32] (at most what the table's width holds); a row without
+ * tokens is 0. dim 64, 128 or 256; heads a multiple of kv_heads, at most 16 to one. pr (nullable): y is multiplied by
+ * sigmoid(pr[r, 2 dim h + dim + d]), the gate of jb_gate_mul. fp32 with one rounding to bf16. The keys of all rows
+ * are cut into equal shares over the GPU and rows that were cut are joined from `scratch`
+ * in a fixed order. */
+int jb_decode_attention(const uint16_t* q, int64_t ldq, const void* kv, int64_t pages, int64_t page_bytes,
+                        int attn_layer, int attn_layers, const int32_t* tables, int table_stride, int width,
+                        int kv_entry, const int32_t* lengths, int b, int heads, int kv_heads, int dim, float scale,
+                        const uint16_t* pr, int64_t ldpr, uint16_t* y, int64_t ldy, float* scratch,
+                        int64_t scratch_floats, void* stream);
+
+/* Linear attention with a decay for each head, over n tokens of b rows: S_t = e^g S_{t-1} + k_t v_t^T, o_t = S_t^T q_t
+ * / sqrt(128), states (128, 128) fp32 as jb_gdn_scan's (flat head first_head + h). q, k, v: 128 contiguous values a
+ * head, heads 128 apart, their token and row strides given (multiples of 8); o (b, n, heads, 128). g: fp32, a head's
+ * log-decay at g[row * g_row + token * g_tok + h] (strides 0, 0: one decay for each head). real (nullable): row r has
+ * real[r] tokens; outputs past them are 0 and the state stays. out_tables (nullable): the final states' pages; the
+ * reserved pages 0 and 1 are never written. */
+int jb_linear_scan(const uint16_t* q, int64_t q_row, int64_t q_tok, const uint16_t* k, int64_t k_row, int64_t k_tok,
+                   const uint16_t* v, int64_t v_row, int64_t v_tok, const float* g, int64_t g_row, int64_t g_tok,
+                   const int32_t* real, uint16_t* o, int b, int n, int heads, void* state, int64_t pages,
+                   int64_t page_bytes, int heads_per_page, int first_head, const int32_t* tables, int table_stride,
+                   const int32_t* out_tables, int out_stride, float* scratch, int64_t scratch_floats, void* stream);
+
+/* jb_linear_scan's recurrence for one token per row (q, k, v (b, heads, 128), g (b, heads) or one decay for each head,
+ * o (b, heads, 128)), the new states written to out_tables' pages (the same tables: in place). beta (nullable, bf16
+ * (b, heads)): the gated delta rule of jb_gdn_scan, v replaced by beta (v - (e^g S)^T k). */
+int jb_linear_step(const uint16_t* q, int64_t q_row, const uint16_t* k, int64_t k_row, const uint16_t* v,
+                   int64_t v_row, const float* g, int64_t g_row, const uint16_t* beta, uint16_t* o, int b, int heads,
+                   void* state, int64_t pages, int64_t page_bytes, int heads_per_page, int first_head,
+                   const int32_t* tables, int table_stride, const int32_t* out_tables, int out_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,23 +16,26 @@ HEADER = HERE.parent / "include" / "jeffb200.h"
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
+_F = ctypes.c_float
 
 
 
 def parse_header(text: str) -> dict[str, tuple[str, str]]:
-    """{entry point: (return kind, argument kinds)} from the header: "p" pointer, "i" int, "l" int64_t."""
+    """{entry point: (return kind, argument kinds)} from the header: "p" pointer, "i" int, "l" int64_t,
+    "f" float."""
     out: dict[str, tuple[str, str]] = {}
     for ret, name, params in re.findall(r"^\s*(int|const char\*)\s+(jb_\w+)\(([^)]*)\);", text, flags=re.M | re.S):
         kinds = ""
         for param in (x.strip() for x in params.split(",")):
             if not param or param == "void":
                 continue
-            kinds += "p" if "*" in param else ("l" if "int64_t" in param else "i")
+            kinds += ("p" if "*" in param else "l" if "int64_t" in param else "f" if param.startswith("float ")
+                      else "i")
         out[name] = ("s" if ret.startswith("const char") else "i", kinds)
     return out
 
 
-_CT = {"p": _P, "i": _I, "l": _L}
+_CT = {"p": _P, "i": _I, "l": _L, "f": _F}
 
 
 class JbError(RuntimeError):

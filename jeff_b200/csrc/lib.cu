@@ -158,6 +158,8 @@ int make_tmap_nd(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, 
 #include "gdn_tc.cu"
 #include "attention.cu"
 #include "attention_tc.cu"
+#include "decode.cu"
+#include "linear.cu"
 
 extern "C" int jb_abi_version(void) { return 2; }
 

@@ -1,0 +1,204 @@
+// Linear attention with a decay for each head, each row resuming from its state in the prefix pool:
+//   S_t = e^{g_t} S_{t-1} + k_t v_t^T,   o_t = S_t^T q_t / sqrt(128)
+// over (128 key, 128 value) fp32 states: a chunked form for prompts and a recurrent one for single tokens, which with
+// beta is the gated delta rule (v_t replaced by beta_t (v_t - (e^{g_t} S_{t-1})^T k_t)).
+//
+// A state is at slot (flat head % heads_per_page) of page tables[r][flat head / heads_per_page], as in gdn.cu. A page
+// outside the pool reads as zeros; nothing is written to such a page or to the reserved pages (the sink, the zeros).
+
+namespace jb {
+namespace lin {
+
+constexpr int D = 128;
+constexpr int64_t STATE_BYTES = (int64_t)D * D * 4;
+constexpr int RESERVED = 2;
+
+struct Pool {
+  uint8_t* base;
+  int64_t pages, page_bytes;
+  int heads_per_page, first_head;
+  const int* tables;
+  int table_stride;
+  const int* out_tables;
+  int out_stride;
+};
+
+__device__ __forceinline__ const float* state_in(const Pool& p, int row, int h) {
+  const int flat = p.first_head + h;
+  const int page = p.tables[(int64_t)row * p.table_stride + flat / p.heads_per_page];
+  if (page < 0 || page >= p.pages) return nullptr;
+  return reinterpret_cast<const float*>(p.base + page * p.page_bytes + (flat % p.heads_per_page) * STATE_BYTES);
+}
+__device__ __forceinline__ float* state_out(const Pool& p, int row, int h) {
+  if (!p.out_tables) return nullptr;
+  const int flat = p.first_head + h;
+  const int page = p.out_tables[(int64_t)row * p.out_stride + flat / p.heads_per_page];
+  if (page < RESERVED || page >= p.pages) return nullptr;
+  return reinterpret_cast<float*>(p.base + page * p.page_bytes + (flat % p.heads_per_page) * STATE_BYTES);
+}
+
+struct Args {
+  const __nv_bfloat16* q;
+  const __nv_bfloat16* k;
+  const __nv_bfloat16* v;
+  int64_t q_row, k_row, v_row;   // strides in elements between rows, and between a row's tokens
+  int64_t q_tok, k_tok, v_tok;
+  const float* g;
+  int64_t g_row, g_tok;          // both 0: a constant decay for each head
+  const __nv_bfloat16* beta;     // (b, heads) or null
+  const int* real;               // (b,) or null
+  __nv_bfloat16* o;
+  int64_t o_row, o_tok;
+  int n, heads;
+  Pool pool;
+};
+
+// ------------------------------------------------------------------ token by token
+//
+// One CTA per (row, head); warp w holds key rows [16 w, 16 w + 16) of the state in registers, lane l value columns
+// [4 l, 4 l + 4): 16-byte accesses, 512 contiguous bytes a warp and instruction, all 16 of a thread in flight.
+
+__device__ __forceinline__ float4 ld_bf4(const __nv_bfloat16* p) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  return make_float4(bf_lo(u.x), bf_hi(u.x), bf_lo(u.y), bf_hi(u.y));
+}
+
+template <bool DELTA>
+__global__ void __launch_bounds__(256) recurrent_kernel(const Args a) {
+  pdl_begin();
+  __shared__ float sk[D], sq[D];
+  __shared__ float4 part[8][32];
+  const int row = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int stop = a.real ? min(max(a.real[row], 0), a.n) : a.n;
+  const float* in = state_in(a.pool, row, h);
+  float4 S[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    S[i] = in ? reinterpret_cast<const float4*>(in + (warp * 16 + i) * D)[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+  const float scale = rsqrtf((float)D);
+  for (int t = 0; t < stop; ++t) {
+    if (threadIdx.x < D) sk[threadIdx.x] = bf2f(a.k[row * a.k_row + t * a.k_tok + h * D + threadIdx.x]);
+    else sq[threadIdx.x - D] = bf2f(a.q[row * a.q_row + t * a.q_tok + h * D + threadIdx.x - D]);
+    float4 v = ld_bf4(a.v + row * a.v_row + t * a.v_tok + h * D + 4 * lane);
+    const float e = expf(a.g[row * a.g_row + t * a.g_tok + h]);
+    __syncthreads();
+    float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (DELTA) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float kk = sk[warp * 16 + i];
+        c.x += S[i].x * kk;
+        c.y += S[i].y * kk;
+        c.z += S[i].z * kk;
+        c.w += S[i].w * kk;
+      }
+      part[warp][lane] = c;
+      __syncthreads();
+      c = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const float4 x = part[w][lane];
+        c.x += x.x;
+        c.y += x.y;
+        c.z += x.z;
+        c.w += x.w;
+      }
+      const float b = bf2f(a.beta[(int64_t)row * a.heads + h]);
+      v.x = b * (v.x - e * c.x);
+      v.y = b * (v.y - e * c.y);
+      v.z = b * (v.z - e * c.z);
+      v.w = b * (v.w - e * c.w);
+      c = make_float4(0.f, 0.f, 0.f, 0.f);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float kk = sk[warp * 16 + i], qq = sq[warp * 16 + i];
+      S[i].x = S[i].x * e + kk * v.x;
+      S[i].y = S[i].y * e + kk * v.y;
+      S[i].z = S[i].z * e + kk * v.z;
+      S[i].w = S[i].w * e + kk * v.w;
+      c.x += S[i].x * qq;
+      c.y += S[i].y * qq;
+      c.z += S[i].z * qq;
+      c.w += S[i].w * qq;
+    }
+    part[warp][lane] = c;
+    __syncthreads();
+    if (threadIdx.x < D) {
+      float o = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) o += reinterpret_cast<const float*>(part[w])[threadIdx.x];
+      a.o[row * a.o_row + t * a.o_tok + h * D + threadIdx.x] = f2bf(o * scale);
+    }
+    __syncthreads();
+  }
+  for (int t = stop + warp; t < a.n; t += 8)
+    reinterpret_cast<uint2*>(a.o + row * a.o_row + t * a.o_tok + h * D)[lane] = make_uint2(0, 0);
+  float* out = state_out(a.pool, row, h);
+  if (out)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) reinterpret_cast<float4*>(out + (warp * 16 + i) * D)[lane] = S[i];
+}
+
+inline bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
+
+int check(const char* who, const Args& a, int b) {
+  const Pool& p = a.pool;
+  JB_REQUIRE(a.q && a.k && a.v && a.g && a.o && p.base && p.tables, "%s: null pointer", who);
+  JB_REQUIRE(b > 0 && a.n > 0 && a.heads > 0, "%s: %d rows, %d tokens, %d heads", who, b, a.n, a.heads);
+  JB_REQUIRE((int64_t)b * a.heads <= 0x7fffffff, "%s: %d rows of %d heads", who, b, a.heads);
+  JB_REQUIRE(aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.o) && aligned16(p.base) &&
+                 p.page_bytes % 16 == 0,
+             "%s: q, k, v, o and the pages must be 16-byte aligned", who);
+  JB_REQUIRE(((a.q_row | a.k_row | a.v_row | a.o_row | a.q_tok | a.k_tok | a.v_tok | a.o_tok) & 7) == 0,
+             "%s: the strides of q, k, v and o must be multiples of 8", who);
+  JB_REQUIRE(p.heads_per_page > 0 && p.heads_per_page * STATE_BYTES <= p.page_bytes,
+             "%s: %d heads per page do not fit pages of %lld bytes", who, p.heads_per_page, (long long)p.page_bytes);
+  const int last = p.first_head + a.heads - 1;
+  JB_REQUIRE(p.first_head >= 0 && last / p.heads_per_page < p.table_stride &&
+                 (!p.out_tables || last / p.heads_per_page < p.out_stride),
+             "%s: heads %d.. reach past the block table", who, p.first_head);
+  return JB_OK;
+}
+
+}  // namespace lin
+}  // namespace jb
+
+extern "C" int jb_linear_scan(const uint16_t* q, int64_t q_row, int64_t q_tok, const uint16_t* k, int64_t k_row,
+                              int64_t k_tok, const uint16_t* v, int64_t v_row, int64_t v_tok, const float* g,
+                              int64_t g_row, int64_t g_tok, const int32_t* real, uint16_t* o, int b, int n, int heads,
+                              void* state, int64_t pages, int64_t page_bytes, int heads_per_page, int first_head,
+                              const int32_t* tables, int table_stride, const int32_t* out_tables, int out_stride,
+                              float* scratch, int64_t scratch_floats, void* stream) {
+  using namespace jb;
+  const lin::Args a = {reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<const __nv_bfloat16*>(k),
+                       reinterpret_cast<const __nv_bfloat16*>(v), q_row, k_row, v_row, q_tok, k_tok, v_tok, g, g_row,
+                       g_tok, nullptr, real, reinterpret_cast<__nv_bfloat16*>(o), (int64_t)n * heads * lin::D,
+                       (int64_t)heads * lin::D, n, heads,
+                       {static_cast<uint8_t*>(state), pages, page_bytes, heads_per_page, first_head, tables,
+                        table_stride, out_tables, out_stride}};
+  if (int st = lin::check("jb_linear_scan", a, b)) return st;
+  launch_pdl(lin::recurrent_kernel<false>, b * heads, 256, 0, (cudaStream_t)stream, a);
+  return check_launch("linear recurrent_kernel");
+}
+
+extern "C" int jb_linear_step(const uint16_t* q, int64_t q_row, const uint16_t* k, int64_t k_row, const uint16_t* v,
+                              int64_t v_row, const float* g, int64_t g_row, const uint16_t* beta, uint16_t* o, int b,
+                              int heads, void* state, int64_t pages, int64_t page_bytes, int heads_per_page,
+                              int first_head, const int32_t* tables, int table_stride, const int32_t* out_tables,
+                              int out_stride, void* stream) {
+  using namespace jb;
+  const lin::Args a = {reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<const __nv_bfloat16*>(k),
+                       reinterpret_cast<const __nv_bfloat16*>(v), q_row, k_row, v_row, 0, 0, 0, g, g_row, 0,
+                       reinterpret_cast<const __nv_bfloat16*>(beta), nullptr, reinterpret_cast<__nv_bfloat16*>(o),
+                       (int64_t)heads * lin::D, 0, 1, heads,
+                       {static_cast<uint8_t*>(state), pages, page_bytes, heads_per_page, first_head, tables,
+                        table_stride, out_tables, out_stride}};
+  if (int st = lin::check("jb_linear_step", a, b)) return st;
+  JB_REQUIRE(out_tables, "jb_linear_step: null pointer (out_tables: where the new states go)");
+  if (beta) launch_pdl(lin::recurrent_kernel<true>, b * heads, 256, 0, (cudaStream_t)stream, a);
+  else launch_pdl(lin::recurrent_kernel<false>, b * heads, 256, 0, (cudaStream_t)stream, a);
+  return check_launch("linear recurrent_kernel");
+}

@@ -4,12 +4,18 @@ CPU fallback). Names, arguments and returns follow the reference's engine module
 - int4_product (int4_kernels.py:132-177), lora_shrink (fast_path.py:159-177): the fused W4A16 + multi-LoRA product;
 - add_rms, gated_norm, gate_mul, silu_mul (fast_path.py:80-156), rms_last (batched_path.py:274-275), embed;
 - gdn_prep_rows, gdn_scan (batched_kernels.py:89-261 and fla's chunk kernel), attn_prep_rows, paged_attention,
-  kv_scatter (batched_kernels.py:302-486, batched_path.py:345-349), readout_rows (batched_kernels.py:492-559).
+  kv_scatter (batched_kernels.py:302-486, batched_path.py:345-349), readout_rows (batched_kernels.py:492-559);
+- block_tables, attn_prep_axes, decode_attention, linear_scan, linear_step: single tokens over the prefix pool and
+  linear attention with a decay for each head, which the reference does not have. They take the pool's typed views
+  (PrefixPool.kv, PrefixPool.state), whose strides say where a page lies, and run on their tensors' device.
 
 Every function launches on the current torch stream and allocates its outputs only when no `out` is given (the
 recorded passes pass preallocated buffers, so graphs capture no allocation)."""
 
 from __future__ import annotations
+
+from collections.abc import Sequence
+from typing import NamedTuple
 
 import torch
 
@@ -349,3 +355,253 @@ def kv_scatter(kn: torch.Tensor, vn: torch.Tensor, n: int, real: torch.Tensor, p
     _lib.call("jb_kv_scatter", ptr(kn), ptr(vn), b, n, ptr(real), ptr(pool.data), pool.shapes.page_bytes,
               ptr(out_tables), out_tables.stride(0), pool.fixed_pages, attn_layer, pool.shapes.attn_layers,
               stream_ptr())
+
+
+# ---------------------------------------------------------------- single tokens over the prefix pool
+
+
+def _rows_of(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, ...], inner: int,
+             device: torch.device) -> None:
+    """`t` (shape) of `dtype` on `device`, its last `inner` dimensions packed and the others strided as they like."""
+    if t.dtype != dtype or tuple(t.shape) != shape:
+        raise ValueError(f"{name}: expected {dtype} of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA tensor, got one on {t.device}")
+    if t.device != device:
+        raise ValueError(f"{name}: expected a tensor on {device} as the others, got one on {t.device}")
+    step = 1
+    for size, stride in zip(reversed(shape[len(shape) - inner:]), reversed(t.stride()[len(shape) - inner:])):
+        if stride != step and size != 1:
+            raise ValueError(f"{name}: expected the last {inner} dimension(s) packed, got strides {t.stride()}")
+        step *= size
+
+
+def _tables_of(tables: torch.Tensor, name: str, rows: int, width: int, device: torch.device) -> None:
+    if tables.dim() != 2 or tables.shape[0] < rows or tables.shape[1] < width or tables.dtype != torch.int32 or \
+            tables.stride(1) != 1:
+        raise ValueError(f"{name}: expected int32 (rows >= {rows}, width >= {width}) with packed rows, got "
+                         f"{tuple(tables.shape)} {tables.dtype}, strides {tables.stride()}")
+    if tables.device != device:
+        raise ValueError(f"{name}: expected a tensor on {device}, got one on {tables.device}")
+
+
+def _cache_of(kv: torch.Tensor, attn_layer: int, device: torch.device) -> tuple[int, int]:
+    """(key/value heads, their width) of a cache of pages kv[page, layer, K|V, 32 tokens, head, dim]."""
+    if kv.dim() != 6 or kv.dtype != DT or kv.shape[2:4] != (2, 32):
+        raise ValueError(f"kv: expected bf16 pages (page, layer, 2, 32, heads, dim), got {kv.dtype} {tuple(kv.shape)}")
+    _rows_of(kv, "kv", DT, tuple(kv.shape), 5, device)
+    if not 0 <= attn_layer < kv.shape[1]:
+        raise ValueError(f"attn_layer {attn_layer}: the pages hold {kv.shape[1]} layers")
+    return kv.shape[4], kv.shape[5]
+
+
+def _on(device: torch.device, name: str, *args) -> None:
+    """One library call on `device` and its current stream."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, stream_ptr())
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, stream_ptr())
+
+
+class SlotMap(NamedTuple):
+    """Where a pass's new tokens go (block_tables): per packed token its slot in the cache (page * page_tokens + place,
+    -1 for none), its row and its position; each row's first token and the pages taken by the rows before it."""
+    slots: torch.Tensor       # (tokens,) int64
+    rows: torch.Tensor        # (tokens,) int32
+    positions: torch.Tensor   # (tokens,) int32
+    starts: torch.Tensor      # (b + 1,) int32
+    taken: torch.Tensor       # (b + 1,) int32
+
+
+def block_tables(lengths: torch.Tensor, new: torch.Tensor, free: torch.Tensor, tables: torch.Tensor, kv_entry: int,
+                 tokens: int, *, page_tokens: int = 32, fixed: bool = False, out: SlotMap | None = None) -> SlotMap:
+    """Block tables and slot maps from the requests' lengths, without the host. Row r holds lengths[r] tokens and adds
+    new[r]; the pages its new tokens need come off `free` (int32 page ids, the first to take first) in row order and
+    are written behind the row's own in `tables`, in place; fixed: a row that holds no token yet first takes kv_entry
+    pages into its entries [0, kv_entry) (a prefix's state and convolution pages, PrefixPool.reserve's order). Every
+    other entry stays as it was. `tokens` is the pass's capacity. taken[-1] > len(free) says that the free list was too
+    short: the entries it leaves without a page name the sink (0), and their tokens' slots are -1, as are those of
+    tokens past the table's width."""
+    dev = lengths.device
+    b = lengths.shape[0] if lengths.dim() == 1 else -1
+    _rows_of(lengths, "lengths", torch.int32, (b,), 1, dev)
+    _rows_of(new, "new", torch.int32, (b,), 1, dev)
+    if free.dim() != 1:
+        raise ValueError(f"free: expected a vector of page ids, got {tuple(free.shape)}")
+    _rows_of(free, "free", torch.int32, tuple(free.shape), 1, dev)
+    _tables_of(tables, "tables", b, kv_entry + 1, dev)
+    if out is None:
+        buf = torch.empty(4 * tokens + 2 * (b + 1), dtype=torch.int32, device=dev)
+        out = SlotMap(buf[:2 * tokens].view(torch.int64), buf[2 * tokens:3 * tokens], buf[3 * tokens:4 * tokens],
+                      buf[4 * tokens:4 * tokens + b + 1], buf[4 * tokens + b + 1:])
+    else:
+        for name, dtype, size in (("slots", torch.int64, tokens), ("rows", torch.int32, tokens),
+                                  ("positions", torch.int32, tokens), ("starts", torch.int32, b + 1),
+                                  ("taken", torch.int32, b + 1)):
+            _rows_of(getattr(out, name), name, dtype, (size,), 1, dev)
+    _on(dev, "jb_block_tables", ptr(lengths), ptr(new), b, ptr(free), free.shape[0], ptr(tables), tables.stride(0),
+        tables.shape[1], kv_entry, page_tokens, 1 if fixed else 0, tokens, *map(ptr, out))
+    return out
+
+
+def rope_axes(sections: Sequence[int], interleaved: bool = False) -> int:
+    """Which axis's position turns each of the 32 rotary frequencies, for attn_prep_axes: sections[a] frequencies of
+    axis a, one axis after the other, or interleaved (frequency i belongs to axis i mod the number of axes while that
+    axis has frequencies left, to axis 0 after that). At most four axes; 2 bits a frequency."""
+    n = len(sections)
+    if not 1 <= n <= 4 or sum(sections) != C.ROT // 2 or min(sections) < 0:
+        raise ValueError(f"sections {tuple(sections)}: one to four axes with {C.ROT // 2} frequencies in all")
+    if interleaved:
+        of = [i % n if i // n < sections[i % n] else 0 for i in range(C.ROT // 2)]
+    else:
+        of = [a for a, count in enumerate(sections) for _ in range(count)]
+    return sum(a << 2 * i for i, a in enumerate(of))
+
+
+def attn_prep_axes(pr: torch.Tensor, q_w1: torch.Tensor, k_w1: torch.Tensor, inv_freq: torch.Tensor,
+                   positions: torch.Tensor, axes: int, *, kn: torch.Tensor | None = None,
+                   vn: torch.Tensor | None = None, kv: torch.Tensor | None = None, attn_layer: int = 0,
+                   slots: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """attn_prep_rows for any number of tokens, with positions (axes, t) int32 of several axes (axes from rope_axes;
+    one axis: text). q (t, 8, 256); keys and values to kn and vn (t, 2, 256), into the cache pages kv at slots (t,)
+    int64 (block_tables; -1: nowhere), or both. Two tokens must not have the same slot. Unlike attn_prep_rows, which
+    keeps the reference's rounding points, everything between is fp32 (the angle fp64) and rounded once."""
+    dev, t = pr.device, pr.shape[0]
+    if pr.dim() != 2 or pr.shape[1] < C.ATTN_PROJ:
+        raise ValueError(f"pr: expected (tokens, at least {C.ATTN_PROJ}), got {tuple(pr.shape)}")
+    _rows_of(pr, "pr", DT, tuple(pr.shape), 1, dev)
+    _rows_of(q_w1, "q_w1", torch.float32, (C.HD,), 1, dev)
+    _rows_of(k_w1, "k_w1", torch.float32, (C.HD,), 1, dev)
+    _rows_of(inv_freq, "inv_freq", torch.float32, (C.ROT // 2,), 1, dev)
+    count = positions.shape[0] if positions.dim() == 2 else -1
+    _rows_of(positions, "positions", torch.int32, (count, t), 1, dev)
+    if not 0 <= axes < 1 << C.ROT or any(axes >> 2 * i & 3 >= count for i in range(C.ROT // 2)):
+        raise ValueError(f"axes: a frequency has an axis past the positions' {count}")
+    for name, x in (("kn", kn), ("vn", vn)):
+        if x is not None:
+            _rows_of(x, name, DT, (t, C.NKV, C.HD), 3, dev)
+    if slots is not None:
+        _rows_of(slots, "slots", torch.int64, (t,), 1, dev)
+    if kv is not None and _cache_of(kv, attn_layer, dev) != (C.NKV, C.HD):
+        raise ValueError(f"kv: expected pages of {C.NKV} heads of {C.HD}, got {tuple(kv.shape)}")
+    if out is None:
+        out = torch.empty(t, C.NQ, C.HD, dtype=DT, device=dev)
+    else:
+        _rows_of(out, "out", DT, (t, C.NQ, C.HD), 3, dev)
+    _on(dev, "jb_attn_prep_axes", ptr(pr), pr.stride(0), t, ptr(q_w1), ptr(k_w1), ptr(inv_freq), ptr(positions),
+        positions.stride(0), axes - (1 << 64) if axes >> 63 else axes, ptr(out), ptr(kn), ptr(vn), ptr(kv),
+        0 if kv is None else kv.shape[0], 0 if kv is None else 2 * kv.stride(0), attn_layer,
+        0 if kv is None else kv.shape[1], ptr(slots))
+    return out
+
+
+def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, attn_layer: int, lengths: torch.Tensor,
+                     kv_entry: int, *, scale: float | None = None, pr: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token per row, q (b, heads, dim), over the row's lengths[r] cached tokens (its own among
+    them, once attn_prep_axes has written it) in the pages tables[r][kv_entry + j // 32] of kv; heads of 64, 128 or
+    256, up to 16 query heads to a key/value head, scale 1 / sqrt(dim) unless given. A row without tokens is zeros.
+    With pr (the q_proj output, query and gate interleaved per head): times sigmoid(gate), as (b, heads * dim), the
+    o_proj's input; without, (b, heads, dim). fp32 with one rounding."""
+    dev = q.device
+    if q.dim() != 3:
+        raise ValueError(f"q: expected (rows, heads, dim), got {tuple(q.shape)}")
+    b, heads, dim = q.shape
+    _rows_of(q, "q", DT, (b, heads, dim), 2, dev)
+    kv_heads, kv_dim = _cache_of(kv, attn_layer, dev)
+    if kv_dim != dim:
+        raise ValueError(f"q: heads of {dim}, the pages' keys are {kv_dim} wide")
+    _tables_of(tables, "tables", b, kv_entry, dev)
+    _rows_of(lengths, "lengths", torch.int32, (b,), 1, dev)
+    if pr is not None:
+        if pr.dim() != 2 or pr.shape[1] < 2 * heads * dim:
+            raise ValueError(f"pr: expected (rows, at least {2 * heads * dim}), got {tuple(pr.shape)}")
+        _rows_of(pr, "pr", DT, (b, pr.shape[1]), 1, dev)
+    shape = (b, heads, dim) if pr is None else (b, heads * dim)
+    if out is None:
+        out = torch.empty(shape, dtype=DT, device=dev)
+    else:
+        _rows_of(out, "out", DT, shape, len(shape) - 1, dev)
+    if scratch is not None:
+        _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), dev)
+    _on(dev, "jb_decode_attention", ptr(q), q.stride(0), ptr(kv), kv.shape[0], 2 * kv.stride(0), attn_layer,
+        kv.shape[1], ptr(tables), tables.stride(0), tables.shape[1], kv_entry, ptr(lengths), b, heads, kv_heads, dim,
+        dim ** -0.5 if scale is None else scale, ptr(pr), 0 if pr is None else pr.stride(0), ptr(out), out.stride(0),
+        ptr(scratch), 0 if scratch is None else scratch.numel())
+    return out
+
+
+# ---------------------------------------------------------------- linear attention with a decay for each head
+
+
+def _linear_of(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor,
+               tables: torch.Tensor, layer: int, out_tables: torch.Tensor | None,
+               out: torch.Tensor | None) -> tuple[torch.Tensor, tuple]:
+    """What linear_scan and linear_step check alike; (o, the states' arguments)."""
+    dev = q.device
+    b, heads = q.shape[0], q.shape[-2]
+    shape = (*q.shape[:-1], C.DK)
+    for name, x in (("q", q), ("k", k), ("v", v)):
+        _rows_of(x, name, DT, shape, 2, dev)
+    if g.dim() == 1:
+        _rows_of(g, "g", torch.float32, (heads,), 1, dev)
+    else:
+        _rows_of(g, "g", torch.float32, shape[:-1], 1, dev)
+    if state.dim() != 4 or state.shape[2:] != (C.DK, C.DV):
+        raise ValueError(f"state: expected pages (page, heads per page, {C.DK}, {C.DV}), got {tuple(state.shape)}")
+    _rows_of(state, "state", torch.float32, tuple(state.shape), 3, dev)
+    if layer < 0:
+        raise ValueError(f"layer {layer}: layers count from 0")
+    width = (layer * heads + heads - 1) // state.shape[1] + 1
+    _tables_of(tables, "tables", b, width, dev)
+    if out_tables is not None:
+        _tables_of(out_tables, "out_tables", b, width, dev)
+    if out is None:
+        out = torch.empty(shape, dtype=DT, device=dev)
+    else:
+        _rows_of(out, "out", DT, shape, len(shape), dev)
+    return out, (ptr(state), state.shape[0], 4 * state.stride(0), state.shape[1], layer * heads, ptr(tables),
+                 tables.stride(0), ptr(out_tables), 0 if out_tables is None else out_tables.stride(0))
+
+
+def linear_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor,
+                tables: torch.Tensor, layer: int, *, real: torch.Tensor | None = None,
+                out_tables: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """Linear attention with a decay for each head over q, k, v (b, n, heads, 128): S_t = e^g S_(t-1) + k_t v_t^T,
+    o_t = S_t^T q_t / sqrt(128), each row from its state in the pages `state` (PrefixPool.state; head h of `layer` is
+    flat head layer * heads + h) that its row of tables names. g: log-decays (b, n, heads) fp32, or (heads,), one for
+    each head; -inf forgets. real (b,) int32: row r has real[r] tokens, its outputs past them are zeros. out_tables:
+    the rows' final states are written to these pages (the reserved pages 0 and 1 never are); rows must not share
+    them, nor write pages that another row reads."""
+    if q.dim() != 4:
+        raise ValueError(f"q: expected (rows, tokens, heads, {C.DK}), got {tuple(q.shape)}")
+    b, n, heads = q.shape[:3]
+    o, pool = _linear_of(q, k, v, g, state, tables, layer, out_tables, out)
+    if real is not None:
+        _rows_of(real, "real", torch.int32, (b,), 1, q.device)
+    if scratch is not None:
+        _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), q.device)
+    steps = (0, 0) if g.dim() == 1 else g.stride()[:2]
+    _on(q.device, "jb_linear_scan", ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(v),
+        v.stride(0), v.stride(1), ptr(g), *steps, ptr(real), ptr(o), b, n, heads, *pool, ptr(scratch),
+        0 if scratch is None else scratch.numel())
+    return o
+
+
+def linear_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor,
+                tables: torch.Tensor, layer: int, *, beta: torch.Tensor | None = None,
+                out_tables: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """linear_scan's recurrence for one token per row, q, k, v (b, heads, 128), g (b, heads) or (heads,): o (b, heads,
+    128), the new states written in place, or to out_tables' pages. beta (b, heads) bf16: the gated delta rule of
+    gdn_scan, v replaced by beta (v - (e^g S)^T k)."""
+    if q.dim() != 3:
+        raise ValueError(f"q: expected (rows, heads, {C.DK}), got {tuple(q.shape)}")
+    b, heads = q.shape[:2]
+    o, pool = _linear_of(q, k, v, g, state, tables, layer, tables if out_tables is None else out_tables, out)
+    if beta is not None:
+        _rows_of(beta, "beta", DT, (b, heads), 2, q.device)
+    _on(q.device, "jb_linear_step", ptr(q), q.stride(0), ptr(k), k.stride(0), ptr(v), v.stride(0), ptr(g),
+        0 if g.dim() == 1 else g.stride(0), ptr(beta), ptr(o), b, heads, *pool)
+    return o

@@ -1,0 +1,682 @@
+"""The single-token operators on a B200 against plain implementations in 64 bits: block tables and slot maps, the
+attention input side with several rotary axes, attention of one new token over the paged cache, and linear attention
+with a decay for each head; then a run of them together, as a conversation makes it.
+
+Tolerances: a rounding to bf16 is off by at most half a step, 2^-8 of the value; fp32 arithmetic adds 2^-24 per
+operation of the sum of the terms' magnitudes, counted per test."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from jeff_b200 import constants as C
+from jeff_b200 import kernels
+from jeff_b200.prefix_pool import FAST_PATH_SHAPES, PrefixPool
+
+pytestmark = pytest.mark.gpu
+
+HALF = 2.0 ** -8    # half a bf16 step, relative
+ULP = 2.0 ** -24    # half an fp32 step, relative
+FIXED = FAST_PATH_SHAPES.fixed_pages
+
+
+def gen(seed: int) -> torch.Generator:
+    return torch.Generator("cuda").manual_seed(seed)
+
+
+def normal(g: torch.Generator, *shape: int, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    return torch.randn(*shape, generator=g, device="cuda", dtype=dtype)
+
+
+def i32(values) -> torch.Tensor:
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def close(got: torch.Tensor, want: torch.Tensor, tolerance: torch.Tensor) -> None:
+    off = (got.double() - want).abs() - tolerance
+    assert not torch.isnan(off).any()
+    assert float(off.max()) <= 0, f"off by {float(off.max()):.3g} more than it may be"
+
+
+# ---------------------------------------------------------------- block tables and slot maps
+
+
+def plain_tables(lengths, new, free, tables, kv_entry, tokens, page, fixed):
+    """What block_tables does, one row after the other on the host."""
+    tables = [list(r) for r in tables]
+    width = len(tables[0])
+    slots, rows, positions, starts, taken = [], [], [], [0], [0]
+    at = 0
+    for r, (have, add) in enumerate(zip(lengths, new)):
+        have, add = max(have, 0), max(add, 0)
+
+        def take():
+            nonlocal at
+            at += 1
+            return free[at - 1] if at <= len(free) else 0
+
+        if fixed and have == 0 and add > 0:
+            for e in range(kv_entry):
+                tables[r][e] = take()
+        fresh = {}
+        for j in range(min(-(-have // page), width - kv_entry), min(-(-(have + add) // page), width - kv_entry)):
+            short = at >= len(free)
+            tables[r][kv_entry + j] = take()
+            if short:
+                fresh[j] = True
+        for pos in range(have, have + add):
+            j = pos // page
+            lost = j >= width - kv_entry or j in fresh
+            slots.append(-1 if lost else tables[r][kv_entry + j] * page + pos % page)
+            rows.append(r)
+            positions.append(pos)
+        starts.append(starts[-1] + add)
+        taken.append(at)
+    pad = max(0, tokens - len(slots))
+    return (tables, (slots + [-1] * pad)[:tokens], (rows + [-1] * pad)[:tokens], (positions + [0] * pad)[:tokens],
+            starts, taken)
+
+
+@pytest.mark.parametrize(("lengths", "new", "spare", "entry", "width", "tokens", "page", "fixed"), [
+    ([0], [1], 5, 0, 4, 1, 32, False),                                   # the smallest call
+    ([31, 32, 33, 0, 64], [1, 1, 1, 1, 0], 10, 2, 9, 8, 32, False),      # before, at and past a page's end; a row idle
+    ([0, 5, 0, 0], [40, 3, 0, 64], 30, 3, 8, 120, 32, True),             # fresh rows take their fixed pages too
+    ([7, 0, 100], [70, 200, 1], 3, 1, 12, 300, 32, False),               # the free list runs out
+    ([0, 60], [200, 100], 40, 2, 4, 300, 32, False),                     # rows past their tables
+    ([-4, 3], [2, -7], 9, 1, 6, 5, 16, False),                           # negative counts are zero
+    ([5, 6, 7], [30, 30, 30], 40, 1, 9, 50, 7, True),                    # fewer places than tokens; pages of 7
+    ([3], [4], 0, 1, 5, 9, 4, False),                                    # an empty free list, one page needed
+    ([i * 37 % 500 for i in range(1500)], [i % 4 for i in range(1500)], 900, 5, 30, 2500, 32, True),
+    ([0] * 300, [i % 90 for i in range(300)], 40000, 50, 60, 16384, 32, True),
+    ([2 ** 31 - 1, 0], [5, 2], 4, 1, 3, 9, 32, False),                   # a length at the type's end
+])
+def test_block_tables(lengths, new, spare, entry, width, tokens, page, fixed) -> None:
+    b = len(lengths)
+    filler = [[1000 + 70 * r + e for e in range(width)] for r in range(b)]
+    free = [5 + 3 * i for i in range(spare)]
+    if lengths[0] == 2 ** 31 - 1:
+        new_plain = [0, 2]   # no position past the type's end exists
+    else:
+        new_plain = new
+    want = plain_tables([min(x, 10 ** 6) for x in lengths], new_plain, free, filler, entry, tokens, page, fixed)
+    wide = torch.full((b + 1, width + 3), -7, dtype=torch.int32, device="cuda")   # rows and entries behind: untouched
+    wide[:b, :width] = i32(filler)
+    tables = wide[:, :width]
+    got = kernels.block_tables(i32(lengths), i32(new), i32(free), tables, entry, tokens, page_tokens=page, fixed=fixed)
+    assert tables[:b].tolist() == want[0]
+    assert bool((wide[b] == -7).all()) and bool((wide[:, width:] == -7).all())
+    for name, x in zip(("slots", "rows", "positions", "starts", "taken"), want[1:]):
+        assert getattr(got, name).tolist() == x, name
+
+
+def test_block_tables_give_the_pools_own_order() -> None:
+    """Fresh rows get the tables that PrefixPool.reserve gives them."""
+    counts = [45, 1, 320, 64]
+    pool = PrefixPool(400, "cuda", max_prefix_tokens=512)
+    slots = [pool.reserve(0, f"p{i}", n) for i, n in enumerate(counts)]
+    free = torch.arange(2, 400, dtype=torch.int32, device="cuda")
+    tables = torch.zeros(4, pool.width, dtype=torch.int32, device="cuda")
+    got = kernels.block_tables(i32([0] * 4), i32(counts), free, tables, FIXED, sum(counts), fixed=True)
+    assert torch.equal(tables, pool.tables[torch.tensor(slots, device="cuda")])
+    assert int(got.taken[-1]) == 400 - 2 - pool.free_page_count()
+
+
+# ---------------------------------------------------------------- attention input side
+
+
+def plain_prep(pr, q_w1, k_w1, inv_freq, positions, axis_of):
+    t = pr.shape[0]
+    x = pr[:, :C.ATTN_PROJ].double()
+    q = x[:, :4096].view(t, 8, 512)[:, :, :256]
+    k = x[:, 4096:4608].view(t, 2, 256)
+    angle = positions[axis_of].T.double() * inv_freq.double()
+    c, s = angle.cos()[:, None], angle.sin()[:, None]
+
+    def head(y, w):
+        y = y / torch.sqrt(y.square().mean(-1, keepdim=True) + C.EPS) * w.double()
+        a, b = y[..., :32], y[..., 32:64]
+        return torch.cat([a * c - b * s, b * c + a * s, y[..., 64:]], -1)
+
+    return head(q, q_w1), head(k, k_w1), pr[:, 4608:5120].view(t, 2, 256)
+
+
+@pytest.mark.parametrize(("t", "sections", "interleaved", "reach"), [
+    (1, (32,), False, 5), (3, (11, 11, 10), True, 100), (31, (8, 12, 12), False, 9000),
+    (64, (16, 16), False, 2 ** 31 - 1), (1000, (8, 8, 8, 8), True, 300000), (1217, (0, 32, 0), False, 60),
+])
+def test_attn_prep_axes(t, sections, interleaved, reach) -> None:
+    g = gen(t)
+    wide = normal(g, t, C.ATTN_PROJ + 24)
+    pr = wide[:, :C.ATTN_PROJ + 8]   # a strided input
+    if t > 2:
+        pr[1] = 0                    # a token of zeros
+        pr[2] *= 1e4
+    q_w1, k_w1 = 1 + 0.2 * normal(g, 256, dtype=torch.float32), 1 + 0.2 * normal(g, 256, dtype=torch.float32)
+    inv_freq = 1.0 / (C.ROPE_THETA ** (torch.arange(0, 64, 2, dtype=torch.float32, device="cuda") / 64))
+    positions = torch.randint(-min(reach, 50), reach, (len(sections), t), generator=g, device="cuda").int()
+    axes = kernels.rope_axes(sections, interleaved)
+    of = torch.tensor([axes >> 2 * i & 3 for i in range(32)], device="cuda")
+    q, k, v = plain_prep(pr, q_w1, k_w1, inv_freq, positions, of)
+    pages = -(-t // 32) + 3
+    kv = torch.full((pages, 3, 2, 32, 2, 256), 7.0, dtype=torch.bfloat16, device="cuda")
+    slots = torch.randperm(pages * 32, generator=g, device="cuda")[:t]
+    slots[0] = -1                    # a token that is not kept
+    if t > 4:
+        slots[3], slots[4] = pages * 32, 2 ** 40   # slots past the pool are written nowhere
+    kn, vn = (torch.empty(t, 2, 256, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    got = kernels.attn_prep_axes(pr, q_w1, k_w1, inv_freq, positions, axes, kn=kn, vn=vn, kv=kv, attn_layer=1,
+                                 slots=slots)
+    # the norm: 256 squares summed, a root and two products; the turn: two products and a sum; sine and cosine to 2^-21
+    slack = 32 * ULP * 8
+    for out, want in ((got, q), (kn, k)):
+        top = want.abs().amax(-1, keepdim=True)
+        close(out, want, HALF * want.abs() + slack * top)
+    assert torch.equal(vn, v)
+    want_kv = torch.full_like(kv, 7.0)
+    for i, slot in enumerate(slots.tolist()):
+        if 0 <= slot < pages * 32:
+            want_kv[slot // 32, 1, 0, slot % 32] = kn[i]
+            want_kv[slot // 32, 1, 1, slot % 32] = vn[i]
+    assert torch.equal(kv, want_kv)
+    only = torch.full_like(kv, 7.0)   # the pages alone, and kn and vn alone, give the same
+    q2 = kernels.attn_prep_axes(pr, q_w1, k_w1, inv_freq, positions, axes, kv=only, attn_layer=1, slots=slots)
+    assert torch.equal(only, kv) and torch.equal(q2, got)
+
+
+def test_attn_prep_axes_agrees_with_the_text_form() -> None:
+    """With one axis it is attn_prep_rows up to that one's own rounding points: the norm's result, the sine and cosine,
+    each product and the sum (half a step each, of values up to |a| + |b|)."""
+    g = gen(5)
+    t = 64
+    pr = normal(g, t, C.ATTN_PROJ)
+    w = 1 + 0.1 * normal(g, 256, dtype=torch.float32)
+    inv_freq = 1.0 / (C.ROPE_THETA ** (torch.arange(0, 64, 2, dtype=torch.float32, device="cuda") / 64))
+    kn, vn, kn2, vn2 = (torch.empty(t, 2, 256, dtype=torch.bfloat16, device="cuda") for _ in range(4))
+    rows = kernels.attn_prep_rows(pr, w, w, inv_freq, i32([40, 900]), kn, vn, 32)
+    positions = torch.cat([torch.arange(40, 72), torch.arange(900, 932)]).int().cuda()[None]
+    axes = kernels.attn_prep_axes(pr, w, w, inv_freq, positions, kernels.rope_axes((32,)), kn=kn2, vn=vn2)
+    assert torch.equal(vn, vn2)
+    for a, b in ((rows, axes), (kn, kn2)):
+        x = torch.maximum(a[..., :32].float().abs(), a[..., 32:64].float().abs())
+        size = torch.cat([2 * x, 2 * x, a[..., 64:].float().abs()], -1)
+        close(a, b.double(), 5 * HALF * size + 900 * 2.0 ** -23)
+
+
+def test_attn_prep_axes_refuses() -> None:
+    w = torch.ones(256, device="cuda")
+    f = torch.ones(32, device="cuda")
+    pr = torch.zeros(3, C.ATTN_PROJ, dtype=torch.bfloat16, device="cuda")
+    pos = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    kn = torch.empty(3, 2, 256, dtype=torch.bfloat16, device="cuda")
+    kv = torch.zeros(3, 6, 2, 32, 2, 256, dtype=torch.bfloat16, device="cuda")
+    slots = torch.zeros(3, dtype=torch.int64, device="cuda")
+    call = lambda **kw: kernels.attn_prep_axes(**(dict(pr=pr, q_w1=w, k_w1=w, inv_freq=f, positions=pos,  # noqa: E731
+                                                       axes=kernels.rope_axes((16, 16)), kn=kn, vn=kn.clone()) | kw))
+    for over, says in (({"axes": kernels.rope_axes((11, 11, 10))}, "axis past"), ({"vn": None}, "keys and values"),
+                       ({"kv": kv}, "keys and values"), ({"slots": slots}, "keys and values"),
+                       ({"kv": kv[:, :, :, :16], "slots": slots}, "kv: expected"),
+                       ({"kv": kv, "slots": slots, "attn_layer": 6}, "6 layers"),
+                       ({"kv": kv[..., :128], "slots": slots}, "packed"),
+                       ({"slots": slots.int(), "kv": kv}, "slots: expected"),
+                       ({"positions": pos[:, :2]}, "positions: expected"), ({"q_w1": w[:255]}, "q_w1: expected"),
+                       ({"pr": torch.cat([pr, pr[:, :1]], 1)}, "ldpr 5121")):
+        with pytest.raises(ValueError, match=says):
+            call(**over)
+
+
+# ---------------------------------------------------------------- attention of one new token
+
+
+def cache(g: torch.Generator, lengths: list[int], layers: int, layer: int, kv_heads: int, dim: int, entry: int,
+          extra: int = 0, tail: float = math.nan):
+    """A paged cache of these lengths, its pages in random order; what no token fills holds `tail`."""
+    held = [-(-max(n, 0) // 32) for n in lengths]
+    total = sum(held) + 3
+    kv = torch.full((total, layers, 2, 32, kv_heads, dim), tail, dtype=torch.bfloat16, device="cuda")
+    width = entry + max([*held, 1]) + extra
+    tables = torch.full((len(lengths), width), -1, dtype=torch.int32)
+    order = (torch.randperm(total - 3, generator=torch.Generator().manual_seed(len(lengths))) + 3).tolist()
+    dense = []
+    for r, n in enumerate(lengths):
+        n = max(n, 0)
+        mine = [order.pop() for _ in range(held[r])]
+        tables[r, entry:entry + held[r]] = torch.tensor(mine, dtype=torch.int32)
+        rows = normal(g, 2, n, kv_heads, dim)
+        for j, page in enumerate(mine):
+            part = rows[:, 32 * j:32 * j + 32]
+            kv[page, layer, :, :part.shape[1]] = part
+        dense.append(rows)
+    return kv, tables.cuda(), dense
+
+
+def plain_decode(q, dense, scale, pr=None):
+    """(want, tolerance) in 64 bits. The scores' fp32 error is d + 2 operations on the magnitudes of their terms, and
+    with the exponential's 2^-21 it moves a weight by that much relative to it, numerator and denominator alike; the
+    weights may be held as two bf16 parts (2^-17), and the sums over the keys add an operation for each of 64 partial
+    sums and one for each key that a warp adds."""
+    b, heads, dim = q.shape
+    want, tol = torch.zeros(b, heads, dim, dtype=torch.float64, device="cuda"), torch.zeros(
+        b, heads, dim, dtype=torch.float64, device="cuda")
+    for r, both in enumerate(dense):
+        n = both.shape[1]
+        if n == 0:
+            continue
+        group = heads // both.shape[2]
+        k, v = (x.double().repeat_interleave(group, 1) for x in both)
+        s = torch.einsum("hd,jhd->hj", q[r].double(), k) * scale
+        size = torch.einsum("hd,jhd->hj", q[r].double().abs(), k.abs()) * abs(scale)
+        p = torch.softmax(s, -1)
+        want[r] = torch.einsum("hj,jhd->hd", p, v)
+        moved = (dim + 2) * ULP * size.amax(-1, keepdim=True) + 2.0 ** -21 + 2.0 ** -17 + (64 + n / 4) * ULP
+        tol[r] = 2 * moved * torch.einsum("hj,jhd->hd", p, v.abs())
+    if pr is not None:
+        gate = torch.sigmoid(pr[:, :2 * heads * dim].double().view(b, heads, 2, dim)[:, :, 1])
+        want, tol = want * gate, (tol + 8 * ULP * want.abs()) * gate
+    return want, HALF * want.abs() + tol + 1e-30
+
+
+@pytest.mark.parametrize(("lengths", "heads", "kv_heads", "dim", "gated"), [
+    ([1], 8, 2, 256, True),
+    ([0, 1, 2, 31, 32, 33, 0, 63, 64, 65, 100], 8, 2, 256, True),
+    ([1000], 8, 2, 256, False),
+    ([8192, 5, 777, 0], 8, 2, 256, True),
+    ([300, 17, 1025], 6, 2, 256, True),       # three query heads to a key/value head
+    ([129, 16], 1, 1, 256, False),
+    ([250, 47, 400, 3], 32, 8, 128, False),   # other head layouts
+    ([500, 33], 16, 1, 128, True),            # sixteen query heads to one
+    ([40, 41, 700], 5, 1, 64, False),
+    ([99, 1500], 12, 12, 64, True),
+    ([64] * 200, 8, 2, 256, False),           # more rows than SMs
+    ([1] * 700, 14, 2, 64, True),
+    ([20000], 2, 2, 128, False),
+])
+def test_decode_attention(lengths, heads, kv_heads, dim, gated) -> None:
+    g = gen(sum(lengths) + heads)
+    kv, tables, dense = cache(g, lengths, 3, 1, kv_heads, dim, entry=2)
+    b = len(lengths)
+    q = normal(g, b, heads + 1, dim)[:, :heads]   # rows apart
+    pr = normal(g, b, 2 * heads * dim + 16) if gated else None
+    got = kernels.decode_attention(q, kv, tables, 1, i32(lengths), 2, pr=pr)
+    assert got.shape == ((b, heads * dim) if gated else (b, heads, dim))
+    want, tol = plain_decode(q, dense, dim ** -0.5, pr)
+    close(got.view(b, heads, dim), want, tol)
+    again = kernels.decode_attention(q, kv, tables, 1, i32(lengths), 2, pr=pr)
+    assert torch.equal(got, again)
+
+
+def test_decode_attention_strided_pages_and_outputs() -> None:
+    """A pool's own view (its pages far apart), an output inside a wider tensor, a scale of the caller's."""
+    g = gen(9)
+    lengths = [70, 45, 1, 0]
+    pool = PrefixPool(300, "cuda")
+    dense, slots = [], []
+    for r, n in enumerate(lengths):
+        slots.append(pool.reserve(0, str(r), n))
+        rows = normal(g, 2, n, 2, 256)
+        pages = pool.block_table(slots[-1])[FIXED:]
+        for j, page in enumerate(pages):
+            pool.kv[page, 4] = math.nan
+            part = rows[:, 32 * j:32 * j + 32]
+            pool.kv[page, 4, :, :part.shape[1]] = part
+        dense.append(rows)
+    tables = pool.tables[torch.tensor(slots, device="cuda")]
+    q = normal(g, 4, 8, 256)
+    wide = torch.full((4, 2048 + 32), 3.0, dtype=torch.bfloat16, device="cuda")
+    out = wide[:, 16:2064].unflatten(1, (8, 256))
+    kernels.decode_attention(q, pool.kv, tables, 4, i32(lengths), FIXED, scale=-0.11, out=out)
+    want, tol = plain_decode(q, dense, -0.11)
+    close(out, want, tol)
+    assert bool((wide[:, :16] == 3).all()) and bool((wide[:, 2064:] == 3).all())
+
+
+def test_decode_attention_large_scores() -> None:
+    """Scores of both signs far beyond what an exponential holds, and a single key that takes all."""
+    g = gen(10)
+    lengths = [400, 129]
+    kv, tables, dense = cache(g, lengths, 1, 0, 2, 256, entry=0)
+    q = 64 * normal(g, 2, 8, 256)
+    for x in dense:
+        x[0, 100] = 30.0
+    for r in range(2):
+        kv[tables[r, 3], 0, 0, 4] = 30.0
+    q[0] = q[0].abs()
+    got = kernels.decode_attention(q, kv, tables, 0, i32(lengths), 0)
+    want, tol = plain_decode(q, dense, 1 / 16)
+    close(got, want, tol)
+
+
+def test_decode_attention_bad_pages_and_lengths() -> None:
+    """An entry outside the pool is no page: its tokens are left out. A length past the table's width is cut there,
+    one below zero is none; a row whose pages are all bad is zeros."""
+    g = gen(11)
+    lengths = [200, 128, 96, 64]
+    kv, tables, dense = cache(g, lengths, 2, 0, 2, 256, entry=1)
+    tables[0, 1 + 2] = -3
+    tables[0, 1 + 4] = kv.shape[0]
+    tables[2, 1:] = 2 ** 31 - 1
+    width = 1 + 4
+    narrow = tables[:, :width]
+    q = normal(g, 4, 8, 256)
+    got = kernels.decode_attention(q, kv, narrow, 0, i32([200, 100000, 96, -5]), 1)
+    keep = [j for j in range(128) if not 64 <= j < 96]
+    seen = [dense[0][:, keep], dense[1][:, :128], dense[2][:, :0], dense[3][:, :0]]
+    want, tol = plain_decode(q, seen, 1 / 16)
+    close(got, want, tol)
+    assert not got[2:].any()
+    got = kernels.decode_attention(q, kv, tables, 0, i32(lengths), 1)
+    keep = [j for j in range(200) if not (64 <= j < 96 or 128 <= j < 160)]
+    want, tol = plain_decode(q, [dense[0][:, keep], dense[1], dense[2][:, :0], dense[3]], 1 / 16)
+    close(got, want, tol)
+
+
+def test_decode_attention_far_pages() -> None:
+    """A cache whose bytes pass 32 bits, its last page among those read."""
+    g = gen(12)
+    pages = (1 << 32) // (2 * 2 * 32 * 2 * 256) + 40   # 65,536 bytes a page of one layer: past 4 GB
+    kv = torch.empty(pages, 1, 2, 32, 2, 256, dtype=torch.bfloat16, device="cuda")
+    tables = i32([[pages - 1, 3, pages - 20]])
+    rows = normal(g, 2, 90, 2, 256)
+    for j, page in enumerate(tables[0].tolist()):
+        kv[page, 0] = math.nan
+        part = rows[:, 32 * j:32 * j + 32]
+        kv[page, 0, :, :part.shape[1]] = part
+    q = normal(g, 1, 8, 256)
+    got = kernels.decode_attention(q, kv, tables, 0, i32([90]), 0)
+    close(got, *plain_decode(q, [rows], 1 / 16))
+
+
+# ---------------------------------------------------------------- linear attention
+
+
+def spots(tables: torch.Tensor, layer: int, heads: int, per: int):
+    flat = layer * heads + torch.arange(heads, device="cuda")
+    return tables[:, flat // per].long(), (flat % per).expand(tables.shape[0], -1)
+
+
+def plain_linear(q, k, v, g, begin, real, beta=None):
+    """(o, its terms' magnitudes, state, its terms' magnitudes) token by token in 64 bits."""
+    b, n, heads, d = q.shape
+    o, mag = (torch.zeros(b, n, heads, d, dtype=torch.float64, device="cuda") for _ in range(2))
+    s, m = begin.double(), begin.double().abs()
+    e = torch.exp(g.double()).expand(b, n, heads)
+    for t in range(n):
+        live = (t < real)[:, None, None, None]
+        qt, kt, vt = (x[:, t].double() for x in (q, k, v))
+        s1, m1 = e[:, t, :, None, None] * s, e[:, t, :, None, None] * m
+        va = vt.abs()
+        if beta is not None:
+            bt = beta[:, t].double()[..., None]
+            vt = bt * (vt - torch.einsum("bhij,bhi->bhj", s1, kt))
+            va = bt * (va + torch.einsum("bhij,bhi->bhj", m1, kt.abs()))
+        s = torch.where(live, s1 + kt[..., None] * vt[..., None, :], s)
+        m = torch.where(live, m1 + kt.abs()[..., None] * va[..., None, :], m)
+        o[:, t] = torch.where(live[..., 0], torch.einsum("bhij,bhi->bhj", s, qt) * d ** -0.5, 0.0)
+        mag[:, t] = torch.where(live[..., 0], torch.einsum("bhij,bhi->bhj", m, qt.abs()) * d ** -0.5, 0.0)
+    return o, mag, s, m
+
+
+def linear_case(seed, b, n, heads, per, layer, kind):
+    g = gen(seed)
+    shape = (b, n, heads, 128)
+    q, k = (torch.nn.functional.normalize(normal(g, *shape).float(), dim=-1).bfloat16() for _ in range(2))
+    v = normal(g, *shape)
+    if kind == "heads":
+        decay = -0.5 * torch.rand(heads, generator=g, device="cuda")
+    elif kind == "strong":
+        decay = -30 * torch.rand(b, n, heads, generator=g, device="cuda")
+    elif kind == "none":
+        decay = torch.zeros(b, n, heads, device="cuda")
+    else:
+        decay = -torch.exp(2 * normal(g, b, n, heads, dtype=torch.float32) - 3)
+        if kind == "resets":
+            decay[torch.rand(b, n, heads, generator=g, device="cuda") < 0.05] = -math.inf
+    width = (layer + 1) * heads // per + 3
+    pages = 2 * b * width + 2
+    state = torch.full((pages, per, 128, 128), 5.0, device="cuda")
+    ids = (torch.randperm(pages - 2, generator=g, device="cuda") + 2).int().view(2, b, width)
+    begin = 0.3 * normal(g, b, heads, 128, 128, dtype=torch.float32)
+    page, slot = spots(ids[0], layer, heads, per)
+    state[page, slot] = begin
+    return q, k, v, decay, state, ids[0], ids[1], begin
+
+
+SCANS = [
+    (1, 1, 16, 6, 0, "mixed", None), (2, 2, 16, 6, 17, "mixed", None), (3, 63, 16, 6, 3, "mixed", (63, 1, 0)),
+    (2, 64, 16, 6, 5, "resets", (64, 33)), (2, 65, 4, 4, 1, "heads", (65, 64)), (3, 127, 5, 2, 0, "strong", None),
+    (2, 128, 16, 6, 2, "none", (128, 127)), (2, 129, 16, 6, 9, "resets", (129, 128)), (1, 300, 3, 1, 0, "mixed", None),
+    (4, 257, 16, 6, 1, "mixed", (257, 0, 130, 256)), (1, 1000, 16, 6, 4, "heads", None), (20, 96, 16, 6, 0, "heads", None),
+    (1, 1024, 2, 6, 0, "none", None), (2, 700, 1, 1, 3, "resets", (699, 700)),
+]
+
+
+@pytest.mark.parametrize(("b", "n", "heads", "per", "layer", "kind", "real"), SCANS)
+def test_linear_scan(b, n, heads, per, layer, kind, real) -> None:
+    q, k, v, g, state, tables, outs, begin = linear_case(b * 1000 + n, b, n, heads, per, layer, kind)
+    lengths = i32(list(real) if real else [n] * b)
+    before = state.clone()
+    got = kernels.linear_scan(q, k, v, g, state, tables, layer, real=lengths if real else None, out_tables=outs)
+    o, mag, s, m = plain_linear(q, k, v, g, begin, lengths)
+    # a chunked form may round the probabilities and the state to bf16 ahead of their products (half a step of each
+    # term) and the result once more; its sums add 128 terms a chunk and one a chunk
+    close(got, o, HALF * o.abs() + (HALF + 2.0 ** -13) * mag)
+    page, slot = spots(outs, layer, heads, per)
+    ends = state[page, slot]
+    # the state's terms: three bf16 parts of a decayed key (2^-24 of it), a decay factor to 2^-21, the sums
+    close(ends, s, (2.0 ** -20 + (n / 4 + 64) * ULP) * m + 1e-30)
+    assert float((ends.double() - s).norm()) <= 2.0 ** -19 * float(s.norm())
+    before[page, slot] = ends
+    assert torch.equal(state, before)   # nothing else is written
+    for r, count in enumerate(lengths.tolist()):
+        assert not got[r, count:].any()
+    again = kernels.linear_scan(q, k, v, g, state, tables, layer, real=lengths if real else None)
+    assert torch.equal(got, again) and torch.equal(state, before)
+
+
+def test_linear_scan_strided_inputs_in_place() -> None:
+    """q, k and v as parts of one projection, the decays as part of a wider tensor, the states updated in place."""
+    b, n, heads = 2, 150, 16
+    q, k, v, g, state, tables, _, begin = linear_case(7, b, n, heads, 6, 2, "mixed")
+    wide = torch.cat([x.flatten(2) for x in (q, k, v)] + [q[..., 0, :24]], 2)
+    parts = [wide[..., 2048 * i:2048 * i + 2048].unflatten(2, (16, 128)) for i in range(3)]
+    gates = torch.cat([g, g + 1], 2)[..., :16]
+    got = kernels.linear_scan(*parts, gates, state, tables, 2, out_tables=tables)
+    o, mag, s, m = plain_linear(q, k, v, g, begin, i32([n] * b))
+    close(got, o, HALF * o.abs() + (HALF + 2.0 ** -13) * mag)
+    page, slot = spots(tables, 2, heads, 6)
+    close(state[page, slot], s, (2.0 ** -20 + (n / 4 + 64) * ULP) * m + 1e-30)
+
+
+def test_linear_scan_long_prompt_continues() -> None:
+    """One long prompt at once gives what its two halves give one after the other (the tolerances of both)."""
+    b, n, heads = 1, 4099, 16
+    q, k, v, g, state, tables, outs, begin = linear_case(8, b, n, heads, 6, 1, "mixed")
+    whole = kernels.linear_scan(q, k, v, g, state, tables, 1, out_tables=outs)
+    page, slot = spots(outs, 1, heads, 6)
+    end = state[page, slot].clone()
+    cut = 2050
+    one = kernels.linear_scan(q[:, :cut], k[:, :cut], v[:, :cut], g[:, :cut], state, tables, 1, out_tables=outs)
+    two = kernels.linear_scan(q[:, cut:], k[:, cut:], v[:, cut:], g[:, cut:], state, outs, 1, out_tables=outs)
+    o, mag, s, m = plain_linear(q, k, v, g, begin, i32([n]))
+    both = torch.cat([one, two], 1)
+    for got in (whole, both):
+        close(got, o, HALF * o.abs() + (HALF + 2.0 ** -13) * mag)
+    for got in (end, state[page, slot]):
+        close(got, s, (2.0 ** -20 + (n / 4 + 64) * ULP) * m + 1e-30)
+
+
+def test_linear_bad_pages() -> None:
+    """An entry outside the pool reads as zeros and is not written; the reserved pages are never written."""
+    q, k, v, g, state, tables, outs, begin = linear_case(9, 3, 40, 6, 6, 0, "mixed")
+    tables[0, 0] = -1
+    tables[1, 0] = state.shape[0]
+    outs[0, 0], outs[1, 0], outs[2, 0] = 1, 2 ** 31 - 1, 0
+    before = state.clone()
+    begin[:2] = 0
+    got = kernels.linear_scan(q, k, v, g, state, tables, 0, out_tables=outs)
+    o, mag, _, _ = plain_linear(q, k, v, g, begin, i32([40] * 3))
+    close(got, o, HALF * o.abs() + (HALF + 2.0 ** -13) * mag)
+    assert torch.equal(state, before)
+    first = kernels.linear_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], state, tables, 0, out_tables=outs)
+    close(first, o[:, 0], HALF * o[:, 0].abs() + (HALF + 2.0 ** -13) * mag[:, 0])
+    assert torch.equal(state, before)
+
+
+@pytest.mark.parametrize("delta", [False, True])
+@pytest.mark.parametrize(("b", "heads", "per", "layer", "kind"), [
+    (1, 16, 6, 0, "mixed"), (5, 16, 6, 17, "mixed"), (3, 5, 2, 1, "resets"), (64, 16, 6, 3, "heads"),
+    (2, 1, 1, 4, "strong"), (40, 3, 4, 2, "none"),
+])
+def test_linear_step(b, heads, per, layer, kind, delta) -> None:
+    q, k, v, g, state, tables, outs, begin = linear_case(b + 50, b, 1, heads, per, layer, kind)
+    beta = torch.sigmoid(normal(gen(b), b, 1, heads, dtype=torch.float32)).bfloat16() if delta else None
+    o, mag, s, m = plain_linear(q, k, v, g, begin, i32([1] * b), beta)
+    page, slot = spots(tables, layer, heads, per)
+    opage, oslot = spots(outs, layer, heads, per)
+    one = g if g.dim() == 1 else g[:, 0]
+    for target in (outs, None):
+        before = state.clone()
+        got = kernels.linear_step(q[:, 0], k[:, 0], v[:, 0], one, state, tables, layer,
+                                  beta=None if beta is None else beta[:, 0], out_tables=target)
+        # two sums of 128 terms (three with beta), a decay factor to 2^-22
+        close(got, o[:, 0], HALF * o[:, 0].abs() + (300 * ULP + 2.0 ** -21) * mag[:, 0])
+        at = (opage, oslot) if target is not None else (page, slot)
+        close(state[at], s, (140 * ULP + 2.0 ** -21) * m + 1e-30)
+        before[at] = state[at]
+        assert torch.equal(state, before)
+
+
+def test_linear_refusals() -> None:
+    q, k, v, g, state, tables, outs, _ = linear_case(3, 2, 8, 16, 6, 0, "mixed")
+    for over, says in (({"k": k[:, :7]}, "k: expected"), ({"v": v.float()}, "v: expected"),
+                       ({"g": g[..., :15]}, "g: expected"), ({"g": g.bfloat16()}, "g: expected"),
+                       ({"state": state[..., :64]}, "state: expected"), ({"layer": -1}, "layer -1"),
+                       ({"layer": 1}, "tables: expected"), ({"tables": tables[:1]}, "tables: expected"),
+                       ({"out_tables": outs.long()}, "out_tables: expected"),
+                       ({"real": i32([1, 2, 3])}, "real: expected"),
+                       ({"out": torch.empty(2, 8, 2048, device="cuda")}, "out: expected"),
+                       ({"q": q.transpose(2, 3).contiguous().transpose(2, 3)}, "packed")):
+        with pytest.raises(ValueError, match=says):
+            kernels.linear_scan(**(dict(q=q, k=k, v=v, g=g, state=state, tables=tables[:, :4], layer=0) | over))
+    with pytest.raises(ValueError, match="beta: expected"):
+        kernels.linear_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], state, tables, 0, beta=g[:, 0])
+
+
+# ---------------------------------------------------------------- together
+
+
+def test_a_conversation() -> None:
+    """Three requests of mixed lengths: block tables for their prompts, the prompts' keys and values into the pages and
+    their recurrent states, then tokens one by one: new slots, the token's keys and values, its attention over the whole
+    cache and its step of the recurrent state. The steps run once eagerly and once as one captured graph replayed, with
+    the same bits, each step's outputs against 64 bits. A fourth row is idle throughout."""
+    g = gen(77)
+    pool = PrefixPool(500, "cuda", max_prefix_tokens=256)
+    b, prompts, steps, attn, lin = 4, [45, 31, 96, 0], 4, 2, 7
+    free = torch.arange(2, 500, dtype=torch.int32, device="cuda")
+    tables = torch.zeros(b, pool.width, dtype=torch.int32, device="cuda")
+    fill = sum(prompts) + 5
+    m = kernels.block_tables(i32([0] * b), i32(prompts), free, tables, FIXED, fill, fixed=True)
+    left = free[int(m.taken[-1]):]
+    w = torch.ones(256, device="cuda")
+    inv_freq = 1.0 / (C.ROPE_THETA ** (torch.arange(0, 64, 2, dtype=torch.float32, device="cuda") / 64))
+    axes = kernels.rope_axes((11, 11, 10), True)
+    pool.kv[2:] = math.nan   # what nothing has written; the reserved page of zeros stays
+
+    pr = normal(g, fill, C.ATTN_PROJ)
+    kn, vn = (torch.empty(fill, 2, 256, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    kernels.attn_prep_axes(pr, w, w, inv_freq, m.positions.expand(3, -1).contiguous(), axes, kn=kn, vn=vn, kv=pool.kv,
+                           attn_layer=attn, slots=m.slots)
+    bounds = m.starts.tolist()
+    dense = [torch.stack([kn[bounds[r]:bounds[r + 1]], vn[bounds[r]:bounds[r + 1]]]) for r in range(b)]
+
+    n = max(prompts) + steps
+    q, k = (torch.nn.functional.normalize(normal(g, b, n, 16, 128).float(), dim=-1).bfloat16() for _ in range(2))
+    v, decay = normal(g, b, n, 16, 128), -0.2 * torch.rand(b, n, 16, generator=g, device="cuda")
+    zeros = torch.ones(b, pool.width, dtype=torch.int32, device="cuda")   # the empty prefix: the page of zeros
+    real = i32(prompts)
+    page, slot = spots(tables, lin, 16, 6)
+    kernels.linear_scan(q[:, :96], k[:, :96], v[:, :96], decay[:, :96], pool.state, zeros, lin, real=real,
+                        out_tables=tables)
+    o, mag, _, _ = plain_linear(*(torch.stack([torch.cat([x[r, :prompts[r]], x[r, 96:], x[r, prompts[r]:96]])
+                                               for r in range(b)]) for x in (q, k, v, decay)),
+                                torch.zeros(b, 16, 128, 128, device="cuda"), i32([p + steps if p else 0 for p in prompts]))
+
+    new = i32([1, 1, 1, 0])
+    lengths, held = i32(prompts), left.clone()
+    step_pr = normal(g, steps, b, C.ATTN_PROJ)
+    x = {"pr": step_pr[0].clone(), "q": q[:, 96].clone(), "k": k[:, 96].clone(), "v": v[:, 96].clone(),
+         "g": decay[:, 96].clone()}
+    start = (lengths.clone(), tables.clone(), pool.data.clone(), held.clone())
+
+    def step():
+        mm = kernels.block_tables(lengths, new, held, tables, FIXED, b)
+        # the rows' tokens are packed in row order and the idle row is the last: token i is row i's
+        aq = kernels.attn_prep_axes(x["pr"], w, w, inv_freq, mm.positions.expand(3, -1).contiguous(), axes,
+                                    kv=pool.kv, attn_layer=attn, slots=mm.slots)
+        lengths.add_(new)
+        y = kernels.decode_attention(aq, pool.kv, tables, attn, lengths, FIXED, pr=x["pr"])
+        lo = kernels.linear_step(x["q"], x["k"], x["v"], x["g"], pool.state, tables, lin)
+        # the pages taken leave the front of the free list
+        held.copy_(held[(torch.arange(len(held), device="cuda") + mm.taken[-1]) % len(held)])
+        return aq, y, lo
+
+    def reset():
+        for target, source in zip((lengths, tables, pool.data, held), start):
+            target.copy_(source)
+
+    eager = []
+    for t in range(steps):
+        for name, source in (("pr", step_pr[t]), ("q", q[:, 96 + t]), ("k", k[:, 96 + t]), ("v", v[:, 96 + t]),
+                             ("g", decay[:, 96 + t])):
+            x[name].copy_(source)
+        aq, y, lo = step()
+        eager.append((aq, y, lo))
+        for r in range(3):
+            assert int(lengths[r]) == prompts[r] + t + 1
+            last = int(lengths[r]) - 1
+            mine = pool.kv[int(tables[r, FIXED + last // 32]), attn, :, last % 32]
+            dense[r] = torch.cat([dense[r], mine[:, None]], 1)
+        want, tol = plain_decode(aq, dense, 1 / 16, x["pr"])
+        close(y.view(b, 8, 256), want, tol)
+        for r in range(3):
+            i = prompts[r] + t
+            close(lo[r], o[r, i], HALF * o[r, i].abs() + 2.0 ** -13 * mag[r, i])
+    reset()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    reset()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    reset()
+    for t in range(steps):
+        for name, source in (("pr", step_pr[t]), ("q", q[:, 96 + t]), ("k", k[:, 96 + t]), ("v", v[:, 96 + t]),
+                             ("g", decay[:, 96 + t])):
+            x[name].copy_(source)
+        graph.replay()
+        for a, e in zip(outs, eager[t]):
+            assert torch.equal(a[:3], e[:3])
+
+
+def test_on_a_stream_of_its_own() -> None:
+    """Work on two streams at once, each with its own inputs, gives what one stream gives."""
+    g = gen(21)
+    lengths = [900, 64, 300]
+    kv, tables, _ = cache(g, lengths, 1, 0, 2, 256, entry=0)
+    cases = [normal(g, 3, 8, 256) for _ in range(8)]
+    want = [kernels.decode_attention(q, kv, tables, 0, i32(lengths), 0) for q in cases]
+    n = i32(lengths)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i, q in enumerate(cases):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(kernels.decode_attention(q, kv, tables, 0, n, 0))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
