@@ -240,64 +240,434 @@ __global__ void __launch_bounds__(384) prep_axes_kernel(const PrepParams p) {
 
 // ------------------------------------------------------------------ attention of one new token per row
 //
-// o = sum_j softmax_j(scale q . k_j) v_j over the row's cached tokens j < lengths[r], one pass with the running
-// maximum and sum. CTA per (row, query head), a warp per key, fp32 throughout.
+// o = sum_j softmax_j(scale q . k_j) v_j over the row's cached tokens j < lengths[r], in one pass over the pages with
+// a running maximum and sum. Every key and value is read once, for all query heads of its head: 4 operations a byte
+// with 4 of them, so the bound is HBM.
+//
+// Shares: a (row, key/value head) is cut into steps of WARPS x 16 tokens, all steps of the call into as many equal
+// shares as there are CTAs (one per SM), in row order: a share's work does not depend on how the lengths are spread. A
+// CTA finishes what it holds in full; of a row cut by a share's border each part leaves its unnormalised sum, maximum
+// and weight in scratch, and join_kernel adds a row's parts in order.
+//
+// In a CTA each warp takes one 16-token tile of a step, with a ring of its own in shared memory (cp.async, rows past the
+// end filled with zeros) and no barrier with the other warps until a row ends, when the warps' sums are joined in
+// shared memory. Scores and output are taken transposed, S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16: the 16
+// rows of the tile are keys (then 16 of the head's dimensions), the 8 columns the query heads, so 4 query heads cost
+// half of what a 16-row query tile would. (tcgen05 has no use here: its 128-row tile would be filled with 4 rows.)
+// The weights are held as two bf16 parts, p = hi + lo to 2^-17: with at most 4 query heads the lo parts ride in
+// columns 4-7, which would be empty, against the queries repeated there; with more they take a second product.
 
 template <int D>
-__global__ void __launch_bounds__(256) decode_plain_kernel(
-    const __nv_bfloat16* __restrict__ q, int64_t ldq, const uint8_t* __restrict__ kv, int64_t pages,
-    int64_t page_bytes, const int* __restrict__ tables, int table_stride, int width, int kv_entry,
-    const int* __restrict__ lengths, int nq, int nkv, float scale_log2, const __nv_bfloat16* __restrict__ pr,
-    int64_t ldpr, __nv_bfloat16* __restrict__ y, int64_t ldy) {
+struct Dec {
+  static constexpr int WARPS = D == 256 ? 4 : 8;
+  static constexpr int STAGES = D == 64 ? 5 : 3;
+  static constexpr int STEP = WARPS * 16;         // tokens
+  static constexpr int PITCH = D * 2 + 16;        // bytes of a key in shared memory: ldmatrix without conflicts
+  static constexpr int SLOT = 2 * 16 * PITCH;     // a tile's keys, then its values; a warp's output at a row's end
+  static constexpr int SMEM = WARPS * STAGES * SLOT;
+  static constexpr int OPITCH = D + 8;            // floats of a head's output there
+  static_assert(16 * OPITCH * 4 <= SLOT, "sixteen heads' outputs fit a slot");
+  static_assert(SMEM + 4096 <= 227 * 1024, "shared memory");
+};
+
+constexpr int SHARES = 148;   // one CTA per SM
+
+struct DecParams {
+  const __nv_bfloat16* q;
+  int64_t ldq;
+  const uint8_t* kv;   // the layer's keys in page 0
+  int64_t pages, page_bytes;
+  const int* tables;
+  int table_stride, kv_entry, most;   // tokens the table holds
+  const int* lengths;
+  int b, kv_heads, group, dim;
+  float scale_log2;
+  const __nv_bfloat16* pr;
+  int64_t ldpr;
+  __nv_bfloat16* y;
+  int64_t ldy;
+  float* scratch;
+};
+
+__device__ __forceinline__ int dec_length(const DecParams& p, int r) { return min(max(p.lengths[r], 0), p.most); }
+
+// Units (steps of one key/value head) of the rows before `row`, and with row = b of all; warp-collective.
+template <int STEP>
+__device__ long long dec_units_before(const DecParams& p, int row) {
+  const int lane = threadIdx.x & 31;
+  long long sum = 0;
+  for (int r0 = 0; r0 < row; r0 += 128) {
+    int n[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + 32 * i + lane;
+      n[i] = r < row ? dec_length(p, r) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += (n[i] + STEP - 1) / STEP;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum * p.kv_heads;
+}
+
+struct Cursor {   // a unit: a step of a row's head
+  int row, head, step, steps;
+};
+
+// The unit `u` (below the total); warp-collective.
+template <int STEP>
+__device__ Cursor dec_find(const DecParams& p, long long u) {
+  const int lane = threadIdx.x & 31;
+  long long before = 0;
+  for (int r0 = 0; r0 < p.b; r0 += 32) {
+    const int steps = r0 + lane < p.b ? (dec_length(p, r0 + lane) + STEP - 1) / STEP : 0;
+    long long upto = (long long)steps * p.kv_heads;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    upto += before;
+    const unsigned over = __ballot_sync(0xffffffffu, upto > u);
+    if (over) {
+      const int l = __ffs(over) - 1;
+      const int n = __shfl_sync(0xffffffffu, steps, l);
+      const long long in = u - (__shfl_sync(0xffffffffu, upto, l) - (long long)n * p.kv_heads);
+      return {r0 + l, (int)(in / n), (int)(in % n), n};
+    }
+    before = __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return {p.b, 0, 0, 0};
+}
+
+template <int STEP>
+__device__ __forceinline__ void dec_next(const DecParams& p, Cursor& c) {
+  if (++c.step < c.steps) return;
+  c.step = 0;
+  if (++c.head < p.kv_heads) return;
+  c.head = 0;
+  do {
+    ++c.row;
+    c.steps = c.row < p.b ? (dec_length(p, c.row) + STEP - 1) / STEP : 1;
+  } while (c.steps == 0);
+}
+
+// the base of the exponentials while every score so far is -inf (their weights are then 0, not NaN)
+__device__ __forceinline__ float finite(float m) { return m == -INFINITY ? 0.f : m; }
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// NT: 8-column tiles of query heads; PAIR: at most 4 query heads, the weights' lo parts in columns 4-7
+template <int D, int NT, bool PAIR>
+__global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const DecParams p) {
   pdl_begin();
-  constexpr int E = D / 32;
-  __shared__ float sm[8], sl[8], so[8][D];
-  const int r = blockIdx.x / nq, h = blockIdx.x % nq, g = h / (nq / nkv);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int len = (int)min((long long)max(lengths[r], 0), (long long)(width - kv_entry) * PAGE);
-  float qv[E], o[E], m = -INFINITY, l = 0.f;
+  using L = Dec<D>;
+  constexpr int KS = D / 16, CH = D / 8;   // 16-wide k steps, 16-byte chunks of a key
+  extern __shared__ __align__(16) uint8_t sm[];
+  __shared__ float s_m[L::WARPS][16], s_l[L::WARPS][16];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, tq = lane & 3;
+  const long long total = dec_units_before<L::STEP>(p, p.b);
+  const long long shares = min((long long)SHARES, total);   // none of them empty
+  if (blockIdx.x >= shares) return;
+  const long long u0 = total * blockIdx.x / shares, u1 = total * (blockIdx.x + 1) / shares;
+  uint8_t* ring = sm + warp * L::STAGES * L::SLOT;
+  Cursor c = dec_find<L::STEP>(p, u0), f = c;
+  const int half_bytes = PAGE * p.kv_heads * D * 2;   // a page's keys of one layer, then its values
+
+  auto page_of = [&](const Cursor& x) -> int {   // the page of this warp's tile of a unit, -1: none
+    const int j = x.step * L::STEP + warp * 16;
+    if (x.row >= p.b || j >= dec_length(p, x.row)) return -1;
+    const int page = p.tables[(int64_t)x.row * p.table_stride + p.kv_entry + j / PAGE];
+    return page >= 0 && page < p.pages ? page : -1;
+  };
+  auto fetch = [&](const Cursor& x, int page, int slot) {
+    if (page >= 0) {
+      const int j0 = x.step * L::STEP + warp * 16;
+      const int live = min(16, dec_length(p, x.row) - j0);
+      const uint8_t* src = p.kv + (int64_t)page * p.page_bytes + ((j0 % PAGE) * p.kv_heads + x.head) * D * 2;
+      const uint32_t dst = smem_u32(ring + slot * L::SLOT);
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    qv[e] = bf2f(q[r * ldq + (int64_t)h * D + lane + 32 * e]);
-    o[e] = 0.f;
-  }
-  for (int j = warp; j < len; j += 8) {
-    const int page = tables[(int64_t)r * table_stride + kv_entry + j / PAGE];
-    if (page < 0 || page >= pages) continue;
-    const __nv_bfloat16* k = reinterpret_cast<const __nv_bfloat16*>(kv + page * page_bytes) +
-                             ((int64_t)(j % PAGE) * nkv + g) * D;
-    const __nv_bfloat16* v = k + (int64_t)PAGE * nkv * D;
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s += qv[e] * bf2f(k[lane + 32 * e]);
-    s = ew::warp_sum(s) * scale_log2;
-    const float mn = fmaxf(m, s), a = m == -INFINITY ? 0.f : exp2f(m - mn), w = exp2f(s - mn);
-    l = l * a + w;
-    m = mn;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * a + w * bf2f(v[lane + 32 * e]);
-  }
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) so[warp][lane + 32 * e] = o[e];
-  __syncthreads();
-  if (threadIdx.x < D) {
-    float mx = -INFINITY;
-    for (int w = 0; w < 8; ++w) mx = fmaxf(mx, sm[w]);
-    float sum = 0.f, out = 0.f;
-    if (mx != -INFINITY)
-      for (int w = 0; w < 8; ++w) {
-        const float a = exp2f(sm[w] - mx);
-        sum += a * sl[w];
-        out += a * so[w][threadIdx.x];
+      for (int i = 0; i < CH; ++i) {   // 32 keys and values x CH chunks: consecutive lanes along a row
+        const int idx = i * 32 + lane, r = idx / CH, ch = idx % CH;   // row 0-15 of the keys, 16-31 of the values
+        const int key = r & 15;
+        const uint8_t* s = src + (int64_t)(r >> 4) * half_bytes + key * (p.kv_heads * D * 2) + ch * 16;
+        attn::cp_async16(dst + r * L::PITCH + ch * 16, key < live ? s : p.kv, key < live);
       }
-    out = sum > 0.f ? out / sum : 0.f;
-    if (pr) out *= ew::sigmoid(bf2f(pr[r * ldpr + ((int64_t)2 * h + 1) * D + threadIdx.x]));
-    y[r * ldy + (int64_t)h * D + threadIdx.x] = f2bf(out);
+    }
+    attn::cp_async_commit();
+  };
+
+  // the ring's first tiles; `page` runs one tile ahead of the fetches, so that its load never stands in their way
+  long long uf = u0;   // the next unit to fetch
+  int page = page_of(f);
+  int pages_in[L::STAGES];
+#pragma unroll
+  for (int s = 0; s < L::STAGES; ++s) {
+    pages_in[s] = uf < u1 ? page : -1;
+    fetch(f, pages_in[s], s);
+    ++uf;
+    if (uf < u1) {
+      dec_next<L::STEP>(p, f);
+      page = page_of(f);
+    }
   }
+
+  uint32_t qf[NT][KS][2];
+  float o[NT][KS][4], m[NT][2], l[NT][2];
+  auto begin = [&]() {   // a row's head: its queries as B fragments, empty sums
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int h = PAIR ? (gr & 3) : nt * 8 + gr;
+      const bool live = h < p.group;
+      const __nv_bfloat16* src = p.q + c.row * p.ldq + ((int64_t)c.head * p.group + (live ? h : 0)) * D + 2 * tq;
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) {
+        qf[nt][kk][0] = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16) : 0u;
+        qf[nt][kk][1] = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8) : 0u;
+        o[nt][kk][0] = o[nt][kk][1] = o[nt][kk][2] = o[nt][kk][3] = 0.f;
+      }
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+  };
+  begin();
+  int slot = 0;
+  bool from_start = true;   // the current row's head began at the share's first unit
+  int first_step = c.step;
+  for (long long u = u0; u < u1; ++u) {
+    attn::cp_async_wait<L::STAGES - 1>();
+    __syncwarp();
+    int mine = -1;
+#pragma unroll
+    for (int s = 0; s < L::STAGES; ++s)
+      if (s == slot) mine = pages_in[s];
+    uint8_t* tile = ring + slot * L::SLOT;
+    if (mine >= 0) {
+      const int j0 = c.step * L::STEP + warp * 16;
+      const int live = dec_length(p, c.row) - j0;
+      // S^T: 16 keys x 8 heads, four chains of products
+      float s[NT][4][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[nt][i][0] = s[nt][i][1] = s[nt][i][2] = s[nt][i][3] = 0.f;
+      const uint32_t ka = smem_u32(tile) + ((lane & 7) + (lane & 8)) * L::PITCH + (lane >> 4) * 16;
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) {
+        uint32_t a0, a1, a2, a3;
+        attn::ldsm_x4(ka + kk * 32, a0, a1, a2, a3);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) attn::mma16816(s[nt][kk & 3], a0, a1, a2, a3, qf[nt][kk][0], qf[nt][kk][1]);
+      }
+      uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = ((s[nt][0][e] + s[nt][1][e]) + (s[nt][2][e] + s[nt][3][e])) * p.scale_log2;
+          if (gr + (e >> 1) * 8 >= live) x[e] = -INFINITY;
+        }
+        float n0 = fmaxf(x[0], x[2]), n1 = fmaxf(x[1], x[3]);
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, off));
+          n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, off));
+        }
+        if (__any_sync(0xffffffffu, n0 > m[nt][0] || n1 > m[nt][1])) {
+          n0 = fmaxf(n0, m[nt][0]);
+          n1 = fmaxf(n1, m[nt][1]);
+          const float a0 = exp2f(m[nt][0] - finite(n0)), a1 = exp2f(m[nt][1] - finite(n1));
+          m[nt][0] = n0;
+          m[nt][1] = n1;
+          l[nt][0] *= a0;
+          l[nt][1] *= a1;
+#pragma unroll
+          for (int kk = 0; kk < KS; ++kk) {
+            o[nt][kk][0] *= a0;
+            o[nt][kk][1] *= a1;
+            o[nt][kk][2] *= a0;
+            o[nt][kk][3] *= a1;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = exp2f(x[e] - finite(m[nt][e & 1]));
+          l[nt][e & 1] += x[e];
+        }
+#pragma unroll
+        for (int e2 = 0; e2 < 2; ++e2) {
+          const uint32_t h = pack_bf2(x[2 * e2], x[2 * e2 + 1]);
+          const uint32_t r = pack_bf2(x[2 * e2] - bf_lo(h), x[2 * e2 + 1] - bf_hi(h));
+          if (PAIR) hi[nt][e2] = transpose8x8(tq < 2 ? h : r);
+          else {
+            hi[nt][e2] = transpose8x8(h);
+            lo[nt][e2] = transpose8x8(r);
+          }
+        }
+      }
+      // O^T += V^T P^T, 16 dimensions at a time
+      const uint32_t va =
+          smem_u32(tile) + 16 * L::PITCH + ((lane & 7) + ((lane >> 4) << 3)) * L::PITCH + ((lane >> 3) & 1) * 16;
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) {
+        uint32_t a0, a1, a2, a3;
+        attn::ldsm_x4_trans(va + kk * 32, a0, a1, a2, a3);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          attn::mma16816(o[nt][kk], a0, a1, a2, a3, hi[nt][0], hi[nt][1]);
+          if (!PAIR) attn::mma16816(o[nt][kk], a0, a1, a2, a3, lo[nt][0], lo[nt][1]);
+        }
+      }
+    }
+    __syncwarp();
+    const bool ends = c.step + 1 == c.steps || u + 1 == u1;
+    if (ends) {
+      // the warps' sums into the slots just read, then joined: thread = one dimension of a head
+      float* mo = reinterpret_cast<float*>(tile);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
+        }
+        const int h = nt * 8 + 2 * tq;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v = o[nt][kk][e];
+            if (PAIR) v += __shfl_xor_sync(0xffffffffu, v, 2);   // the lo parts' product
+            if (!PAIR || tq < 2) mo[(h + (e & 1)) * L::OPITCH + kk * 16 + gr + (e >> 1) * 8] = v;
+          }
+        }
+        if (gr == 0) {
+          s_m[warp][h] = m[nt][0];
+          s_m[warp][h + 1] = m[nt][1];
+          s_l[warp][h] = l[nt][0];
+          s_l[warp][h + 1] = l[nt][1];
+        }
+      }
+      __syncthreads();
+      const bool whole = first_step == 0 && c.step + 1 == c.steps;
+      float* part = p.scratch + (2 * (int64_t)blockIdx.x + (from_start ? 0 : 1)) * p.group * (D + 2);
+      for (int i = threadIdx.x; i < p.group * D; i += L::WARPS * 32) {
+        const int h = i / D, d = i % D;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < L::WARPS; ++w) mx = fmaxf(mx, s_m[w][h]);
+        float sum = 0.f, v = 0.f;
+#pragma unroll
+        for (int w = 0; w < L::WARPS; ++w) {
+          if (s_m[w][h] == -INFINITY && s_l[w][h] == 0.f) continue;   // a warp without keys of this row
+          const float a = exp2f(s_m[w][h] - finite(mx));
+          sum += a * s_l[w][h];
+          v += a * reinterpret_cast<const float*>(sm + (w * L::STAGES + slot) * L::SLOT)[h * L::OPITCH + d];
+        }
+        if (whole) {
+          const int head = c.head * p.group + h;
+          v = mx == -INFINITY && sum == 0.f ? 0.f : v / sum;
+          if (p.pr) v *= ew::sigmoid(bf2f(p.pr[c.row * p.ldpr + ((int64_t)2 * head + 1) * D + d]));
+          p.y[c.row * p.ldy + (int64_t)head * D + d] = f2bf(v);
+        } else {
+          part[h * (D + 2) + 2 + d] = v;
+          if (d == 0) {
+            part[h * (D + 2)] = mx;
+            part[h * (D + 2) + 1] = sum;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    // the slot is free: the tile STAGES units on
+#pragma unroll
+    for (int s = 0; s < L::STAGES; ++s)
+      if (s == slot) pages_in[s] = uf < u1 ? page : -1;
+    fetch(f, uf < u1 ? page : -1, slot);
+    ++uf;
+    if (uf < u1) {
+      dec_next<L::STEP>(p, f);
+      page = page_of(f);
+    }
+    slot = slot + 1 == L::STAGES ? 0 : slot + 1;
+    if (u + 1 < u1) {
+      dec_next<L::STEP>(p, c);
+      if (ends) {
+        begin();
+        from_start = false;
+        first_step = 0;
+      }
+    }
+  }
+}
+
+// CTA per (row, query head), thread = dimension: the parts of a row that shares cut, in share order; rows without
+// tokens are zeros; nothing to do for a row that one share held in full.
+template <int D>
+__global__ void __launch_bounds__(D) join_kernel(const DecParams p) {
+  pdl_begin();
+  constexpr int STEP = Dec<D>::STEP;
+  const int heads = p.kv_heads * p.group;
+  const int row = blockIdx.x / heads, head = blockIdx.x % heads, g = head / p.group, h = head % p.group;
+  const int d = threadIdx.x;
+  const int steps = (dec_length(p, row) + STEP - 1) / STEP;
+  __nv_bfloat16* y = p.y + row * p.ldy + (int64_t)head * D + d;
+  if (steps == 0) {
+    *y = f2bf(0.f);
+    return;
+  }
+  const long long total = dec_units_before<STEP>(p, p.b);
+  const long long a = dec_units_before<STEP>(p, row) + (long long)g * steps, z = a + steps - 1;
+  const long long shares = min((long long)SHARES, total);
+  const long long c0 = ((a + 1) * shares - 1) / total, c1 = ((z + 1) * shares - 1) / total;   // unit u's: the last c
+  if (c0 == c1) return;                                                      // with total * c / shares <= u
+  const int stride = p.group * (D + 2);
+  const float* first = p.scratch + (2 * c0 + (total * c0 / shares == a ? 0 : 1)) * stride + h * (D + 2);
+  float mx = first[0];
+  for (long long c = c0 + 1; c <= c1; ++c) mx = fmaxf(mx, p.scratch[2 * c * stride + h * (D + 2)]);
+  float sum = 0.f, v = 0.f;
+#pragma unroll 4
+  for (long long c = c0; c <= c1; ++c) {
+    const float* part = c == c0 ? first : p.scratch + 2 * c * stride + h * (D + 2);
+    const bool none = part[0] == -INFINITY && part[1] == 0.f;
+    const float w = none ? 0.f : exp2f(part[0] - finite(mx));
+    sum += w * part[1];
+    v += w * part[2 + d];
+  }
+  v = mx == -INFINITY && sum == 0.f ? 0.f : v / sum;
+  if (p.pr) v *= ew::sigmoid(bf2f(p.pr[row * p.ldpr + ((int64_t)2 * head + 1) * D + d]));
+  *y = f2bf(v);
+}
+
+template <int D, int NT, bool PAIR>
+int dec_launch(const DecParams& p, cudaStream_t stream) {
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !configured[dev]) {
+    const int r = status_of(cudaFuncSetAttribute(decode_kernel<D, NT, PAIR>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, Dec<D>::SMEM),
+                            "decode_kernel: cudaFuncSetAttribute");
+    if (r) return r;
+    if (dev < 64) configured[dev] = true;
+  }
+  launch_pdl(decode_kernel<D, NT, PAIR>, SHARES, Dec<D>::WARPS * 32, Dec<D>::SMEM, stream, p);
+  if (int r = check_launch("decode_kernel")) return r;
+  launch_pdl(join_kernel<D>, p.b * p.kv_heads * p.group, D, 0, stream, p);
+  return check_launch("join_kernel");
+}
+
+template <int D>
+int dec_launch(const DecParams& p, cudaStream_t stream) {
+  if (p.group <= 4) return dec_launch<D, 1, true>(p, stream);
+  if (p.group <= 8) return dec_launch<D, 1, false>(p, stream);
+  return dec_launch<D, 2, false>(p, stream);
 }
 
 inline bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; }
@@ -373,11 +743,17 @@ extern "C" int jb_decode_attention(const uint16_t* q, int64_t ldq, const void* k
              "jb_decode_attention: row strides %lld, %lld, %lld", (long long)ldq, (long long)ldy, (long long)ldpr);
   JB_REQUIRE(dec::aligned16(q) && dec::aligned16(kv) && dec::aligned16(pr) && dec::aligned16(y),
              "jb_decode_attention: q, the pages, pr and y must be 16-byte aligned");
-  auto kernel = dim == 64 ? dec::decode_plain_kernel<64> : dim == 128 ? dec::decode_plain_kernel<128>
-                                                                      : dec::decode_plain_kernel<256>;
-  launch_pdl(kernel, b * heads, 256, 0, (cudaStream_t)stream, reinterpret_cast<const __nv_bfloat16*>(q), ldq,
-             static_cast<const uint8_t*>(kv) + attn_layer * layer_bytes, pages, page_bytes, tables, table_stride,
-             width, kv_entry, lengths, heads, kv_heads, scale * 1.4426950408889634f,
-             reinterpret_cast<const __nv_bfloat16*>(pr), ldpr, reinterpret_cast<__nv_bfloat16*>(y), ldy);
-  return check_launch("decode_plain_kernel");
+  const int group = heads / kv_heads;
+  JB_REQUIRE((int64_t)b * heads <= 0x7fffffff, "jb_decode_attention: %d rows of %d heads", b, heads);
+  JB_REQUIRE(scratch && scratch_floats >= (int64_t)2 * dec::SHARES * group * (dim + 2),
+             "jb_decode_attention: a scratch of %lld floats, %lld are needed", (long long)scratch_floats,
+             (long long)2 * dec::SHARES * group * (dim + 2));
+  const int64_t most = min((int64_t)(width - kv_entry) * dec::PAGE, (int64_t)0x7fffffc0);
+  const dec::DecParams p = {reinterpret_cast<const __nv_bfloat16*>(q), ldq,
+                            static_cast<const uint8_t*>(kv) + attn_layer * layer_bytes, pages, page_bytes, tables,
+                            table_stride, kv_entry, (int)most, lengths, b, kv_heads, group, dim,
+                            scale * 1.4426950408889634f, reinterpret_cast<const __nv_bfloat16*>(pr), ldpr,
+                            reinterpret_cast<__nv_bfloat16*>(y), ldy, scratch};
+  const cudaStream_t st = (cudaStream_t)stream;
+  return dim == 64 ? dec::dec_launch<64>(p, st) : dim == 128 ? dec::dec_launch<128>(p, st) : dec::dec_launch<256>(p, st);
 }

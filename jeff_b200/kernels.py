@@ -14,6 +14,7 @@ recorded passes pass preallocated buffers, so graphs capture no allocation)."""
 
 from __future__ import annotations
 
+import functools
 from collections.abc import Sequence
 from typing import NamedTuple
 
@@ -363,12 +364,14 @@ def kv_scatter(kn: torch.Tensor, vn: torch.Tensor, n: int, real: torch.Tensor, p
 def _rows_of(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, ...], inner: int,
              device: torch.device) -> None:
     """`t` (shape) of `dtype` on `device`, its last `inner` dimensions packed and the others strided as they like."""
-    if t.dtype != dtype or tuple(t.shape) != shape:
+    if t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name}: expected {dtype} of shape {shape}, got {t.dtype} {tuple(t.shape)}")
     if not t.is_cuda:
         raise ValueError(f"{name}: expected a CUDA tensor, got one on {t.device}")
     if t.device != device:
         raise ValueError(f"{name}: expected a tensor on {device} as the others, got one on {t.device}")
+    if t.is_contiguous():
+        return
     step = 1
     for size, stride in zip(reversed(shape[len(shape) - inner:]), reversed(t.stride()[len(shape) - inner:])):
         if stride != step and size != 1:
@@ -397,11 +400,13 @@ def _cache_of(kv: torch.Tensor, attn_layer: int, device: torch.device) -> tuple[
 
 def _on(device: torch.device, name: str, *args) -> None:
     """One library call on `device` and its current stream."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, stream_ptr())
+    index = device.index
+    # the stream's handle without a Stream object around it: 0.1 us on the host instead of 3.3
+    if index == torch.cuda.current_device():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            _lib.call(name, *args, stream_ptr())
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 class SlotMap(NamedTuple):
@@ -449,14 +454,24 @@ def rope_axes(sections: Sequence[int], interleaved: bool = False) -> int:
     """Which axis's position turns each of the 32 rotary frequencies, for attn_prep_axes: sections[a] frequencies of
     axis a, one axis after the other, or interleaved (frequency i belongs to axis i mod the number of axes while that
     axis has frequencies left, to axis 0 after that). At most four axes; 2 bits a frequency."""
+    return _rope_axes(tuple(sections), interleaved)
+
+
+@functools.lru_cache(maxsize=64)
+def _rope_axes(sections: tuple[int, ...], interleaved: bool) -> int:
     n = len(sections)
     if not 1 <= n <= 4 or sum(sections) != C.ROT // 2 or min(sections) < 0:
-        raise ValueError(f"sections {tuple(sections)}: one to four axes with {C.ROT // 2} frequencies in all")
+        raise ValueError(f"sections {sections}: one to four axes with {C.ROT // 2} frequencies in all")
     if interleaved:
         of = [i % n if i // n < sections[i % n] else 0 for i in range(C.ROT // 2)]
     else:
         of = [a for a, count in enumerate(sections) for _ in range(count)]
     return sum(a << 2 * i for i, a in enumerate(of))
+
+
+@functools.lru_cache(maxsize=64)
+def _axes_fit(axes: int, count: int) -> bool:
+    return 0 <= axes < 1 << C.ROT and all(axes >> 2 * i & 3 < count for i in range(C.ROT // 2))
 
 
 def attn_prep_axes(pr: torch.Tensor, q_w1: torch.Tensor, k_w1: torch.Tensor, inv_freq: torch.Tensor,
@@ -476,7 +491,7 @@ def attn_prep_axes(pr: torch.Tensor, q_w1: torch.Tensor, k_w1: torch.Tensor, inv
     _rows_of(inv_freq, "inv_freq", torch.float32, (C.ROT // 2,), 1, dev)
     count = positions.shape[0] if positions.dim() == 2 else -1
     _rows_of(positions, "positions", torch.int32, (count, t), 1, dev)
-    if not 0 <= axes < 1 << C.ROT or any(axes >> 2 * i & 3 >= count for i in range(C.ROT // 2)):
+    if not _axes_fit(axes, count):
         raise ValueError(f"axes: a frequency has an axis past the positions' {count}")
     for name, x in (("kn", kn), ("vn", vn)):
         if x is not None:
@@ -496,6 +511,12 @@ def attn_prep_axes(pr: torch.Tensor, q_w1: torch.Tensor, k_w1: torch.Tensor, inv
     return out
 
 
+def decode_scratch(heads: int, kv_heads: int, dim: int) -> int:
+    """The floats of decode_attention's scratch, whatever its rows and lengths: two cut rows for each of its 148 shares
+    (an SM's), each of a key/value head's query heads with a maximum, a sum and `dim` values."""
+    return 2 * 148 * (heads // kv_heads) * (dim + 2)
+
+
 def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, attn_layer: int, lengths: torch.Tensor,
                      kv_entry: int, *, scale: float | None = None, pr: torch.Tensor | None = None,
                      out: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
@@ -503,7 +524,9 @@ def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, at
     them, once attn_prep_axes has written it) in the pages tables[r][kv_entry + j // 32] of kv; heads of 64, 128 or
     256, up to 16 query heads to a key/value head, scale 1 / sqrt(dim) unless given. A row without tokens is zeros.
     With pr (the q_proj output, query and gate interleaved per head): times sigmoid(gate), as (b, heads * dim), the
-    o_proj's input; without, (b, heads, dim). fp32 with one rounding."""
+    o_proj's input; without, (b, heads, dim). fp32 with one rounding. The keys of all rows are cut into equal shares over
+    the SMs, whatever the lengths; scratch (decode_scratch floats, overwritten by every call) holds the cut rows' parts
+    and is allocated unless given."""
     dev = q.device
     if q.dim() != 3:
         raise ValueError(f"q: expected (rows, heads, dim), got {tuple(q.shape)}")
@@ -523,12 +546,14 @@ def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, at
         out = torch.empty(shape, dtype=DT, device=dev)
     else:
         _rows_of(out, "out", DT, shape, len(shape) - 1, dev)
-    if scratch is not None:
+    if scratch is None:
+        scratch = torch.empty(decode_scratch(heads, kv_heads, dim), dtype=torch.float32, device=dev)
+    else:
         _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), dev)
     _on(dev, "jb_decode_attention", ptr(q), q.stride(0), ptr(kv), kv.shape[0], 2 * kv.stride(0), attn_layer,
         kv.shape[1], ptr(tables), tables.stride(0), tables.shape[1], kv_entry, ptr(lengths), b, heads, kv_heads, dim,
         dim ** -0.5 if scale is None else scale, ptr(pr), 0 if pr is None else pr.stride(0), ptr(out), out.stride(0),
-        ptr(scratch), 0 if scratch is None else scratch.numel())
+        ptr(scratch), scratch.numel())
     return out
 
 
