@@ -287,24 +287,31 @@ int jb_attn_prep_axes(const uint16_t* pr, int64_t ldpr, int t, const float* q_w1
  * tokens is 0. dim 64, 128 or 256; heads a multiple of kv_heads, at most 16 to one. pr (nullable): y is multiplied by
  * sigmoid(pr[r, 2 dim h + dim + d]), the gate of jb_gate_mul. fp32 with one rounding to bf16. The keys of all rows
  * are cut into equal shares over the GPU and rows that were cut are joined from `scratch`
- * in a fixed order. */
+ * (at least jb_decode_attention_scratch floats, overwritten) in a fixed order. */
 int jb_decode_attention(const uint16_t* q, int64_t ldq, const void* kv, int64_t pages, int64_t page_bytes,
                         int attn_layer, int attn_layers, const int32_t* tables, int table_stride, int width,
                         int kv_entry, const int32_t* lengths, int b, int heads, int kv_heads, int dim, float scale,
                         const uint16_t* pr, int64_t ldpr, uint16_t* y, int64_t ldy, float* scratch,
                         int64_t scratch_floats, void* stream);
 
+/* The floats of jb_decode_attention's scratch, whatever its rows and lengths (0: heads it does not take). */
+int jb_decode_attention_scratch(int heads, int kv_heads, int dim);
+
 /* Linear attention with a decay for each head, over n tokens of b rows: S_t = e^g S_{t-1} + k_t v_t^T, o_t = S_t^T q_t
  * / sqrt(128), states (128, 128) fp32 as jb_gdn_scan's (flat head first_head + h). q, k, v: 128 contiguous values a
  * head, heads 128 apart, their token and row strides given (multiples of 8); o (b, n, heads, 128). g: fp32, a head's
  * log-decay at g[row * g_row + token * g_tok + h] (strides 0, 0: one decay for each head). real (nullable): row r has
  * real[r] tokens; outputs past them are 0 and the state stays. out_tables (nullable): the final states' pages; the
- * reserved pages 0 and 1 are never written. */
+ * reserved pages 0 and 1 are never written. scratch: at least jb_linear_scan_scratch floats, 16-byte aligned,
+ * overwritten (a few long rows are computed in segments, whose states it holds). */
 int jb_linear_scan(const uint16_t* q, int64_t q_row, int64_t q_tok, const uint16_t* k, int64_t k_row, int64_t k_tok,
                    const uint16_t* v, int64_t v_row, int64_t v_tok, const float* g, int64_t g_row, int64_t g_tok,
                    const int32_t* real, uint16_t* o, int b, int n, int heads, void* state, int64_t pages,
                    int64_t page_bytes, int heads_per_page, int first_head, const int32_t* tables, int table_stride,
                    const int32_t* out_tables, int out_stride, float* scratch, int64_t scratch_floats, void* stream);
+
+/* The floats of jb_linear_scan's scratch (0: none). */
+int jb_linear_scan_scratch(int b, int heads, int n);
 
 /* jb_linear_scan's recurrence for one token per row (q, k, v (b, heads, 128), g (b, heads) or one decay for each head,
  * o (b, heads, 128)), the new states written to out_tables' pages (the same tables: in place). beta (nullable, bf16

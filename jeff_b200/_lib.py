@@ -82,7 +82,8 @@ def stream_ptr(stream: torch.cuda.Stream | None = None) -> int:
 # Kernel launches each entry point makes (the product with LoRA makes two: shrink, then the fused GEMM; the decode
 # attention two: the shares, then the join); counted
 # by `call` so a caller can report how many of this library's kernels a recorded pass launches.
-_NO_LAUNCH = {"jb_abi_version", "jb_last_error", "jb_device_status"}
+_NO_LAUNCH = {"jb_abi_version", "jb_last_error", "jb_device_status", "jb_decode_attention_scratch",
+              "jb_linear_scan_scratch"}
 launches = 0
 
 

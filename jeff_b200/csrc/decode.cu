@@ -757,3 +757,9 @@ extern "C" int jb_decode_attention(const uint16_t* q, int64_t ldq, const void* k
   const cudaStream_t st = (cudaStream_t)stream;
   return dim == 64 ? dec::dec_launch<64>(p, st) : dim == 128 ? dec::dec_launch<128>(p, st) : dec::dec_launch<256>(p, st);
 }
+
+extern "C" int jb_decode_attention_scratch(int heads, int kv_heads, int dim) {
+  return kv_heads > 0 && heads >= kv_heads && heads / kv_heads <= 16 && dim > 0 && dim <= 256
+             ? 2 * jb::dec::SHARES * (heads / kv_heads) * (dim + 2)
+             : 0;
+}

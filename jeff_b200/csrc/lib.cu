@@ -160,6 +160,9 @@ int make_tmap_nd(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, 
 #include "attention_tc.cu"
 #include "decode.cu"
 #include "linear.cu"
+#include "linear_tc.cu"
+
+#include "linear_api.cu"
 
 extern "C" int jb_abi_version(void) { return 2; }
 

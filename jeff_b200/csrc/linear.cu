@@ -165,40 +165,3 @@ int check(const char* who, const Args& a, int b) {
 
 }  // namespace lin
 }  // namespace jb
-
-extern "C" int jb_linear_scan(const uint16_t* q, int64_t q_row, int64_t q_tok, const uint16_t* k, int64_t k_row,
-                              int64_t k_tok, const uint16_t* v, int64_t v_row, int64_t v_tok, const float* g,
-                              int64_t g_row, int64_t g_tok, const int32_t* real, uint16_t* o, int b, int n, int heads,
-                              void* state, int64_t pages, int64_t page_bytes, int heads_per_page, int first_head,
-                              const int32_t* tables, int table_stride, const int32_t* out_tables, int out_stride,
-                              float* scratch, int64_t scratch_floats, void* stream) {
-  using namespace jb;
-  const lin::Args a = {reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<const __nv_bfloat16*>(k),
-                       reinterpret_cast<const __nv_bfloat16*>(v), q_row, k_row, v_row, q_tok, k_tok, v_tok, g, g_row,
-                       g_tok, nullptr, real, reinterpret_cast<__nv_bfloat16*>(o), (int64_t)n * heads * lin::D,
-                       (int64_t)heads * lin::D, n, heads,
-                       {static_cast<uint8_t*>(state), pages, page_bytes, heads_per_page, first_head, tables,
-                        table_stride, out_tables, out_stride}};
-  if (int st = lin::check("jb_linear_scan", a, b)) return st;
-  launch_pdl(lin::recurrent_kernel<false>, b * heads, 256, 0, (cudaStream_t)stream, a);
-  return check_launch("linear recurrent_kernel");
-}
-
-extern "C" int jb_linear_step(const uint16_t* q, int64_t q_row, const uint16_t* k, int64_t k_row, const uint16_t* v,
-                              int64_t v_row, const float* g, int64_t g_row, const uint16_t* beta, uint16_t* o, int b,
-                              int heads, void* state, int64_t pages, int64_t page_bytes, int heads_per_page,
-                              int first_head, const int32_t* tables, int table_stride, const int32_t* out_tables,
-                              int out_stride, void* stream) {
-  using namespace jb;
-  const lin::Args a = {reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<const __nv_bfloat16*>(k),
-                       reinterpret_cast<const __nv_bfloat16*>(v), q_row, k_row, v_row, 0, 0, 0, g, g_row, 0,
-                       reinterpret_cast<const __nv_bfloat16*>(beta), nullptr, reinterpret_cast<__nv_bfloat16*>(o),
-                       (int64_t)heads * lin::D, 0, 1, heads,
-                       {static_cast<uint8_t*>(state), pages, page_bytes, heads_per_page, first_head, tables,
-                        table_stride, out_tables, out_stride}};
-  if (int st = lin::check("jb_linear_step", a, b)) return st;
-  JB_REQUIRE(out_tables, "jb_linear_step: null pointer (out_tables: where the new states go)");
-  if (beta) launch_pdl(lin::recurrent_kernel<true>, b * heads, 256, 0, (cudaStream_t)stream, a);
-  else launch_pdl(lin::recurrent_kernel<false>, b * heads, 256, 0, (cudaStream_t)stream, a);
-  return check_launch("linear recurrent_kernel");
-}

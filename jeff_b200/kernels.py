@@ -511,12 +511,6 @@ def attn_prep_axes(pr: torch.Tensor, q_w1: torch.Tensor, k_w1: torch.Tensor, inv
     return out
 
 
-def decode_scratch(heads: int, kv_heads: int, dim: int) -> int:
-    """The floats of decode_attention's scratch, whatever its rows and lengths: two cut rows for each of its 148 shares
-    (an SM's), each of a key/value head's query heads with a maximum, a sum and `dim` values."""
-    return 2 * 148 * (heads // kv_heads) * (dim + 2)
-
-
 def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, attn_layer: int, lengths: torch.Tensor,
                      kv_entry: int, *, scale: float | None = None, pr: torch.Tensor | None = None,
                      out: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
@@ -525,8 +519,8 @@ def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, at
     256, up to 16 query heads to a key/value head, scale 1 / sqrt(dim) unless given. A row without tokens is zeros.
     With pr (the q_proj output, query and gate interleaved per head): times sigmoid(gate), as (b, heads * dim), the
     o_proj's input; without, (b, heads, dim). fp32 with one rounding. The keys of all rows are cut into equal shares over
-    the SMs, whatever the lengths; scratch (decode_scratch floats, overwritten by every call) holds the cut rows' parts
-    and is allocated unless given."""
+    the SMs, whatever the lengths; scratch (fp32, jb_decode_attention_scratch of them, overwritten by every call)
+    holds the cut rows' parts and is allocated unless given."""
     dev = q.device
     if q.dim() != 3:
         raise ValueError(f"q: expected (rows, heads, dim), got {tuple(q.shape)}")
@@ -547,7 +541,8 @@ def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, at
     else:
         _rows_of(out, "out", DT, shape, len(shape) - 1, dev)
     if scratch is None:
-        scratch = torch.empty(decode_scratch(heads, kv_heads, dim), dtype=torch.float32, device=dev)
+        scratch = torch.empty(_lib.load().jb_decode_attention_scratch(heads, kv_heads, dim), dtype=torch.float32,
+                              device=dev)
     else:
         _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), dev)
     _on(dev, "jb_decode_attention", ptr(q), q.stride(0), ptr(kv), kv.shape[0], 2 * kv.stride(0), attn_layer,
@@ -599,14 +594,18 @@ def linear_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     flat head layer * heads + h) that its row of tables names. g: log-decays (b, n, heads) fp32, or (heads,), one for
     each head; -inf forgets. real (b,) int32: row r has real[r] tokens, its outputs past them are zeros. out_tables:
     the rows' final states are written to these pages (the reserved pages 0 and 1 never are); rows must not share
-    them, nor write pages that another row reads."""
+    them, nor write pages that another row reads. scratch (fp32, jb_linear_scan_scratch of them) is allocated unless
+    given."""
     if q.dim() != 4:
         raise ValueError(f"q: expected (rows, tokens, heads, {C.DK}), got {tuple(q.shape)}")
     b, n, heads = q.shape[:3]
     o, pool = _linear_of(q, k, v, g, state, tables, layer, out_tables, out)
     if real is not None:
         _rows_of(real, "real", torch.int32, (b,), 1, q.device)
-    if scratch is not None:
+    if scratch is None:
+        need = _lib.load().jb_linear_scan_scratch(b, heads, n)
+        scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
+    else:
         _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), q.device)
     steps = (0, 0) if g.dim() == 1 else g.stride()[:2]
     _on(q.device, "jb_linear_scan", ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(v),
