@@ -5,19 +5,23 @@
 // every product an M = 128 MMA with the transposed state S^T (lanes: value columns) in tensor memory:
 //   MMA1  D = [K; Q] K^T              (lanes 64-127: Q K^T; the stacked A is the K and Q tiles laid out back to back)
 //   MMA2  D = bf16(S^T) Q'^T          (A in tensor memory; Q' = e^gc Q as two bf16 parts)
-//   MMA3  D += V^T P^T = O^T          (P = Q K^T ∘ Γ as two bf16 parts)
-//   MMA4  S^T += V^T Kd               (Kd = e^{gl - gc} K as three bf16 parts, S^T scaled by e^gl beforehand)
-// Rounding: the state is fp32 and what enters it keeps 24 bits (three parts of a decayed key, the value exact); its
-// bf16 copy for the outputs is the one rounding ahead of theirs. Sums of decays are fp64, their differences rounded
-// to fp32 once, so that a strong decay early in a chunk takes no accuracy from the tokens behind it (-inf is held as
-// -10000, whose exponential is 0).
+//   MMA3  D += V^T P^T = O^T          (P = bf16(Q K^T ∘ Γ))
+//   MMA4  S^T += V^T Kd               (Kd = e^{gl - gc} K in bf16 parts, S^T scaled by e^gl beforehand)
+// Rounding: the state is fp32 and what enters it keeps 24 bits (three bf16 parts of a decayed key, the value exact).
+// Ahead of an output's own rounding its terms are rounded once, by P for the tokens of its chunk, by the state's bf16
+// copy for those before (where the state itself is another launch's, two parts of Kd, 16 bits, serve that copy). Sums
+// of decays are fp64, their differences rounded to fp32 once, so that a strong decay early in a chunk takes no accuracy
+// from the tokens behind it (-inf is held as -10000, whose exponential is 0).
 //
-// Tensor memory, 256 columns: S^T 0-127, its bf16 copy 128-191, D 192-255. Shared memory 113 KB: two CTAs per SM, whose
-// phases (TMA, tensor core, CUDA cores) fill each other's waits. A (row, head) is one CTA, or, where those are fewer
-// than the CTAs that fit, is cut into segments of whole chunks: a first launch leaves each segment's own contribution
-// to the state in scratch (no Q, no outputs), a second turns these into the state ahead of each segment and the final
-// one, the third computes the outputs. Waits are bounded (%globaltimer, 2 s): on expiry the CTA records JB_DEV_TIMEOUT
-// | 50.. in the device status word and returns.
+// Tensor memory, 256 columns: S^T 0-127, its bf16 copy 128-191, D 192-255. Shared memory 107 KB: two CTAs per SM, whose
+// phases (TMA, tensor core, CUDA cores) fill each other's waits. Within a chunk Kd's later parts are formed while MMA1
+// runs, the next chunk's gates while MMA2-4 run, and the next tiles travel during the output and the state's copy: two
+// block barriers a chunk. Of Γ's four 32 x 32 blocks one is zero and one a product of two vectors, so two warps of
+// eight form exponentials and the others Q'. A (row, head) is one CTA, or, where those are fewer than the CTAs that
+// fit, is cut into segments of whole chunks: a first launch leaves each segment's own contribution to the state in
+// scratch (no Q, no outputs), a second turns these into the state ahead of each segment and the final one, the third
+// computes the outputs. Waits are bounded (%globaltimer, 2 s): on expiry the CTA records JB_DEV_TIMEOUT | 50.. in the
+// device status word and returns.
 
 namespace jb {
 namespace lintc {
@@ -34,14 +38,14 @@ using lin::D;
 
 constexpr int C = 64, THREADS = 256;
 constexpr uint32_t TILE = C * D * 2;   // 16 KB: two 64-column atoms of 64 rows x 128 B
-constexpr int OFF_KQ = 0;              // atom a: K at a * 16384, Q at + 8192; then Kd's and Q's first parts in place
-constexpr int OFF_KM = 32768, OFF_KL = OFF_KM + TILE;   // Kd's second and third parts (atoms 8192 apart)
-constexpr int OFF_QL = OFF_KL + TILE;                   // Q's second part
+constexpr int OFF_KQ = 0;              // atom a: K at a * 16384, Q at + 8192; then parts of Kd and Q' in place
+constexpr int OFF_KM = 32768, OFF_KL = OFF_KM + TILE;   // other parts of Kd (atoms 8192 apart)
+constexpr int OFF_QL = OFF_KL + TILE;  // Q's second part; then the output tile
 constexpr int OFF_V = OFF_QL + TILE;
-constexpr int OFF_P = OFF_V + TILE;    // P's two parts, 64 rows x 128 B each; then the output tile (two atoms)
-constexpr int OFF_G = OFF_P + TILE;    // gc (as two floats), e^{gl - gc}
-constexpr int OFF_MISC = OFF_G + 3 * C * 4;
-constexpr int ALLOC = OFF_MISC + 48;
+constexpr int OFF_P = OFF_V + TILE;    // 64 rows x 128 B
+constexpr int OFF_G = OFF_P + TILE / 2;   // two sets of gates
+constexpr int OFF_MISC = OFF_G + 2 * 5 * C * 4;
+constexpr int ALLOC = OFF_MISC + 64;
 static_assert(2 * (ALLOC + 1024) <= 228 * 1024, "two CTAs per SM");
 constexpr uint32_t TM_S = 0, TM_B = 128, TM_D = 192, TM_COLS = 256;
 constexpr int FIT = 2 * 148;           // CTAs that run at once
@@ -83,12 +87,46 @@ __device__ __forceinline__ void split8(const uint4& x, float f, uint4 (&y)[PARTS
   for (int p = 0; p < PARTS; ++p) y[p] = make_uint4(out[p][0], out[p][1], out[p][2], out[p][3]);
 }
 
+// A chunk's gates, from the sums gc of its log-decays: gc in two floats (their differences are the exponents inside the
+// chunk), e^gc, e^{gl - gc}, and Γ's lower left 32 x 32 block as cross[32 + i] cross[j].
+struct Gates {
+  float hi[C], lo[C], from_start[C], to_end[C], cross[C];
+};
+
+__device__ __forceinline__ void form_gates(Gates& g, float a, float b, int lane, volatile float* whole, double& sum) {
+  double x = a, y = b;   // tokens lane and lane + 32
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const double yx = __shfl_up_sync(0xffffffffu, x, off), yy = __shfl_up_sync(0xffffffffu, y, off);
+    if (lane >= off) {
+      x += yx;
+      y += yy;
+    }
+  }
+  const double mid = __shfl_sync(0xffffffffu, x, 31);
+  y += mid;
+  const double all = __shfl_sync(0xffffffffu, y, 31);
+  g.hi[lane] = (float)x;
+  g.hi[lane + 32] = (float)y;
+  g.lo[lane] = (float)(x - (double)(float)x);
+  g.lo[lane + 32] = (float)(y - (double)(float)y);
+  g.from_start[lane] = expf((float)x);
+  g.from_start[lane + 32] = expf((float)y);
+  g.to_end[lane] = expf((float)(all - x));
+  g.to_end[lane + 32] = expf((float)(all - y));
+  g.cross[lane] = expf((float)(mid - x));
+  g.cross[lane + 32] = expf((float)(y - mid));
+  if (lane == 0) *whole = expf((float)all);
+  sum += all;
+}
+
 template <int MODE>
 __global__ void __launch_bounds__(THREADS, 2)
     scan_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o, const Args a,
                 const Seg seg, int* err) {
   pdl_begin();
+  constexpr int PARTS = MODE == OUTPUTS ? 2 : 3;   // of Kd
   extern __shared__ __align__(1024) uint8_t sm[];
   uint8_t* kq = sm + OFF_KQ;
   uint8_t* km = sm + OFF_KM;
@@ -96,16 +134,12 @@ __global__ void __launch_bounds__(THREADS, 2)
   uint8_t* ql = sm + OFF_QL;
   uint8_t* vb = sm + OFF_V;
   uint8_t* pt = sm + OFF_P;
-  float* gh = reinterpret_cast<float*>(sm + OFF_G);
-  float* gr = gh + C;
-  float* ed = gr + C;
+  Gates* gates = reinterpret_cast<Gates*>(sm + OFF_G);
   uint64_t* mma_bar = reinterpret_cast<uint64_t*>(sm + OFF_MISC);
   uint64_t* in_bar = mma_bar + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + OFF_MISC + 16);
-  volatile int* ok_flag = reinterpret_cast<volatile int*>(sm + OFF_MISC + 20);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + OFF_MISC + 24);
-  volatile float* el_all = reinterpret_cast<volatile float*>(sm + OFF_MISC + 28);   // the chunk's whole decay factor
-  double* el_sum = reinterpret_cast<double*>(sm + OFF_MISC + 32);                   // the segment's log-decay so far
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + OFF_MISC + 20);
+  volatile float* whole = reinterpret_cast<volatile float*>(sm + OFF_MISC + 24);   // [2] the chunks' decay factors
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int qd = warp & 3, ch = warp >> 2;
@@ -116,17 +150,15 @@ __global__ void __launch_bounds__(THREADS, 2)
   const int stop = a.real ? min(max(a.real[row], 0), a.n) : a.n;
   const int begin = part * seg.chunks * C, end = min(begin + seg.chunks * C, a.n);
   const int work = min(end, stop);   // tokens past it are padding: zeros out, the state stays
-  const bool aligned = (smem_u32(sm) & 1023) == 0;
-  if (!aligned) {
+  if (smem_u32(sm) & 1023) {         // the swizzled tiles' base
     if (tid == 0) atomicCAS(err, 0, JB_DEV_LAUNCH | 50);
     return;
   }
 
   if (tid == 0) {
     mbar_init(mma_bar, 1);
-    mbar_init(in_bar, 1);
+    mbar_init(in_bar, 2);   // the loads, and that the previous output tile has left its place
     *abort_flag = 0;
-    *el_sum = 0.0;
     fence_barrier_init();
   }
   if (warp == 0) {
@@ -146,18 +178,31 @@ __global__ void __launch_bounds__(THREADS, 2)
     tma_load_4d(vb, &tm_v, in_bar, 0, h, c0, row);
     tma_load_4d(vb + 8192, &tm_v, in_bar, 64, h, c0, row);
   };
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  if (tid == 0 && begin < work) load(begin);
-  const uint32_t tmem = *tmem_slot;
   const float* gp = a.g + row * a.g_row + h;
   auto gate = [&](int t) {   // the log-decay of token t, 0 past the row's end, -inf as a finite number
     if (t >= work) return 0.f;
     const float x = gp[t * a.g_tok];
     return x < -1e4f ? -1e4f : x;
   };
-  float g_next = tid < C ? gate(begin + tid) : 0.f;
+  double decays = 0.0;   // warp 0: the segment's log-decay
+  float g0 = 0.f, g1 = 0.f;
+  if (warp == 0) {
+    g0 = gate(begin + lane);
+    g1 = gate(begin + 32 + lane);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (tid == 0 && begin < work) load(begin);
+  const uint32_t tmem = *tmem_slot;
+  if (warp == 0) {
+    form_gates(gates[0], g0, g1, lane, whole, decays);
+    g0 = gate(begin + C + lane);
+    g1 = gate(begin + C + 32 + lane);
+  }
+  if (MODE != STATES)   // P's upper right block is never anything else
+    for (int i = tid; i < 32 * 4; i += THREADS)
+      *reinterpret_cast<uint4*>(swz(pt, i >> 2, 4 + (i & 3))) = make_uint4(0, 0, 0, 0);
 
   // the state ahead of the segment: lane = value column, columns = key rows
   {
@@ -171,31 +216,46 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
     tc_wait_st();
   }
+  // the state's bf16 copy, then its decay over the chunk
+  auto turn_state = [&](float el) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint32_t ta = tmem + lane_bits + TM_S + 64 * ch + 32 * half;
+      uint32_t r[32];
+      tmem_ld32(ta, r);
+      tc_wait_ld();
+      if (MODE != STATES) {
+        uint32_t b[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) b[e] = pack_bf2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+        tmem_st16(tmem + lane_bits + TM_B + 32 * ch + 16 * half, b);
+      }
+#pragma unroll
+      for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * el);
+      tmem_st32(ta, r);
+    }
+    tc_wait_st();
+  };
+  __syncthreads();
+  if (begin < work) turn_state(whole[0]);
 
-  uint32_t mma_phase = 0, in_phase = 0;
-  auto wait_bar = [&](uint64_t* bar, uint32_t parity, int where) -> bool {   // bounded; every thread learns the outcome
-    if (tid == 0) *ok_flag = mbar_wait(bar, parity, abort_flag, err, where) ? 1 : 0;
-    __syncthreads();
-    tc_fence_after();
-    return *ok_flag != 0;
-  };
-  auto wait_mma = [&]() -> bool {
-    const bool r = wait_bar(mma_bar, mma_phase, 51);
-    mma_phase ^= 1;
-    return r;
-  };
   const uint32_t kq_a = smem_u32(kq), km_a = smem_u32(km), kl_a = smem_u32(kl), ql_a = smem_u32(ql),
                  vb_a = smem_u32(vb), pt_a = smem_u32(pt);
-  bool ok = true;
-
-  for (int c0 = begin; c0 < work && ok; c0 += C) {
+  uint32_t mma_phase = 0, in_phase = 0, set = 0;
+  for (int c0 = begin; c0 < work; c0 += C) {
     const int live = min(C, work - c0);
-    if (tid < C) gh[tid] = g_next;
-    if (!(ok = wait_bar(in_bar, in_phase, 52))) break;
-    mbar_try_wait(in_bar, in_phase);   // every thread acquires the copies itself
+    const bool more = c0 + C < work;
+    const Gates& gt = gates[set];
+    if (tid == 0) {
+      if (MODE != STATES) tma_store_wait_read();
+      mbar_arrive(in_bar);
+    }
+    mbar_wait(in_bar, in_phase, abort_flag, err, 52);
     in_phase ^= 1;
     // ---- MMA1
     if (MODE != STATES && warp == 1) {
+      __syncwarp();
+      tc_fence_after();
       constexpr uint32_t id1 = idesc_bf16(128, 64);
       const bool issuer = elect_one();
 #pragma unroll
@@ -206,112 +266,80 @@ __global__ void __launch_bounds__(THREADS, 2)
       if (issuer) tc_commit(mma_bar);
       __syncwarp();
     }
-    // sums of the 64 log-decays in fp64, then the per-token factors
-    if (warp == 0) {
-      double x = gh[lane], y = gh[lane + 32];
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const double yx = __shfl_up_sync(0xffffffffu, x, off), yy = __shfl_up_sync(0xffffffffu, y, off);
-        if (lane >= off) {
-          x += yx;
-          y += yy;
-        }
-      }
-      y += __shfl_sync(0xffffffffu, x, 31);
-      const double all = __shfl_sync(0xffffffffu, y, 31);
-      gh[lane] = (float)x;
-      gh[lane + 32] = (float)y;
-      gr[lane] = (float)(x - (double)(float)x);
-      gr[lane + 32] = (float)(y - (double)(float)y);
-      ed[lane] = expf((float)(all - x));
-      ed[lane + 32] = expf((float)(all - y));
-      if (lane == 0) {
-        *el_all = expf((float)all);
-        *el_sum += all;
-      }
-    }
     // values past the row's end may be anything: zeros, so that a zero weight keeps them out
     if (live < C)
       for (int i = tid; i < (C - live) * 16; i += THREADS) {
         const int t = live + (i >> 4), c = i & 15;
         *reinterpret_cast<uint4*>(swz(vb + (c >> 3) * 8192, t, c & 7)) = make_uint4(0, 0, 0, 0);
       }
-    if (tid == 0 && MODE != STATES) tma_store_wait_read();   // the previous output tile has left P's place
-    __syncthreads();
-    // ---- the state: its bf16 copy, then its decay over the chunk
-    {
-      const float el = *el_all;
+    // ---- Kd: thread = 16-byte piece of a token; with three parts the first waits for MMA1 to have read K
+    uint4 first[4];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t ta = tmem + lane_bits + TM_S + 64 * ch + 32 * half;
-        uint32_t r[32];
-        tmem_ld32(ta, r);
-        tc_wait_ld();
-        if (MODE != STATES) {
-          uint32_t b[16];
+    for (int it = 0; it < 4; ++it) {
+      const int i = it * THREADS + tid, t = i >> 4, c = i & 15, at = c >> 3;
+      uint4 y[PARTS];
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            b[e] = pack_bf2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
-          tmem_st16(tmem + lane_bits + TM_B + 32 * ch + 16 * half, b);
-        }
-#pragma unroll
-        for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * el);
-        tmem_st32(ta, r);
-      }
-      tc_wait_st();
+      for (int p = 0; p < PARTS; ++p) y[p] = make_uint4(0, 0, 0, 0);
+      if (t < live) split8(*reinterpret_cast<const uint4*>(swz(kq + at * 16384, t, c & 7)), gt.to_end[t], y);
+      *reinterpret_cast<uint4*>(swz(km + at * 8192, t, c & 7)) = y[PARTS - 2];
+      *reinterpret_cast<uint4*>(swz(kl + at * 8192, t, c & 7)) = y[PARTS - 1];
+      first[it] = y[0];
     }
     if (MODE != STATES) {
-      if (!(ok = wait_mma())) break;
-      // ---- Q' over Q, its second part behind
-      for (int i = tid; i < C * 16; i += THREADS) {
-        const int t = i >> 4, c = i & 15, at = c >> 3;
-        uint8_t* p = swz(kq + at * 16384 + 8192, t, c & 7);
-        uint4 y[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-        if (t < live) split8(*reinterpret_cast<const uint4*>(p), expf(gh[t]), y);
-        *reinterpret_cast<uint4*>(p) = y[0];
-        *reinterpret_cast<uint4*>(swz(ql + at * 8192, t, c & 7)) = y[1];
+      mbar_wait(mma_bar, mma_phase, abort_flag, err, 51);
+      mma_phase ^= 1;
+      tc_fence_after();
+    }
+    if (PARTS == 3) {
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const int i = it * THREADS + tid, t = i >> 4, c = i & 15;
+        *reinterpret_cast<uint4*>(swz(kq + (c >> 3) * 16384, t, c & 7)) = first[it];
       }
     }
-    if (MODE == STATES || qd < 2) {
-      // ---- Kd over K and behind: warps of lanes 0-63 (all of them without outputs)
-      const int me = MODE == STATES ? tid : (ch * 2 + qd) * 32 + lane, step = MODE == STATES ? THREADS : THREADS / 2;
-      for (int i = me; i < C * 16; i += step) {
-        const int t = i >> 4, c = i & 15, at = c >> 3;
-        uint8_t* p = swz(kq + at * 16384, t, c & 7);
-        uint4 y[3] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-        if (t < live) split8(*reinterpret_cast<const uint4*>(p), ed[t], y);
-        *reinterpret_cast<uint4*>(p) = y[0];
-        *reinterpret_cast<uint4*>(swz(km + at * 8192, t, c & 7)) = y[1];
-        *reinterpret_cast<uint4*>(swz(kl + at * 8192, t, c & 7)) = y[2];
-      }
-    } else {
-      // ---- P from D's lanes 64-127: row i = L - 64, columns 32 ch .. + 31
-      uint32_t r[32];
-      tmem_ld32(tmem + lane_bits + TM_D + 32 * ch, r);
-      tc_wait_ld();
-      const int i = L - C;
-      const float hi = gh[i], ri = gr[i];
-      const int upto = i < live ? i : -1;
+    if (MODE != STATES) {
+      if (qd >= 2 && !(qd == 2 && ch == 1)) {
+        // ---- P from D's lanes 64-127: row i = L - 64, columns 32 ch .. + 31
+        uint32_t r[32];
+        tmem_ld32(tmem + lane_bits + TM_D + 32 * ch, r);
+        tc_wait_ld();
+        const int i = L - C;
+        const float hi = gt.hi[i], lo = gt.lo[i], ci = gt.cross[i];
+        const int upto = i < live ? i : -1;
 #pragma unroll
-      for (int c8 = 0; c8 < 4; ++c8) {
-        uint32_t p0[4], p1[4];
+        for (int c8 = 0; c8 < 4; ++c8) {
+          uint32_t pk[4];
 #pragma unroll
-        for (int e2 = 0; e2 < 4; ++e2) {
-          const int j = 32 * ch + 8 * c8 + 2 * e2;
-          const float x = j <= upto ? __uint_as_float(r[8 * c8 + 2 * e2]) *
-                                          exp_neg((hi - gh[j]) + (ri - gr[j])) : 0.f;
-          const float y = j + 1 <= upto ? __uint_as_float(r[8 * c8 + 2 * e2 + 1]) *
-                                              exp_neg((hi - gh[j + 1]) + (ri - gr[j + 1])) : 0.f;
-          p0[e2] = pack_bf2(x, y);
-          p1[e2] = pack_bf2(x - bf_lo(p0[e2]), y - bf_hi(p0[e2]));
+          for (int e2 = 0; e2 < 4; ++e2) {
+            float x[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int j = 32 * ch + 8 * c8 + 2 * e2 + e;
+              const float f = qd == 3 && ch == 0 ? ci * gt.cross[j] : exp_neg((hi - gt.hi[j]) + (lo - gt.lo[j]));
+              x[e] = j <= upto ? __uint_as_float(r[8 * c8 + 2 * e2 + e]) * f : 0.f;
+            }
+            pk[e2] = pack_bf2(x[0], x[1]);
+          }
+          *reinterpret_cast<uint4*>(swz(pt, i, 4 * ch + c8)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
         }
-        *reinterpret_cast<uint4*>(swz(pt, i, 4 * ch + c8)) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
-        *reinterpret_cast<uint4*>(swz(pt + 8192, i, 4 * ch + c8)) = make_uint4(p1[0], p1[1], p1[2], p1[3]);
+      }
+      if (warp != 2 && warp != 7) {
+        // ---- Q' over Q, its second part behind: the six warps that form no exponentials
+        const int me = (warp - (warp > 2)) * 32 + lane;
+        for (int i = me; i < C * 16; i += 6 * 32) {
+          const int t = i >> 4, c = i & 15, at = c >> 3;
+          uint8_t* p = swz(kq + at * 16384 + 8192, t, c & 7);
+          uint4 y[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+          if (t < live) split8(*reinterpret_cast<const uint4*>(p), gt.from_start[t], y);
+          *reinterpret_cast<uint4*>(p) = y[0];
+          *reinterpret_cast<uint4*>(swz(ql + at * 8192, t, c & 7)) = y[1];
+        }
       }
     }
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag) break;
     // ---- MMA2, MMA3, MMA4
     if (warp == 1) {
       tc_fence_after();
@@ -329,12 +357,8 @@ __global__ void __launch_bounds__(THREADS, 2)
         }
 #pragma unroll
         for (int kk = 0; kk < C / 16; ++kk) {
-          const uint64_t av = mn_desc(vb_a + kk * 2048, 8192);
-          const uint64_t b0 = sw128_desc(pt_a + 32 * kk), b1 = sw128_desc(pt_a + 8192 + 32 * kk);
-          if (issuer) {
-            tc_mma_bf16(tmem + TM_D, av, b0, id3, 1);
-            tc_mma_bf16(tmem + TM_D, av, b1, id3, 1);
-          }
+          const uint64_t av = mn_desc(vb_a + kk * 2048, 8192), b0 = sw128_desc(pt_a + 32 * kk);
+          if (issuer) tc_mma_bf16(tmem + TM_D, av, b0, id3, 1);
         }
       }
       constexpr uint32_t id4 = idesc_bf16(128, 128) | A_MN | B_MN;
@@ -346,22 +370,29 @@ __global__ void __launch_bounds__(THREADS, 2)
         if (issuer) {
           tc_mma_bf16(tmem + TM_S, av, b2, id4, 1);   // the small parts first
           tc_mma_bf16(tmem + TM_S, av, b1, id4, 1);
-          tc_mma_bf16(tmem + TM_S, av, b0, id4, 1);
+          if (PARTS == 3) tc_mma_bf16(tmem + TM_S, av, b0, id4, 1);
         }
       }
       if (issuer) tc_commit(mma_bar);
       __syncwarp();
     }
-    if (tid < C) g_next = gate(c0 + C + tid);
-    if (!(ok = wait_mma())) break;
-    if (tid == 0 && c0 + C < work) load(c0 + C);   // every tile has been read
+    if (warp == 0 && more) {   // the next chunk's gates, and the decays of the one after it
+      form_gates(gates[set ^ 1], g0, g1, lane, whole + (set ^ 1), decays);
+      g0 = gate(c0 + 2 * C + lane);
+      g1 = gate(c0 + 2 * C + 32 + lane);
+    }
+    set ^= 1;
+    mbar_wait(mma_bar, mma_phase, abort_flag, err, 51);
+    mma_phase ^= 1;
+    tc_fence_after();
+    if (tid == 0 && more) load(c0 + C);   // every tile has been read
     if (MODE != STATES) {
-      // ---- O^T -> bf16 -> the output tile over P, laid out as the loads -> TMA store
+      // ---- O^T -> bf16 -> the output tile over Q's second part, laid out as the loads -> TMA store
       uint32_t r[32];
       tmem_ld32(tmem + lane_bits + TM_D + 32 * ch, r);
       tc_wait_ld();
       const float scale = rsqrtf((float)D);
-      __nv_bfloat16* ot = reinterpret_cast<__nv_bfloat16*>(pt + (L >> 6) * 8192);
+      __nv_bfloat16* ot = reinterpret_cast<__nv_bfloat16*>(ql + (L >> 6) * 8192);
       const int cl = L & 63;
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
@@ -370,19 +401,26 @@ __global__ void __launch_bounds__(THREADS, 2)
       }
       fence_proxy_async_smem();
       tc_fence_before();
-      __syncthreads();
-      if (tid == 0) {
-        tma_store_4d(&tm_o, pt, 0, h, c0, row);
-        tma_store_4d(&tm_o, pt + 8192, 64, h, c0, row);
-        tma_store_commit();
-      }
     }
+    __syncthreads();
+    if (*abort_flag) break;
+    if (MODE != STATES && tid == 0) {
+      tma_store_4d(&tm_o, ql, 0, h, c0, row);
+      tma_store_4d(&tm_o, ql + 8192, 64, h, c0, row);
+      tma_store_commit();
+    }
+    if (more) turn_state(whole[set]);
   }
+  const bool ok = *abort_flag == 0;
   if (tid == 0) {
     if (MODE != STATES) tma_store_wait_all();
-    // a CTA that gave up waits (bounded) for the copies it issued before its shared memory goes away
-    const uint64_t t0 = global_ns();
-    while (issued && !mbar_try_wait(in_bar, (issued - 1) & 1) && global_ns() - t0 < kWaitNs) {
+    // a CTA that gave up waits (bounded) for the copies it issued before its shared memory goes away: without its own
+    // arrival their phase may never end, so it arrives first
+    if (!ok && issued) {
+      mbar_arrive(in_bar);
+      const uint64_t t0 = global_ns();
+      while (!mbar_try_wait(in_bar, (issued - 1) & 1) && global_ns() - t0 < kWaitNs) {
+      }
     }
   }
   if (MODE != STATES) {   // chunks that hold padding only
@@ -401,7 +439,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
       for (int i = 0; i < 32; ++i) out[(ch * 64 + half * 32 + i) * D + L] = __uint_as_float(r[i]);
     }
-    if (MODE == STATES && tid == 0) seg.decay[(int64_t)pair * seg.count + part] = expf((float)*el_sum);
+    if (MODE == STATES && tid == 0) seg.decay[(int64_t)pair * seg.count + part] = expf((float)decays);
   }
   tc_fence_before();
   __syncthreads();
@@ -421,12 +459,22 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a, const Seg seg) 
   float4 s = in ? reinterpret_cast<const float4*>(in)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
   float4* parts = reinterpret_cast<float4*>(seg.states + (int64_t)pair * seg.count * STATE) + i;
   const float* decay = seg.decay + (int64_t)pair * seg.count;
-#pragma unroll 4
-  for (int p = 0; p < seg.count; ++p) {
-    const float4 x = parts[(int64_t)p * (STATE / 4)];
-    const float e = decay[p];
-    parts[(int64_t)p * (STATE / 4)] = s;
-    s = make_float4(s.x * e + x.x, s.y * e + x.y, s.z * e + x.z, s.w * e + x.w);
+  constexpr int AHEAD = 8;   // segments read before the first of them is overwritten
+  for (int p0 = 0; p0 < seg.count; p0 += AHEAD) {
+    float4 x[AHEAD];
+    float e[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (p0 + j < seg.count) {
+        x[j] = parts[(int64_t)(p0 + j) * (STATE / 4)];
+        e[j] = decay[p0 + j];
+      }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (p0 + j < seg.count) {
+        parts[(int64_t)(p0 + j) * (STATE / 4)] = s;
+        s = make_float4(s.x * e[j] + x[j].x, s.y * e[j] + x[j].y, s.z * e[j] + x[j].z, s.w * e[j] + x[j].w);
+      }
   }
   if (float* out = lin::state_out(a.pool, row, h)) reinterpret_cast<float4*>(out)[i] = s;
 }
