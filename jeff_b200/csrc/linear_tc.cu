@@ -4,8 +4,8 @@
 //   S <- e^gl S + (e^{gl - gc} K)^T V,
 // every product an M = 128 MMA with the transposed state S^T (lanes: value columns) in tensor memory:
 //   MMA1  D = [K; Q] K^T              (lanes 64-127: Q K^T; the stacked A is the K and Q tiles laid out back to back)
-//   MMA2  D = bf16(S^T) Q'^T          (A in tensor memory; Q' = e^gc Q as two bf16 parts)
-//   MMA3  D += V^T P^T = O^T          (P = bf16(Q K^T ∘ Γ))
+//   MMA2  D = bf16(S^T) Q^T           (A in tensor memory)
+//   MMA3  E = V^T P^T                 (P = bf16(Q K^T ∘ Γ)); O^T = e^gc D + E, a factor for each of D's columns
 //   MMA4  S^T += V^T Kd               (Kd = e^{gl - gc} K in bf16 parts, S^T scaled by e^gl beforehand)
 // Rounding: the state is fp32 and what enters it keeps 24 bits (three bf16 parts of a decayed key, the value exact).
 // Ahead of an output's own rounding its terms are rounded once, by P for the tokens of its chunk, by the state's bf16
@@ -13,15 +13,15 @@
 // of decays are fp64, their differences rounded to fp32 once, so that a strong decay early in a chunk takes no accuracy
 // from the tokens behind it (-inf is held as -10000, whose exponential is 0).
 //
-// Tensor memory, 256 columns: S^T 0-127, its bf16 copy 128-191, D 192-255. Shared memory 107 KB: two CTAs per SM, whose
-// phases (TMA, tensor core, CUDA cores) fill each other's waits. Within a chunk Kd's later parts are formed while MMA1
-// runs, the next chunk's gates while MMA2-4 run, and the next tiles travel during the output and the state's copy: two
-// block barriers a chunk. Of Γ's four 32 x 32 blocks one is zero and one a product of two vectors, so two warps of
-// eight form exponentials and the others Q'. A (row, head) is one CTA, or, where those are fewer than the CTAs that
-// fit, is cut into segments of whole chunks: a first launch leaves each segment's own contribution to the state in
-// scratch (no Q, no outputs), a second turns these into the state ahead of each segment and the final one, the third
-// computes the outputs. Waits are bounded (%globaltimer, 2 s): on expiry the CTA records JB_DEV_TIMEOUT | 50.. in the
-// device status word and returns.
+// Tensor memory, 256 columns: S^T 0-127, its bf16 copy 128-191 (E once MMA2 has read it), D 192-255. Shared memory 107
+// KB: two CTAs per SM, whose phases (TMA, tensor core, CUDA cores) fill each other's waits. Within a chunk the warps of
+// lanes 64-127 form P (of Γ's four 32 x 32 blocks one is zero, one a product of two vectors, two need exponentials) and
+// the others most of Kd; the next chunk's gates are formed and its K and V fetched while MMA2-4 run, its Q once MMA2 is
+// done. Two block barriers a chunk. A (row, head) is one CTA, or, where those are fewer than the CTAs that fit, is cut
+// into segments of whole chunks: a first launch leaves each segment's own contribution to the state in scratch (no Q,
+// no outputs), a second turns these into the state ahead of each segment and the final one, the third computes the
+// outputs. Waits are bounded (%globaltimer, 2 s): on expiry the CTA records JB_DEV_TIMEOUT | 50.. in the device status
+// word and returns.
 
 namespace jb {
 namespace lintc {
@@ -38,10 +38,10 @@ using lin::D;
 
 constexpr int C = 64, THREADS = 256;
 constexpr uint32_t TILE = C * D * 2;   // 16 KB: two 64-column atoms of 64 rows x 128 B
-constexpr int OFF_KQ = 0;              // atom a: K at a * 16384, Q at + 8192; then parts of Kd and Q' in place
-constexpr int OFF_KM = 32768, OFF_KL = OFF_KM + TILE;   // other parts of Kd (atoms 8192 apart)
-constexpr int OFF_QL = OFF_KL + TILE;  // Q's second part; then the output tile
-constexpr int OFF_V = OFF_QL + TILE;
+constexpr int OFF_KQ = 0;              // atom a: K at a * 16384, Q at + 8192 (no Q: the second V)
+constexpr int OFF_K0 = 32768, OFF_K1 = OFF_K0 + TILE;   // the parts of Kd (atoms 8192 apart); over the first then the
+constexpr int OFF_K2 = OFF_K1 + TILE;  // output tile. The third part, or with two the second V
+constexpr int OFF_V = OFF_K2 + TILE;
 constexpr int OFF_P = OFF_V + TILE;    // 64 rows x 128 B
 constexpr int OFF_G = OFF_P + TILE / 2;   // two sets of gates
 constexpr int OFF_MISC = OFF_G + 2 * 5 * C * 4;
@@ -68,23 +68,51 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       : "memory");
 }
 
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
 // eight bf16 values times f, in `parts` bf16 parts
 template <int PARTS>
 __device__ __forceinline__ void split8(const uint4& x, float f, uint4 (&y)[PARTS]) {
   const uint32_t in[4] = {x.x, x.y, x.z, x.w};
   uint32_t out[PARTS][4];
+  const uint64_t ff = pair2(f, f), minus = pair2(-1.f, -1.f);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float a = bf_lo(in[i]) * f, b = bf_hi(in[i]) * f;
+    uint64_t v = pair2(bf_lo(in[i]), bf_hi(in[i]));
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(ff));
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
+      float a, b;
+      asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
       out[p][i] = pack_bf2(a, b);
-      a -= bf_lo(out[p][i]);
-      b -= bf_hi(out[p][i]);
+      if (p + 1 < PARTS) {
+        const uint64_t h = pair2(bf_lo(out[p][i]), bf_hi(out[p][i]));
+        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(v) : "l"(h), "l"(minus));
+      }
     }
   }
 #pragma unroll
   for (int p = 0; p < PARTS; ++p) y[p] = make_uint4(out[p][0], out[p][1], out[p][2], out[p][3]);
+}
+
+// 32 columns of 16 tensor-memory lanes, as matrix fragments: register 4 i + e of lane l is row l / 4 + 8 (e / 2), column
+// 8 i + 2 (l % 4) + e % 2
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+// four 8 x 8 matrices of such fragments, transposed: lane l gives the address of row l % 8 of matrix l / 8
+__device__ __forceinline__ void st_frags_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b),
+               "r"(c), "r"(d)
+               : "memory");
 }
 
 // A chunk's gates, from the sums gc of its log-decays: gc in two floats (their differences are the exponents inside the
@@ -94,7 +122,7 @@ struct Gates {
 };
 
 __device__ __forceinline__ void form_gates(Gates& g, float a, float b, int lane, volatile float* whole, double& sum) {
-  double x = a, y = b;   // tokens lane and lane + 32
+  double x = a < -1e4f ? -1e4f : a, y = b < -1e4f ? -1e4f : b;   // tokens lane and lane + 32
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const double yx = __shfl_up_sync(0xffffffffu, x, off), yy = __shfl_up_sync(0xffffffffu, y, off);
@@ -126,20 +154,22 @@ __global__ void __launch_bounds__(THREADS, 2)
                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o, const Args a,
                 const Seg seg, int* err) {
   pdl_begin();
+  constexpr bool OUT = MODE != STATES;
   constexpr int PARTS = MODE == OUTPUTS ? 2 : 3;   // of Kd
+  constexpr bool TWO_V = MODE != WHOLE;            // a second V tile: the next chunk's comes early
   extern __shared__ __align__(1024) uint8_t sm[];
   uint8_t* kq = sm + OFF_KQ;
-  uint8_t* km = sm + OFF_KM;
-  uint8_t* kl = sm + OFF_KL;
-  uint8_t* ql = sm + OFF_QL;
-  uint8_t* vb = sm + OFF_V;
   uint8_t* pt = sm + OFF_P;
+  uint8_t* ot = sm + OFF_K0;
   Gates* gates = reinterpret_cast<Gates*>(sm + OFF_G);
-  uint64_t* mma_bar = reinterpret_cast<uint64_t*>(sm + OFF_MISC);
-  uint64_t* in_bar = mma_bar + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + OFF_MISC + 16);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + OFF_MISC + 20);
-  volatile float* whole = reinterpret_cast<volatile float*>(sm + OFF_MISC + 24);   // [2] the chunks' decay factors
+  uint64_t* mma_bar = reinterpret_cast<uint64_t*>(sm + OFF_MISC);   // MMA1, MMA2-4 of a chunk in turn
+  uint64_t* d_bar = mma_bar + 1;                                    // MMA2
+  uint64_t* k_bar = mma_bar + 2;
+  uint64_t* q_bar = mma_bar + 3;
+  uint64_t* v_bar = mma_bar + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + OFF_MISC + 40);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + OFF_MISC + 44);
+  volatile float* whole = reinterpret_cast<volatile float*>(sm + OFF_MISC + 48);   // [2] the chunks' decay factors
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int qd = warp & 3, ch = warp >> 2;
@@ -157,7 +187,10 @@ __global__ void __launch_bounds__(THREADS, 2)
 
   if (tid == 0) {
     mbar_init(mma_bar, 1);
-    mbar_init(in_bar, 2);   // the loads, and that the previous output tile has left its place
+    mbar_init(d_bar, 1);
+    mbar_init(k_bar, 2);   // the load, and that the previous output tile has left its place
+    mbar_init(q_bar, 1);
+    mbar_init(v_bar, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -165,25 +198,35 @@ __global__ void __launch_bounds__(THREADS, 2)
     tmem_alloc(tmem_slot, TM_COLS);
     tmem_relinquish();
   }
-  int issued = 0;
-  auto load = [&](int c0) {
-    ++issued;
-    mbar_arrive_expect_tx(in_bar, (MODE == STATES ? 2 : 3) * TILE);
-    tma_load_4d(kq, &tm_k, in_bar, 0, h, c0, row);
-    tma_load_4d(kq + 16384, &tm_k, in_bar, 64, h, c0, row);
-    if (MODE != STATES) {
-      tma_load_4d(kq + 8192, &tm_q, in_bar, 0, h, c0, row);
-      tma_load_4d(kq + 16384 + 8192, &tm_q, in_bar, 64, h, c0, row);
-    }
-    tma_load_4d(vb, &tm_v, in_bar, 0, h, c0, row);
-    tma_load_4d(vb + 8192, &tm_v, in_bar, 64, h, c0, row);
+  // the place of the V tile of a chunk (its atoms v_step apart); tile loads, all issued by one lane of warp 1 at a time
+  constexpr int V2 = MODE == STATES ? OFF_KQ + 8192 : OFF_K2;
+  auto v_place = [&](int odd) { return TWO_V && odd ? V2 : OFF_V; };
+  auto v_step = [&](int odd) { return MODE == STATES && odd ? 16384 : 8192; };
+  int k_issued = 0, q_issued = 0, v_issued = 0;
+  auto load_k = [&](int c0, bool me) {
+    ++k_issued;
+    if (!me) return;
+    mbar_arrive_expect_tx(k_bar, TILE);
+    tma_load_4d(kq, &tm_k, k_bar, 0, h, c0, row);
+    tma_load_4d(kq + 16384, &tm_k, k_bar, 64, h, c0, row);
+  };
+  auto load_q = [&](int c0, bool me) {
+    ++q_issued;
+    if (!me) return;
+    mbar_arrive_expect_tx(q_bar, TILE);
+    tma_load_4d(kq + 8192, &tm_q, q_bar, 0, h, c0, row);
+    tma_load_4d(kq + 16384 + 8192, &tm_q, q_bar, 64, h, c0, row);
+  };
+  auto load_v = [&](int c0, int odd, bool me) {
+    ++v_issued;
+    if (!me) return;
+    uint8_t* to = sm + v_place(odd);
+    mbar_arrive_expect_tx(v_bar, TILE);
+    tma_load_4d(to, &tm_v, v_bar, 0, h, c0, row);
+    tma_load_4d(to + v_step(odd), &tm_v, v_bar, 64, h, c0, row);
   };
   const float* gp = a.g + row * a.g_row + h;
-  auto gate = [&](int t) {   // the log-decay of token t, 0 past the row's end, -inf as a finite number
-    if (t >= work) return 0.f;
-    const float x = gp[t * a.g_tok];
-    return x < -1e4f ? -1e4f : x;
-  };
+  auto gate = [&](int t) { return t < work ? gp[t * a.g_tok] : 0.f; };   // 0 past the row's end
   double decays = 0.0;   // warp 0: the segment's log-decay
   float g0 = 0.f, g1 = 0.f;
   if (warp == 0) {
@@ -193,14 +236,20 @@ __global__ void __launch_bounds__(THREADS, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (tid == 0 && begin < work) load(begin);
+  if (warp == 1 && begin < work) {
+    const bool me = elect_one();
+    load_k(begin, me);
+    if (OUT) load_q(begin, me);
+    load_v(begin, 0, me);
+    __syncwarp();
+  }
   const uint32_t tmem = *tmem_slot;
   if (warp == 0) {
     form_gates(gates[0], g0, g1, lane, whole, decays);
     g0 = gate(begin + C + lane);
     g1 = gate(begin + C + 32 + lane);
   }
-  if (MODE != STATES)   // P's upper right block is never anything else
+  if (OUT)   // P's upper right block is never anything else
     for (int i = tid; i < 32 * 4; i += THREADS)
       *reinterpret_cast<uint4*>(swz(pt, i >> 2, 4 + (i & 3))) = make_uint4(0, 0, 0, 0);
 
@@ -224,7 +273,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       uint32_t r[32];
       tmem_ld32(ta, r);
       tc_wait_ld();
-      if (MODE != STATES) {
+      if (OUT) {
         uint32_t b[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) b[e] = pack_bf2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
@@ -239,21 +288,20 @@ __global__ void __launch_bounds__(THREADS, 2)
   __syncthreads();
   if (begin < work) turn_state(whole[0]);
 
-  const uint32_t kq_a = smem_u32(kq), km_a = smem_u32(km), kl_a = smem_u32(kl), ql_a = smem_u32(ql),
-                 vb_a = smem_u32(vb), pt_a = smem_u32(pt);
-  uint32_t mma_phase = 0, in_phase = 0, set = 0;
+  const uint32_t kq_a = smem_u32(kq), kd_a = smem_u32(sm + OFF_K0), pt_a = smem_u32(pt);
+  uint32_t mma_phase = 0, phase = 0, set = 0;   // set: the chunk's parity
   for (int c0 = begin; c0 < work; c0 += C) {
     const int live = min(C, work - c0);
     const bool more = c0 + C < work;
     const Gates& gt = gates[set];
     if (tid == 0) {
-      if (MODE != STATES) tma_store_wait_read();
-      mbar_arrive(in_bar);
+      if (OUT) tma_store_wait_read();
+      mbar_arrive(k_bar);
     }
-    mbar_wait(in_bar, in_phase, abort_flag, err, 52);
-    in_phase ^= 1;
+    mbar_wait(k_bar, phase, abort_flag, err, 52);
     // ---- MMA1
-    if (MODE != STATES && warp == 1) {
+    if (OUT && warp == 1) {
+      mbar_wait(q_bar, phase, abort_flag, err, 53);
       __syncwarp();
       tc_fence_after();
       constexpr uint32_t id1 = idesc_bf16(128, 64);
@@ -267,110 +315,112 @@ __global__ void __launch_bounds__(THREADS, 2)
       __syncwarp();
     }
     // values past the row's end may be anything: zeros, so that a zero weight keeps them out
-    if (live < C)
+    if (live < C) {
+      mbar_wait(v_bar, phase, abort_flag, err, 54);
       for (int i = tid; i < (C - live) * 16; i += THREADS) {
         const int t = live + (i >> 4), c = i & 15;
-        *reinterpret_cast<uint4*>(swz(vb + (c >> 3) * 8192, t, c & 7)) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(swz(sm + v_place(set) + (c >> 3) * v_step(set), t, c & 7)) = make_uint4(0, 0, 0, 0);
       }
-    // ---- Kd: thread = 16-byte piece of a token; with three parts the first waits for MMA1 to have read K
-    uint4 first[4];
-#pragma unroll
-    for (int it = 0; it < 4; ++it) {
-      const int i = it * THREADS + tid, t = i >> 4, c = i & 15, at = c >> 3;
+    }
+    // ---- Kd, a 16-byte piece of a token at a time: six for the warps of lanes 0-63, two for those that form P
+    auto form_kd = [&](int i) {
+      const int t = i >> 4, c = i & 15, at = c >> 3;
       uint4 y[PARTS];
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) y[p] = make_uint4(0, 0, 0, 0);
       if (t < live) split8(*reinterpret_cast<const uint4*>(swz(kq + at * 16384, t, c & 7)), gt.to_end[t], y);
-      *reinterpret_cast<uint4*>(swz(km + at * 8192, t, c & 7)) = y[PARTS - 2];
-      *reinterpret_cast<uint4*>(swz(kl + at * 8192, t, c & 7)) = y[PARTS - 1];
-      first[it] = y[0];
-    }
-    if (MODE != STATES) {
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p)
+        *reinterpret_cast<uint4*>(swz(sm + OFF_K0 + p * TILE + at * 8192, t, c & 7)) = y[p];
+    };
+    if (!OUT) {
+#pragma unroll
+      for (int it = 0; it < 4; ++it) form_kd(it * THREADS + tid);
+    } else if (qd < 2) {
+      const int me = (ch * 2 + qd) * 32 + lane;
+#pragma unroll
+      for (int it = 0; it < 6; ++it) form_kd(it * 128 + me);
+    } else {
+      const int me = (ch * 2 + qd - 2) * 32 + lane;
+#pragma unroll
+      for (int it = 6; it < 8; ++it) form_kd(it * 128 + me);
       mbar_wait(mma_bar, mma_phase, abort_flag, err, 51);
-      mma_phase ^= 1;
       tc_fence_after();
-    }
-    if (PARTS == 3) {
-#pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        const int i = it * THREADS + tid, t = i >> 4, c = i & 15;
-        *reinterpret_cast<uint4*>(swz(kq + (c >> 3) * 16384, t, c & 7)) = first[it];
-      }
-    }
-    if (MODE != STATES) {
-      if (qd >= 2 && !(qd == 2 && ch == 1)) {
-        // ---- P from D's lanes 64-127: row i = L - 64, columns 32 ch .. + 31
-        uint32_t r[32];
-        tmem_ld32(tmem + lane_bits + TM_D + 32 * ch, r);
+      // ---- P from D's lanes 64-127: row i = L - 64; columns 16 ch .. + 15 of the left half, and for rows from 32 on
+      // 32 + 16 ch .. + 15 too
+      const int i = L - C;
+      const float hi = gt.hi[i], lo = gt.lo[i], ci = gt.cross[i];
+      const int upto = i < live ? i : -1;
+      for (int half = 0; half < (qd == 3 ? 2 : 1); ++half) {
+        const bool cross = qd == 3 && half == 0;
+        const int j0 = 32 * half + 16 * ch;
+        uint32_t r[16];
+        lsh::tmem_ld16(tmem + lane_bits + TM_D + j0, r);
         tc_wait_ld();
-        const int i = L - C;
-        const float hi = gt.hi[i], lo = gt.lo[i], ci = gt.cross[i];
-        const int upto = i < live ? i : -1;
 #pragma unroll
-        for (int c8 = 0; c8 < 4; ++c8) {
+        for (int c8 = 0; c8 < 2; ++c8) {
           uint32_t pk[4];
 #pragma unroll
           for (int e2 = 0; e2 < 4; ++e2) {
             float x[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int j = 32 * ch + 8 * c8 + 2 * e2 + e;
-              const float f = qd == 3 && ch == 0 ? ci * gt.cross[j] : exp_neg((hi - gt.hi[j]) + (lo - gt.lo[j]));
+              const int j = j0 + 8 * c8 + 2 * e2 + e;
+              const float f = cross ? ci * gt.cross[j] : exp_neg((hi - gt.hi[j]) + (lo - gt.lo[j]));
               x[e] = j <= upto ? __uint_as_float(r[8 * c8 + 2 * e2 + e]) * f : 0.f;
             }
             pk[e2] = pack_bf2(x[0], x[1]);
           }
-          *reinterpret_cast<uint4*>(swz(pt, i, 4 * ch + c8)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-        }
-      }
-      if (warp != 2 && warp != 7) {
-        // ---- Q' over Q, its second part behind: the six warps that form no exponentials
-        const int me = (warp - (warp > 2)) * 32 + lane;
-        for (int i = me; i < C * 16; i += 6 * 32) {
-          const int t = i >> 4, c = i & 15, at = c >> 3;
-          uint8_t* p = swz(kq + at * 16384 + 8192, t, c & 7);
-          uint4 y[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-          if (t < live) split8(*reinterpret_cast<const uint4*>(p), gt.from_start[t], y);
-          *reinterpret_cast<uint4*>(p) = y[0];
-          *reinterpret_cast<uint4*>(swz(ql + at * 8192, t, c & 7)) = y[1];
+          *reinterpret_cast<uint4*>(swz(pt, i, (j0 >> 3) + c8)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
         }
       }
     }
+    if (OUT) mma_phase ^= 1;
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
     if (*abort_flag) break;
-    // ---- MMA2, MMA3, MMA4
+    // ---- MMA2, MMA4, MMA3; K has been read by every thread and by MMA1, the other V by the last chunk's products
     if (warp == 1) {
       tc_fence_after();
       const bool issuer = elect_one();
-      if (MODE != STATES) {
-        constexpr uint32_t id2 = idesc_bf16(128, 64), id3 = idesc_bf16(128, 64) | A_MN;
+      if (more) load_k(c0 + C, issuer);
+      if (OUT) {
+        constexpr uint32_t id2 = idesc_bf16(128, 64);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t b0 = sw128_desc(kq_a + 8192 + (kk >> 2) * 16384 + 32 * (kk & 3));
-          const uint64_t b1 = sw128_desc(ql_a + (kk >> 2) * 8192 + 32 * (kk & 3));
-          if (issuer) {
-            w4t::tc_mma_ts(tmem + TM_D, tmem + TM_B + 8 * kk, b0, id2, kk != 0);
-            w4t::tc_mma_ts(tmem + TM_D, tmem + TM_B + 8 * kk, b1, id2, 1);
-          }
+          const uint64_t b = sw128_desc(kq_a + 8192 + (kk >> 2) * 16384 + 32 * (kk & 3));
+          if (issuer) w4t::tc_mma_ts(tmem + TM_D, tmem + TM_B + 8 * kk, b, id2, kk != 0);
         }
-#pragma unroll
-        for (int kk = 0; kk < C / 16; ++kk) {
-          const uint64_t av = mn_desc(vb_a + kk * 2048, 8192), b0 = sw128_desc(pt_a + 32 * kk);
-          if (issuer) tc_mma_bf16(tmem + TM_D, av, b0, id3, 1);
-        }
+        if (issuer) tc_commit(d_bar);
+        __syncwarp();
       }
+      mbar_wait(v_bar, phase, abort_flag, err, 54);
+      __syncwarp();
+      tc_fence_after();
+      if (TWO_V && more) load_v(c0 + C, set ^ 1, issuer);   // its barrier's phase is over
+      const uint32_t v_a = smem_u32(sm + v_place(set));
+      const uint32_t step = v_step(set);
       constexpr uint32_t id4 = idesc_bf16(128, 128) | A_MN | B_MN;
 #pragma unroll
       for (int kk = 0; kk < C / 16; ++kk) {
-        const uint64_t av = mn_desc(vb_a + kk * 2048, 8192);
-        const uint64_t b0 = mn_desc(kq_a + kk * 2048, 16384), b1 = mn_desc(km_a + kk * 2048, 8192),
-                       b2 = mn_desc(kl_a + kk * 2048, 8192);
-        if (issuer) {
-          tc_mma_bf16(tmem + TM_S, av, b2, id4, 1);   // the small parts first
-          tc_mma_bf16(tmem + TM_S, av, b1, id4, 1);
-          if (PARTS == 3) tc_mma_bf16(tmem + TM_S, av, b0, id4, 1);
+        const uint64_t av = mn_desc(v_a + kk * 2048, step);
+#pragma unroll
+        for (int p = PARTS - 1; p >= 0; --p) {   // the small parts first
+          const uint64_t b = mn_desc(kd_a + p * TILE + kk * 2048, 8192);
+          if (issuer) tc_mma_bf16(tmem + TM_S, av, b, id4, 1);
+        }
+      }
+      if (OUT) {
+        mbar_wait(d_bar, phase, abort_flag, err, 55);   // MMA2 has read the state's copy: E goes there
+        __syncwarp();
+        tc_fence_after();
+        if (more) load_q(c0 + C, issuer);
+        constexpr uint32_t id3 = idesc_bf16(128, 64) | A_MN;
+#pragma unroll
+        for (int kk = 0; kk < C / 16; ++kk) {
+          const uint64_t av = mn_desc(v_a + kk * 2048, step), b = sw128_desc(pt_a + 32 * kk);
+          if (issuer) tc_mma_bf16(tmem + TM_B, av, b, id3, kk != 0);
         }
       }
       if (issuer) tc_commit(mma_bar);
@@ -381,49 +431,71 @@ __global__ void __launch_bounds__(THREADS, 2)
       g0 = gate(c0 + 2 * C + lane);
       g1 = gate(c0 + 2 * C + 32 + lane);
     }
-    set ^= 1;
     mbar_wait(mma_bar, mma_phase, abort_flag, err, 51);
     mma_phase ^= 1;
     tc_fence_after();
-    if (tid == 0 && more) load(c0 + C);   // every tile has been read
-    if (MODE != STATES) {
-      // ---- O^T -> bf16 -> the output tile over Q's second part, laid out as the loads -> TMA store
-      uint32_t r[32];
-      tmem_ld32(tmem + lane_bits + TM_D + 32 * ch, r);
-      tc_wait_ld();
+    if (!TWO_V && warp == 1 && more) {
+      load_v(c0 + C, set ^ 1, elect_one());
+      __syncwarp();
+    }
+    if (OUT) {
+      // ---- O^T = e^gc D + E -> bf16 -> the output tile over Kd, laid out as the loads -> TMA store
       const float scale = rsqrtf((float)D);
-      __nv_bfloat16* ot = reinterpret_cast<__nv_bfloat16*>(ql + (L >> 6) * 8192);
-      const int cl = L & 63;
+      const int tq = lane & 3;
+      uint32_t pk[4][4];   // 8 tokens each: the warp's four groups of 8 channels
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const int t = 32 * ch + e;
-        ot[(sw128_offset(t, cl >> 3) >> 1) + (cl & 7)] = f2bf(t < live ? __uint_as_float(r[e]) * scale : 0.f);
+      for (int hf = 0; hf < 2; ++hf) {
+        uint32_t d[16], e[16];
+        const uint32_t ta = tmem + lane_bits + ((uint32_t)(16 * hf) << 16) + 32 * ch;
+        tmem_ld_frag(ta + TM_D, d);
+        tmem_ld_frag(ta + TM_B, e);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = 32 * ch + 8 * i + 2 * tq;
+          const float f0 = gt.from_start[t], f1 = gt.from_start[t + 1];
+          const float s0 = t < live ? scale : 0.f, s1 = t + 1 < live ? scale : 0.f;
+#pragma unroll
+          for (int g8 = 0; g8 < 2; ++g8) {
+            const float x = fmaf(f0, __uint_as_float(d[4 * i + 2 * g8]), __uint_as_float(e[4 * i + 2 * g8]));
+            const float y = fmaf(f1, __uint_as_float(d[4 * i + 2 * g8 + 1]), __uint_as_float(e[4 * i + 2 * g8 + 1]));
+            pk[i][2 * hf + g8] = pack_bf2(s0 != 0.f ? x * s0 : 0.f, s1 != 0.f ? y * s1 : 0.f);
+          }
+        }
       }
+      const int c = 32 * qd + 8 * (lane >> 3);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        st_frags_trans(smem_u32(swz(ot + (c >> 6) * 8192, 32 * ch + 8 * i + (lane & 7), (c & 63) >> 3)), pk[i][0],
+                       pk[i][1], pk[i][2], pk[i][3]);
       fence_proxy_async_smem();
       tc_fence_before();
     }
     __syncthreads();
     if (*abort_flag) break;
-    if (MODE != STATES && tid == 0) {
-      tma_store_4d(&tm_o, ql, 0, h, c0, row);
-      tma_store_4d(&tm_o, ql + 8192, 64, h, c0, row);
+    if (OUT && tid == 0) {
+      tma_store_4d(&tm_o, ot, 0, h, c0, row);
+      tma_store_4d(&tm_o, ot + 8192, 64, h, c0, row);
       tma_store_commit();
     }
+    set ^= 1;
+    phase ^= 1;
     if (more) turn_state(whole[set]);
   }
   const bool ok = *abort_flag == 0;
-  if (tid == 0) {
-    if (MODE != STATES) tma_store_wait_all();
-    // a CTA that gave up waits (bounded) for the copies it issued before its shared memory goes away: without its own
-    // arrival their phase may never end, so it arrives first
-    if (!ok && issued) {
-      mbar_arrive(in_bar);
-      const uint64_t t0 = global_ns();
-      while (!mbar_try_wait(in_bar, (issued - 1) & 1) && global_ns() - t0 < kWaitNs) {
-      }
+  if (OUT && tid == 0) tma_store_wait_all();
+  if (!ok && warp == 1) {
+    // a CTA that gave up waits (bounded) for the copies it issued before its shared memory goes away: without the
+    // other arrival K's phase may never end, so it arrives first
+    if (lane == 0 && k_issued) mbar_arrive(k_bar);
+    const uint64_t t0 = global_ns();
+    while (((k_issued && !mbar_try_wait(k_bar, (k_issued - 1) & 1)) ||
+            (q_issued && !mbar_try_wait(q_bar, (q_issued - 1) & 1)) ||
+            (v_issued && !mbar_try_wait(v_bar, (v_issued - 1) & 1))) &&
+           global_ns() - t0 < kWaitNs) {
     }
   }
-  if (MODE != STATES) {   // chunks that hold padding only
+  if (OUT) {   // chunks that hold padding only
     const int first = max(begin, (work + C - 1) / C * C);
     for (int i = first * 16 + tid; i < end * 16; i += THREADS)
       reinterpret_cast<uint4*>(a.o + row * a.o_row + (int64_t)(i >> 4) * a.o_tok + h * D)[i & 15] =
