@@ -3,8 +3,8 @@
 //   O = scale ((e^gc Q) S + (Q K^T ∘ Γ, causal) V),   Γ_ij = e^{gc_i - gc_j},
 //   S <- e^gl S + (e^{gl - gc} K)^T V,
 // every product an M = 128 MMA with the transposed state S^T (lanes: value columns) in tensor memory:
-//   MMA1  D = [K; Q] K^T              (lanes 64-127: Q K^T; the stacked A is the K and Q tiles laid out back to back)
-//   MMA2  D = bf16(S^T) Q^T           (A in tensor memory)
+//   MMA1  D = bf16(S^T) Q^T           (A in tensor memory)
+//   MMA2  E = [K; Q] K^T              (lanes 64-127: Q K^T; the stacked A is the K and Q tiles laid out back to back)
 //   MMA3  E = V^T P^T                 (P = bf16(Q K^T ∘ Γ)); O^T = e^gc D + E, a factor for each of D's columns
 //   MMA4  S^T += V^T Kd               (Kd = e^{gl - gc} K in bf16 parts, S^T scaled by e^gl beforehand)
 // Rounding: the state is fp32 and what enters it keeps 24 bits (three bf16 parts of a decayed key, the value exact).
@@ -13,14 +13,19 @@
 // of decays are fp64, their differences rounded to fp32 once, so that a strong decay early in a chunk takes no accuracy
 // from the tokens behind it (-inf is held as -10000, whose exponential is 0).
 //
-// Tensor memory, 256 columns: S^T 0-127, its bf16 copy 128-191 (E once MMA2 has read it), D 192-255. Shared memory 107
-// KB: two CTAs per SM, whose phases (TMA, tensor core, CUDA cores) fill each other's waits. Within a chunk the warps of
-// lanes 64-127 form P (of Γ's four 32 x 32 blocks one is zero, one a product of two vectors, two need exponentials) and
-// the others most of Kd; the next chunk's gates are formed and its K and V fetched while MMA2-4 run, its Q once MMA2 is
-// done. Two block barriers a chunk. A (row, head) is one CTA, or, where those are fewer than the CTAs that fit, is cut
-// into segments of whole chunks: a first launch leaves each segment's own contribution to the state in scratch (no Q,
-// no outputs), a second turns these into the state ahead of each segment and the final one, the third computes the
-// outputs. Waits are bounded (%globaltimer, 2 s): on expiry the CTA records JB_DEV_TIMEOUT | 50.. in the device status
+// Tensor memory, 256 columns: S^T 0-127, its bf16 copy 128-191 (E once MMA1 has read it), D 192-255. Shared memory 108
+// KB: two CTAs per SM, whose phases (TMA, tensor core, CUDA cores) fill each other's waits. Within a chunk Kd and the
+// next chunk's gates are formed while MMA1 and MMA2 run, P by the warps of lanes 64-127 (of Γ's four 32 x 32 blocks one
+// is zero, one a product of two vectors, two need exponentials), and the outputs leave while MMA4 runs; the next tiles
+// are fetched as soon as theirs have been read. A (row, head) is one CTA, or, where those are fewer than the CTAs that
+// fit, is cut into segments of whole chunks: a first launch leaves each segment's own contribution to the state in
+// scratch (no Q, no outputs; from the last chunk to the first, Kd = e^{decay to the segment's end} K, so that the sum
+// in tensor memory is never touched), a second turns these into the state ahead of each segment and the final one, the
+// third computes the outputs. Three bounds were measured on the way: the tensor core needs 65 cycles for an M128 N128
+// K16 product and 49 for N64, 1500 a chunk with outputs and 780 without, against HBM's 2800 and 1400; a batch of
+// products waited for costs another 540 cycles, the gates' chain of sums and exponentials 1200, so what bounds a chunk is
+// its chain of phases.
+// Waits are bounded (%globaltimer, 2 s): on expiry the CTA records JB_DEV_TIMEOUT | 50.. in the device status
 // word and returns.
 
 namespace jb {
@@ -28,7 +33,6 @@ namespace lintc {
 
 using gdnt::A_MN;
 using gdnt::B_MN;
-using gdnt::exp_neg;
 using gdnt::mn_desc;
 using gdnt::swz;
 using gdnt::tc_wait_st;
@@ -40,12 +44,12 @@ constexpr int C = 64, THREADS = 256;
 constexpr uint32_t TILE = C * D * 2;   // 16 KB: two 64-column atoms of 64 rows x 128 B
 constexpr int OFF_KQ = 0;              // atom a: K at a * 16384, Q at + 8192 (no Q: the second V)
 constexpr int OFF_K0 = 32768, OFF_K1 = OFF_K0 + TILE;   // the parts of Kd (atoms 8192 apart); over the first then the
-constexpr int OFF_K2 = OFF_K1 + TILE;  // output tile. The third part, or with two the second V
+constexpr int OFF_K2 = OFF_K1 + TILE;  // output tile. The third part, or with two the output tile
 constexpr int OFF_V = OFF_K2 + TILE;
 constexpr int OFF_P = OFF_V + TILE;    // 64 rows x 128 B
 constexpr int OFF_G = OFF_P + TILE / 2;   // two sets of gates
-constexpr int OFF_MISC = OFF_G + 2 * 5 * C * 4;
-constexpr int ALLOC = OFF_MISC + 64;
+constexpr int OFF_MISC = OFF_G + 2 * 7 * C * 4;
+constexpr int ALLOC = OFF_MISC + 80;
 static_assert(2 * (ALLOC + 1024) <= 228 * 1024, "two CTAs per SM");
 constexpr uint32_t TM_S = 0, TM_B = 128, TM_D = 192, TM_COLS = 256;
 constexpr int FIT = 2 * 148;           // CTAs that run at once
@@ -115,14 +119,27 @@ __device__ __forceinline__ void st_frags_trans(uint32_t addr, uint32_t a, uint32
                : "memory");
 }
 
-// A chunk's gates, from the sums gc of its log-decays: gc in two floats (their differences are the exponents inside the
-// chunk), e^gc, e^{gl - gc}, and Γ's lower left 32 x 32 block as cross[32 + i] cross[j].
+// A chunk's gates, from the sums gc of its log-decays: in base 2 as two floats (their differences are the exponents
+// inside the chunk), e^gc, e^{gl - gc} (and its two bf16 parts, each twice), and Γ's lower left 32 x 32 block as
+// cross[32 + i] cross[j].
 struct Gates {
   float hi[C], lo[C], from_start[C], to_end[C], cross[C];
+  uint2 parts[C];
 };
 
-__device__ __forceinline__ void form_gates(Gates& g, float a, float b, int lane, volatile float* whole, double& sum) {
-  double x = a < -1e4f ? -1e4f : a, y = b < -1e4f ? -1e4f : b;   // tokens lane and lane + 32
+__device__ __forceinline__ float exp2_fast(float x) {   // ex2.approx: 2 ulp
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// One of two warps' half of a chunk's gates; a, b: the log-decays of tokens lane and lane + 32, in: the decay (base 2)
+// already in `carry`, which grows by the chunk's. ONLY_END: `to_end` alone, and to `carry`'s end.
+template <bool ONLY_END>
+__device__ __forceinline__ void form_gates(Gates& g, int half, float a, float b, int lane, volatile float* whole,
+                                           double& carry) {
+  constexpr double L2E = 1.4426950408889634;
+  double x = (a < -1e4f ? -1e4f : a) * L2E, y = (b < -1e4f ? -1e4f : b) * L2E;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const double yx = __shfl_up_sync(0xffffffffu, x, off), yy = __shfl_up_sync(0xffffffffu, y, off);
@@ -134,19 +151,47 @@ __device__ __forceinline__ void form_gates(Gates& g, float a, float b, int lane,
   const double mid = __shfl_sync(0xffffffffu, x, 31);
   y += mid;
   const double all = __shfl_sync(0xffffffffu, y, 31);
-  g.hi[lane] = (float)x;
-  g.hi[lane + 32] = (float)y;
-  g.lo[lane] = (float)(x - (double)(float)x);
-  g.lo[lane + 32] = (float)(y - (double)(float)y);
-  g.from_start[lane] = expf((float)x);
-  g.from_start[lane + 32] = expf((float)y);
-  g.to_end[lane] = expf((float)(all - x));
-  g.to_end[lane + 32] = expf((float)(all - y));
-  g.cross[lane] = expf((float)(mid - x));
-  g.cross[lane + 32] = expf((float)(y - mid));
-  if (lane == 0) *whole = expf((float)all);
-  sum += all;
+  const double z = half ? y : x;
+  const int t = lane + 32 * half;
+  const float f = exp2_fast((float)(ONLY_END ? carry + (all - z) : all - z));
+  g.to_end[t] = f;
+  if (!ONLY_END) {
+    const float hi = (float)z;
+    g.hi[t] = hi;
+    g.lo[t] = (float)(z - (double)hi);
+    g.from_start[t] = exp2_fast(hi);
+    const uint32_t f0 = pack_bf2(f, f), f1 = pack_bf2(f - bf_lo(f0), f - bf_lo(f0));
+    g.parts[t] = make_uint2(f0, f1);
+    g.cross[t] = exp2_fast((float)(half ? z - mid : mid - z));
+    if (lane == 0 && half == 0) *whole = exp2_fast((float)all);
+  }
+  carry += all;
 }
+
+// eight bf16 values x times f = f0 + f1 in two bf16 parts, on bf16 pairs: x f0 = p + r exactly (16 bits in two bf16
+// values), and the second part r + x f1 rounded once: 2^-17 of the product
+__device__ __forceinline__ void split8_pairs(const uint4& x, uint2 f, uint4& y0, uint4& y1) {
+  const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+  uint32_t p0[4], p1[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t n;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(p0[i]) : "r"(in[i]), "r"(f.x));
+    n = p0[i] ^ 0x80008000u;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(n) : "r"(in[i]), "r"(f.x), "r"(n));
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(p1[i]) : "r"(in[i]), "r"(f.y), "r"(n));
+  }
+  y0 = make_uint4(p0[0], p0[1], p0[2], p0[3]);
+  y1 = make_uint4(p1[0], p1[1], p1[2], p1[3]);
+}
+template <int N>
+struct Count {
+  static constexpr int value = N;
+};
+template <bool B>
+struct Bool {
+  static constexpr bool value = B;
+};
 
 template <int MODE>
 __global__ void __launch_bounds__(THREADS, 2)
@@ -156,20 +201,23 @@ __global__ void __launch_bounds__(THREADS, 2)
   pdl_begin();
   constexpr bool OUT = MODE != STATES;
   constexpr int PARTS = MODE == OUTPUTS ? 2 : 3;   // of Kd
-  constexpr bool TWO_V = MODE != WHOLE;            // a second V tile: the next chunk's comes early
   extern __shared__ __align__(1024) uint8_t sm[];
   uint8_t* kq = sm + OFF_KQ;
   uint8_t* pt = sm + OFF_P;
-  uint8_t* ot = sm + OFF_K0;
+  // the outputs' tile: with two parts of Kd a place of its own, so that they leave while MMA4 runs
+  constexpr bool EARLY = MODE == OUTPUTS;
+  uint8_t* ot = sm + (EARLY ? OFF_K2 : OFF_K0);
   Gates* gates = reinterpret_cast<Gates*>(sm + OFF_G);
-  uint64_t* mma_bar = reinterpret_cast<uint64_t*>(sm + OFF_MISC);   // MMA1, MMA2-4 of a chunk in turn
-  uint64_t* d_bar = mma_bar + 1;                                    // MMA2
-  uint64_t* k_bar = mma_bar + 2;
-  uint64_t* q_bar = mma_bar + 3;
-  uint64_t* v_bar = mma_bar + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + OFF_MISC + 40);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + OFF_MISC + 44);
-  volatile float* whole = reinterpret_cast<volatile float*>(sm + OFF_MISC + 48);   // [2] the chunks' decay factors
+  uint64_t* d_bar = reinterpret_cast<uint64_t*>(sm + OFF_MISC);   // MMA1; MMA2; MMA3 (EARLY); every product
+  uint64_t* p_bar = d_bar + 1;
+  uint64_t* e_bar = d_bar + 2;
+  uint64_t* all_bar = d_bar + 3;
+  uint64_t* k_bar = d_bar + 4;
+  uint64_t* q_bar = d_bar + 5;
+  uint64_t* v_bar = d_bar + 6;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + OFF_MISC + 56);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + OFF_MISC + 60);
+  volatile float* whole = reinterpret_cast<volatile float*>(sm + OFF_MISC + 64);   // [2] the chunks' decay factors
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int qd = warp & 3, ch = warp >> 2;
@@ -180,227 +228,257 @@ __global__ void __launch_bounds__(THREADS, 2)
   const int stop = a.real ? min(max(a.real[row], 0), a.n) : a.n;
   const int begin = part * seg.chunks * C, end = min(begin + seg.chunks * C, a.n);
   const int work = min(end, stop);   // tokens past it are padding: zeros out, the state stays
+  const int chunks = begin < work ? (work - begin + C - 1) / C : 0;
   if (smem_u32(sm) & 1023) {         // the swizzled tiles' base
     if (tid == 0) atomicCAS(err, 0, JB_DEV_LAUNCH | 50);
     return;
   }
+  auto start_of = [&](int i) { return begin + (OUT ? i : chunks - 1 - i) * C; };   // the first token of chunk i
 
   if (tid == 0) {
-    mbar_init(mma_bar, 1);
-    mbar_init(d_bar, 1);
-    mbar_init(k_bar, 2);   // the load, and that the previous output tile has left its place
-    mbar_init(q_bar, 1);
-    mbar_init(v_bar, 1);
+    for (int i = 0; i < 7; ++i) mbar_init(d_bar + i, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 0) {
+  if (warp == 1) {
     tmem_alloc(tmem_slot, TM_COLS);
     tmem_relinquish();
   }
-  // the place of the V tile of a chunk (its atoms v_step apart); tile loads, all issued by one lane of warp 1 at a time
-  constexpr int V2 = MODE == STATES ? OFF_KQ + 8192 : OFF_K2;
-  auto v_place = [&](int odd) { return TWO_V && odd ? V2 : OFF_V; };
-  auto v_step = [&](int odd) { return MODE == STATES && odd ? 16384 : 8192; };
+  // tile loads, all issued by one lane of warp 0; without Q the V tiles alternate between two places
+  auto v_place = [&](int odd) { return !OUT && odd ? OFF_KQ + 8192 : OFF_V; };
+  auto v_step = [&](int odd) { return !OUT && odd ? 16384 : 8192; };   // between its atoms
   int k_issued = 0, q_issued = 0, v_issued = 0;
-  auto load_k = [&](int c0, bool me) {
+  auto load_k = [&](int i, bool me) {
     ++k_issued;
     if (!me) return;
     mbar_arrive_expect_tx(k_bar, TILE);
-    tma_load_4d(kq, &tm_k, k_bar, 0, h, c0, row);
-    tma_load_4d(kq + 16384, &tm_k, k_bar, 64, h, c0, row);
+    tma_load_4d(kq, &tm_k, k_bar, 0, h, start_of(i), row);
+    tma_load_4d(kq + 16384, &tm_k, k_bar, 64, h, start_of(i), row);
   };
-  auto load_q = [&](int c0, bool me) {
+  auto load_q = [&](int i, bool me) {
     ++q_issued;
     if (!me) return;
     mbar_arrive_expect_tx(q_bar, TILE);
-    tma_load_4d(kq + 8192, &tm_q, q_bar, 0, h, c0, row);
-    tma_load_4d(kq + 16384 + 8192, &tm_q, q_bar, 64, h, c0, row);
+    tma_load_4d(kq + 8192, &tm_q, q_bar, 0, h, start_of(i), row);
+    tma_load_4d(kq + 16384 + 8192, &tm_q, q_bar, 64, h, start_of(i), row);
   };
-  auto load_v = [&](int c0, int odd, bool me) {
+  auto load_v = [&](int i, bool me) {
     ++v_issued;
     if (!me) return;
-    uint8_t* to = sm + v_place(odd);
+    uint8_t* to = sm + v_place(i & 1);
     mbar_arrive_expect_tx(v_bar, TILE);
-    tma_load_4d(to, &tm_v, v_bar, 0, h, c0, row);
-    tma_load_4d(to + v_step(odd), &tm_v, v_bar, 64, h, c0, row);
+    tma_load_4d(to, &tm_v, v_bar, 0, h, start_of(i), row);
+    tma_load_4d(to + v_step(i & 1), &tm_v, v_bar, 64, h, start_of(i), row);
   };
   const float* gp = a.g + row * a.g_row + h;
-  auto gate = [&](int t) { return t < work ? gp[t * a.g_tok] : 0.f; };   // 0 past the row's end
-  double decays = 0.0;   // warp 0: the segment's log-decay
-  float g0 = 0.f, g1 = 0.f;
-  if (warp == 0) {
-    g0 = gate(begin + lane);
-    g1 = gate(begin + 32 + lane);
-  }
-  tc_fence_before();
+  float g0 = 0.f, g1 = 0.f;   // warps 0 and 4: the log-decays of the next chunk's tokens, 0 past the row's end
+  auto gates_of = [&](int i) {
+    const int t = start_of(i) + lane;
+    g0 = i < chunks && t < work ? gp[t * a.g_tok] : 0.f;
+    g1 = i < chunks && t + 32 < work ? gp[(t + 32) * a.g_tok] : 0.f;
+  };
+  double carry = 0.0;         // the same warps: log-decays so far
+  if (qd == 0) gates_of(0);
   __syncthreads();
-  tc_fence_after();
-  if (warp == 1 && begin < work) {
+  if (warp == 0 && chunks) {
     const bool me = elect_one();
-    load_k(begin, me);
-    if (OUT) load_q(begin, me);
-    load_v(begin, 0, me);
+    load_k(0, me);
+    if (OUT) load_q(0, me);
+    load_v(0, me);
     __syncwarp();
   }
-  const uint32_t tmem = *tmem_slot;
-  if (warp == 0) {
-    form_gates(gates[0], g0, g1, lane, whole, decays);
-    g0 = gate(begin + C + lane);
-    g1 = gate(begin + C + 32 + lane);
+  // the state ahead of the segment, its loads in flight while the first gates are formed
+  const float* in = MODE == WHOLE ? lin::state_in(a.pool, row, h)
+                    : MODE == OUTPUTS ? seg.states + ((int64_t)pair * seg.count + part) * STATE : nullptr;
+  uint32_t r[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i] = in ? __float_as_uint(in[(ch * 64 + i) * D + L]) : 0u;
+  if (qd == 0) {
+    form_gates<!OUT>(gates[0], ch, g0, g1, lane, whole, carry);
+    gates_of(1);
   }
   if (OUT)   // P's upper right block is never anything else
     for (int i = tid; i < 32 * 4; i += THREADS)
       *reinterpret_cast<uint4*>(swz(pt, i >> 2, 4 + (i & 3))) = make_uint4(0, 0, 0, 0);
-
-  // the state ahead of the segment: lane = value column, columns = key rows
-  {
-    const float* in = MODE == WHOLE ? lin::state_in(a.pool, row, h)
-                      : MODE == OUTPUTS ? seg.states + ((int64_t)pair * seg.count + part) * STATE : nullptr;
-    for (int half = 0; half < 2; ++half) {
-      uint32_t r[32];
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // lane = value column, columns = key rows: into tensor memory, scaled for the first chunk, and its bf16 copy
+  const uint32_t s_at = tmem + lane_bits + TM_S + 64 * ch, b_at = tmem + lane_bits + TM_B + 32 * ch;
+  auto put_state = [&](int half, float el) {
+    if (OUT) {
+      uint32_t b[16];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) r[i] = in ? __float_as_uint(in[(ch * 64 + half * 32 + i) * D + L]) : 0u;
-      tmem_st32(tmem + lane_bits + TM_S + ch * 64 + half * 32, r);
-    }
-    tc_wait_st();
-  }
-  // the state's bf16 copy, then its decay over the chunk
-  auto turn_state = [&](float el) {
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const uint32_t ta = tmem + lane_bits + TM_S + 64 * ch + 32 * half;
-      uint32_t r[32];
-      tmem_ld32(ta, r);
-      tc_wait_ld();
-      if (OUT) {
-        uint32_t b[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) b[e] = pack_bf2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
-        tmem_st16(tmem + lane_bits + TM_B + 32 * ch + 16 * half, b);
-      }
+      for (int e = 0; e < 16; ++e) b[e] = pack_bf2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+      tmem_st16(b_at + 16 * half, b);
 #pragma unroll
       for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * el);
-      tmem_st32(ta, r);
     }
-    tc_wait_st();
+    tmem_st32(s_at + 32 * half, r);
   };
+  {
+    const float el = OUT && chunks ? whole[0] : 1.f;
+    put_state(0, el);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = in ? __float_as_uint(in[(ch * 64 + 32 + i) * D + L]) : 0u;
+    put_state(1, el);
+    tc_wait_st();
+  }
+  tc_fence_before();
   __syncthreads();
-  if (begin < work) turn_state(whole[0]);
 
   const uint32_t kq_a = smem_u32(kq), kd_a = smem_u32(sm + OFF_K0), pt_a = smem_u32(pt);
-  uint32_t mma_phase = 0, phase = 0, set = 0;   // set: the chunk's parity
-  for (int c0 = begin; c0 < work; c0 += C) {
-    const int live = min(C, work - c0);
-    const bool more = c0 + C < work;
+  uint32_t phase = 0;
+  for (int c = 0; c < chunks; ++c, phase ^= 1) {
+    const int set = c & 1, live = min(C, work - start_of(c));
+    const bool more = c + 1 < chunks;
     const Gates& gt = gates[set];
-    if (tid == 0) {
-      if (OUT) tma_store_wait_read();
-      mbar_arrive(k_bar);
-    }
-    mbar_wait(k_bar, phase, abort_flag, err, 52);
-    // ---- MMA1
+    // ---- MMA1, then, where it has read the state's copy, MMA2
     if (OUT && warp == 1) {
       mbar_wait(q_bar, phase, abort_flag, err, 53);
       __syncwarp();
       tc_fence_after();
-      constexpr uint32_t id1 = idesc_bf16(128, 64);
+      constexpr uint32_t id = idesc_bf16(128, 64);
       const bool issuer = elect_one();
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        const uint64_t dsc = sw128_desc(kq_a + (kk >> 2) * 16384 + 32 * (kk & 3));
-        if (issuer) tc_mma_bf16(tmem + TM_D, dsc, dsc, id1, kk != 0);
+        const uint64_t b = sw128_desc(kq_a + 8192 + (kk >> 2) * 16384 + 32 * (kk & 3));
+        if (issuer) w4t::tc_mma_ts(tmem + TM_D, tmem + TM_B + 8 * kk, b, id, kk != 0);
       }
-      if (issuer) tc_commit(mma_bar);
+      if (issuer) tc_commit(d_bar);
       __syncwarp();
+      mbar_wait(k_bar, phase, abort_flag, err, 52);
+      mbar_wait(d_bar, phase, abort_flag, err, 55);
+      __syncwarp();
+      tc_fence_after();
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint64_t dsc = sw128_desc(kq_a + (kk >> 2) * 16384 + 32 * (kk & 3));
+        if (issuer) tc_mma_bf16(tmem + TM_B, dsc, dsc, id, kk != 0);
+      }
+      if (issuer) tc_commit(p_bar);
+      __syncwarp();
+    }
+    // ---- warps 0 and 4: the next chunk's gates, and the decays of the one after it
+    if (qd == 0 && more) {
+      form_gates<!OUT>(gates[set ^ 1], ch, g0, g1, lane, whole + (set ^ 1), carry);
+      gates_of(c + 2);
     }
     // values past the row's end may be anything: zeros, so that a zero weight keeps them out
     if (live < C) {
       mbar_wait(v_bar, phase, abort_flag, err, 54);
       for (int i = tid; i < (C - live) * 16; i += THREADS) {
-        const int t = live + (i >> 4), c = i & 15;
-        *reinterpret_cast<uint4*>(swz(sm + v_place(set) + (c >> 3) * v_step(set), t, c & 7)) = make_uint4(0, 0, 0, 0);
+        const int t = live + (i >> 4), x = i & 15;
+        *reinterpret_cast<uint4*>(swz(sm + v_place(set) + (x >> 3) * v_step(set), t, x & 7)) = make_uint4(0, 0, 0, 0);
       }
     }
-    // ---- Kd, a 16-byte piece of a token at a time: six for the warps of lanes 0-63, two for those that form P
-    auto form_kd = [&](int i) {
-      const int t = i >> 4, c = i & 15, at = c >> 3;
-      uint4 y[PARTS];
+    // ---- Kd, 16-byte pieces of the tokens' keys: five a thread of the warps that form P, six of warps 1 and 5
+    auto form_kd = [&](auto count, int first, int step) {   // its loads ahead of its stores
+      constexpr int N = decltype(count)::value;
+      mbar_wait(k_bar, phase, abort_flag, err, 52);
+      uint4 x[N];
 #pragma unroll
-      for (int p = 0; p < PARTS; ++p) y[p] = make_uint4(0, 0, 0, 0);
-      if (t < live) split8(*reinterpret_cast<const uint4*>(swz(kq + at * 16384, t, c & 7)), gt.to_end[t], y);
+      for (int it = 0; it < N; ++it) {
+        const int i = min(first + it * step, C * 16 - 1), t = i >> 4, p = i & 15;
+        x[it] = *reinterpret_cast<const uint4*>(swz(kq + (p >> 3) * 16384, t, p & 7));
+      }
 #pragma unroll
-      for (int p = 0; p < PARTS; ++p)
-        *reinterpret_cast<uint4*>(swz(sm + OFF_K0 + p * TILE + at * 8192, t, c & 7)) = y[p];
+      for (int it = 0; it < N; ++it) {
+        const int i = first + it * step, t = min(i >> 4, C - 1), p = i & 15;
+        uint4 y[PARTS];
+        if constexpr (PARTS == 2) split8_pairs(x[it], gt.parts[t], y[0], y[1]);
+        else split8(x[it], gt.to_end[t], y);
+        if (i < C * 16)
+#pragma unroll
+          for (int u = 0; u < PARTS; ++u)
+            *reinterpret_cast<uint4*>(swz(sm + OFF_K0 + u * TILE + (p >> 3) * 8192, t, p & 7)) =
+                t < live ? y[u] : make_uint4(0, 0, 0, 0);
+      }
     };
     if (!OUT) {
-#pragma unroll
-      for (int it = 0; it < 4; ++it) form_kd(it * THREADS + tid);
-    } else if (qd < 2) {
-      const int me = (ch * 2 + qd) * 32 + lane;
-#pragma unroll
-      for (int it = 0; it < 6; ++it) form_kd(it * 128 + me);
-    } else {
-      const int me = (ch * 2 + qd - 2) * 32 + lane;
-#pragma unroll
-      for (int it = 6; it < 8; ++it) form_kd(it * 128 + me);
-      mbar_wait(mma_bar, mma_phase, abort_flag, err, 51);
+      if (qd > 0) form_kd(Count<6>(), (warp - 1 - (warp > 4)) * 32 + lane, 192);
+    } else if (qd == 1) {
+      form_kd(Count<6>(), 640 + ch * 32 + lane, 64);
+    } else if (qd >= 2) {
+      form_kd(Count<5>(), (2 * ch + qd - 2) * 32 + lane, 128);
+      mbar_wait(p_bar, phase, abort_flag, err, 51);
       tc_fence_after();
-      // ---- P from D's lanes 64-127: row i = L - 64; columns 16 ch .. + 15 of the left half, and for rows from 32 on
+      // ---- P from E's lanes 64-127: row i = L - 64; columns 16 ch .. + 15 of the left half, and for rows from 32 on
       // 32 + 16 ch .. + 15 too
       const int i = L - C;
       const float hi = gt.hi[i], lo = gt.lo[i], ci = gt.cross[i];
       const int upto = i < live ? i : -1;
-      for (int half = 0; half < (qd == 3 ? 2 : 1); ++half) {
-        const bool cross = qd == 3 && half == 0;
-        const int j0 = 32 * half + 16 * ch;
-        uint32_t r[16];
-        lsh::tmem_ld16(tmem + lane_bits + TM_D + j0, r);
-        tc_wait_ld();
+      uint32_t d[2][16];
+      lsh::tmem_ld16(tmem + lane_bits + TM_B + 16 * ch, d[0]);
+      if (qd == 3) lsh::tmem_ld16(tmem + lane_bits + TM_B + 32 + 16 * ch, d[1]);
+      tc_wait_ld();
+      auto form_p = [&](const uint32_t (&e)[16], int j0, auto cross) {
 #pragma unroll
         for (int c8 = 0; c8 < 2; ++c8) {
-          uint32_t pk[4];
+          float x[8];
 #pragma unroll
-          for (int e2 = 0; e2 < 4; ++e2) {
-            float x[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int j = j0 + 8 * c8 + 2 * e2 + e;
-              const float f = cross ? ci * gt.cross[j] : exp_neg((hi - gt.hi[j]) + (lo - gt.lo[j]));
-              x[e] = j <= upto ? __uint_as_float(r[8 * c8 + 2 * e2 + e]) * f : 0.f;
+          for (int e4 = 0; e4 < 2; ++e4) {
+            const int j = j0 + 8 * c8 + 4 * e4;
+            float f[4];
+            if constexpr (decltype(cross)::value) {
+              const float4 cj = *reinterpret_cast<const float4*>(&gt.cross[j]);
+              f[0] = ci * cj.x; f[1] = ci * cj.y; f[2] = ci * cj.z; f[3] = ci * cj.w;
+            } else {
+              const float4 hj = *reinterpret_cast<const float4*>(&gt.hi[j]);
+              const float4 lj = *reinterpret_cast<const float4*>(&gt.lo[j]);
+              f[0] = exp2_fast((hi - hj.x) + (lo - lj.x)); f[1] = exp2_fast((hi - hj.y) + (lo - lj.y));
+              f[2] = exp2_fast((hi - hj.z) + (lo - lj.z)); f[3] = exp2_fast((hi - hj.w) + (lo - lj.w));
             }
-            pk[e2] = pack_bf2(x[0], x[1]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              x[4 * e4 + u] = j + u <= upto ? __uint_as_float(e[8 * c8 + 4 * e4 + u]) * f[u] : 0.f;
           }
-          *reinterpret_cast<uint4*>(swz(pt, i, (j0 >> 3) + c8)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+          *reinterpret_cast<uint4*>(swz(pt, i, (j0 >> 3) + c8)) = make_uint4(
+              pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7]));
         }
+      };
+      if (qd == 2) {
+        form_p(d[0], 16 * ch, Bool<false>());
+      } else {
+        form_p(d[0], 16 * ch, Bool<true>());
+        form_p(d[1], 32 + 16 * ch, Bool<false>());
       }
     }
-    if (OUT) mma_phase ^= 1;
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
     if (*abort_flag) break;
-    // ---- MMA2, MMA4, MMA3; K has been read by every thread and by MMA1, the other V by the last chunk's products
-    if (warp == 1) {
-      tc_fence_after();
-      const bool issuer = elect_one();
-      if (more) load_k(c0 + C, issuer);
-      if (OUT) {
-        constexpr uint32_t id2 = idesc_bf16(128, 64);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t b = sw128_desc(kq_a + 8192 + (kk >> 2) * 16384 + 32 * (kk & 3));
-          if (issuer) w4t::tc_mma_ts(tmem + TM_D, tmem + TM_B + 8 * kk, b, id2, kk != 0);
-        }
-        if (issuer) tc_commit(d_bar);
-        __syncwarp();
+    // ---- the next tiles, each once its place has been read: K by every thread and by MMA2, Q by MMA1 and MMA2, the
+    // other V by the last chunk's products
+    if (warp == 0 && more) {
+      const bool me = elect_one();
+      load_k(c + 1, me);
+      if (OUT) load_q(c + 1, me);
+      if (!OUT) {
+        mbar_wait(v_bar, phase, abort_flag, err, 54);   // one load at a time on a barrier
+        load_v(c + 1, me);
       }
+      __syncwarp();
+    }
+    // ---- MMA3, MMA4
+    if (warp == 1) {
       mbar_wait(v_bar, phase, abort_flag, err, 54);
       __syncwarp();
       tc_fence_after();
-      if (TWO_V && more) load_v(c0 + C, set ^ 1, issuer);   // its barrier's phase is over
+      const bool issuer = elect_one();
       const uint32_t v_a = smem_u32(sm + v_place(set));
       const uint32_t step = v_step(set);
+      if (OUT) {
+        constexpr uint32_t id3 = idesc_bf16(128, 64) | A_MN;
+#pragma unroll
+        for (int kk = 0; kk < C / 16; ++kk) {
+          const uint64_t av = mn_desc(v_a + kk * 2048, step), b = sw128_desc(pt_a + 32 * kk);
+          if (issuer) tc_mma_bf16(tmem + TM_B, av, b, id3, kk != 0);
+        }
+        if (EARLY && issuer) tc_commit(e_bar);
+        __syncwarp();
+      }
       constexpr uint32_t id4 = idesc_bf16(128, 128) | A_MN | B_MN;
 #pragma unroll
       for (int kk = 0; kk < C / 16; ++kk) {
@@ -411,35 +489,18 @@ __global__ void __launch_bounds__(THREADS, 2)
           if (issuer) tc_mma_bf16(tmem + TM_S, av, b, id4, 1);
         }
       }
-      if (OUT) {
-        mbar_wait(d_bar, phase, abort_flag, err, 55);   // MMA2 has read the state's copy: E goes there
-        __syncwarp();
-        tc_fence_after();
-        if (more) load_q(c0 + C, issuer);
-        constexpr uint32_t id3 = idesc_bf16(128, 64) | A_MN;
-#pragma unroll
-        for (int kk = 0; kk < C / 16; ++kk) {
-          const uint64_t av = mn_desc(v_a + kk * 2048, step), b = sw128_desc(pt_a + 32 * kk);
-          if (issuer) tc_mma_bf16(tmem + TM_B, av, b, id3, kk != 0);
-        }
-      }
-      if (issuer) tc_commit(mma_bar);
+      if (issuer) tc_commit(all_bar);
       __syncwarp();
     }
-    if (warp == 0 && more) {   // the next chunk's gates, and the decays of the one after it
-      form_gates(gates[set ^ 1], g0, g1, lane, whole + (set ^ 1), decays);
-      g0 = gate(c0 + 2 * C + lane);
-      g1 = gate(c0 + 2 * C + 32 + lane);
-    }
-    mbar_wait(mma_bar, mma_phase, abort_flag, err, 51);
-    mma_phase ^= 1;
+    if (EARLY) mbar_wait(e_bar, phase, abort_flag, err, 56);
+    else mbar_wait(all_bar, phase, abort_flag, err, 57);
     tc_fence_after();
-    if (!TWO_V && warp == 1 && more) {
-      load_v(c0 + C, set ^ 1, elect_one());
+    if (MODE == WHOLE && warp == 0 && more) {
+      load_v(c + 1, elect_one());
       __syncwarp();
     }
     if (OUT) {
-      // ---- O^T = e^gc D + E -> bf16 -> the output tile over Kd, laid out as the loads -> TMA store
+      // ---- O^T = e^gc D + E -> bf16 -> the output tile, laid out as the loads -> TMA store
       const float scale = rsqrtf((float)D);
       const int tq = lane & 3;
       uint32_t pk[4][4];   // 8 tokens each: the warp's four groups of 8 channels
@@ -453,41 +514,58 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int t = 32 * ch + 8 * i + 2 * tq;
-          const float f0 = gt.from_start[t], f1 = gt.from_start[t + 1];
-          const float s0 = t < live ? scale : 0.f, s1 = t + 1 < live ? scale : 0.f;
+          const float2 f = *reinterpret_cast<const float2*>(&gt.from_start[t]);
 #pragma unroll
           for (int g8 = 0; g8 < 2; ++g8) {
-            const float x = fmaf(f0, __uint_as_float(d[4 * i + 2 * g8]), __uint_as_float(e[4 * i + 2 * g8]));
-            const float y = fmaf(f1, __uint_as_float(d[4 * i + 2 * g8 + 1]), __uint_as_float(e[4 * i + 2 * g8 + 1]));
-            pk[i][2 * hf + g8] = pack_bf2(s0 != 0.f ? x * s0 : 0.f, s1 != 0.f ? y * s1 : 0.f);
+            const float x = fmaf(f.x, __uint_as_float(d[4 * i + 2 * g8]), __uint_as_float(e[4 * i + 2 * g8])) * scale;
+            const float y =
+                fmaf(f.y, __uint_as_float(d[4 * i + 2 * g8 + 1]), __uint_as_float(e[4 * i + 2 * g8 + 1])) * scale;
+            pk[i][2 * hf + g8] = pack_bf2(t < live ? x : 0.f, t + 1 < live ? y : 0.f);
           }
         }
       }
-      const int c = 32 * qd + 8 * (lane >> 3);
+      const int x = 32 * qd + 8 * (lane >> 3);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        st_frags_trans(smem_u32(swz(ot + (c >> 6) * 8192, 32 * ch + 8 * i + (lane & 7), (c & 63) >> 3)), pk[i][0],
+        st_frags_trans(smem_u32(swz(ot + (x >> 6) * 8192, 32 * ch + 8 * i + (lane & 7), (x & 63) >> 3)), pk[i][0],
                        pk[i][1], pk[i][2], pk[i][3]);
       fence_proxy_async_smem();
       tc_fence_before();
+      __syncthreads();
+      if (*abort_flag) break;
+      if (tid == 0) {
+        tma_store_4d(&tm_o, ot, 0, h, start_of(c), row);
+        tma_store_4d(&tm_o, ot + 8192, 64, h, start_of(c), row);
+        tma_store_commit();
+      }
+      if (EARLY) {
+        mbar_wait(all_bar, phase, abort_flag, err, 57);
+        tc_fence_after();
+        if (warp == 0 && more) {
+          load_v(c + 1, elect_one());
+          __syncwarp();
+        }
+      }
+      if (more) {
+        // ---- the next chunk's copy of the state, and the state's decay over it
+        const float el = whole[set ^ 1];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          tmem_ld32(s_at + 32 * half, r);
+          tc_wait_ld();
+          put_state(half, el);
+        }
+        tc_wait_st();
+        if (tid == 0) tma_store_wait_read();   // the output tile's place is Kd's, or the next tile's
+        tc_fence_before();
+        __syncthreads();
+      }
     }
-    __syncthreads();
-    if (*abort_flag) break;
-    if (OUT && tid == 0) {
-      tma_store_4d(&tm_o, ot, 0, h, c0, row);
-      tma_store_4d(&tm_o, ot + 8192, 64, h, c0, row);
-      tma_store_commit();
-    }
-    set ^= 1;
-    phase ^= 1;
-    if (more) turn_state(whole[set]);
   }
   const bool ok = *abort_flag == 0;
   if (OUT && tid == 0) tma_store_wait_all();
-  if (!ok && warp == 1) {
-    // a CTA that gave up waits (bounded) for the copies it issued before its shared memory goes away: without the
-    // other arrival K's phase may never end, so it arrives first
-    if (lane == 0 && k_issued) mbar_arrive(k_bar);
+  if (!ok && warp == 0) {
+    // a CTA that gave up waits (bounded) for the copies it issued before its shared memory goes away
     const uint64_t t0 = global_ns();
     while (((k_issued && !mbar_try_wait(k_bar, (k_issued - 1) & 1)) ||
             (q_issued && !mbar_try_wait(q_bar, (q_issued - 1) & 1)) ||
@@ -504,18 +582,18 @@ __global__ void __launch_bounds__(THREADS, 2)
   float* out = MODE == WHOLE ? lin::state_out(a.pool, row, h)
                : MODE == STATES ? seg.states + ((int64_t)pair * seg.count + part) * STATE : nullptr;
   if (ok && out) {
+#pragma unroll
     for (int half = 0; half < 2; ++half) {
-      uint32_t r[32];
-      tmem_ld32(tmem + lane_bits + TM_S + 64 * ch + 32 * half, r);
+      tmem_ld32(s_at + 32 * half, r);
       tc_wait_ld();
 #pragma unroll
       for (int i = 0; i < 32; ++i) out[(ch * 64 + half * 32 + i) * D + L] = __uint_as_float(r[i]);
     }
-    if (MODE == STATES && tid == 0) seg.decay[(int64_t)pair * seg.count + part] = expf((float)decays);
+    if (MODE == STATES && tid == 0) seg.decay[(int64_t)pair * seg.count + part] = exp2_fast((float)carry);
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, TM_COLS);
   }

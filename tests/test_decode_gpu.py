@@ -12,8 +12,8 @@ import math
 import pytest
 import torch
 
+from jeff_b200 import _lib, kernels
 from jeff_b200 import constants as C
-from jeff_b200 import kernels
 from jeff_b200.prefix_pool import FAST_PATH_SHAPES, PrefixPool
 
 pytestmark = pytest.mark.gpu
@@ -21,6 +21,12 @@ pytestmark = pytest.mark.gpu
 HALF = 2.0 ** -8    # half a bf16 step, relative
 ULP = 2.0 ** -24    # half an fp32 step, relative
 FIXED = FAST_PATH_SHAPES.fixed_pages
+
+
+@pytest.fixture(autouse=True)
+def no_wait_gave_up():
+    yield
+    assert _lib.device_status() == 0
 
 
 def gen(seed: int) -> torch.Generator:
