@@ -42,16 +42,17 @@ using lin::D;
 
 constexpr int C = 64, THREADS = 256;
 constexpr uint32_t TILE = C * D * 2;   // 16 KB: two 64-column atoms of 64 rows x 128 B
-constexpr int OFF_KQ = 0;              // atom a: K at a * 16384, Q at + 8192 (no Q: the second V)
-constexpr int OFF_K0 = 32768, OFF_K1 = OFF_K0 + TILE;   // the parts of Kd (atoms 8192 apart); over the first then the
-constexpr int OFF_K2 = OFF_K1 + TILE;  // output tile. The third part, or with two the output tile
+constexpr int OFF_KQ = 0;              // atom a: K at a * 16384, Q (without outputs the second K) at + 8192
+constexpr int OFF_K0 = 32768;          // Kd's first part (atoms 8192 apart), then the output tile; the second V
+constexpr int OFF_K1 = OFF_K0 + TILE;
+constexpr int OFF_K2 = OFF_K1 + TILE;  // its third part, or with two parts the output tile
 constexpr int OFF_V = OFF_K2 + TILE;
 constexpr int OFF_P = OFF_V + TILE;    // 64 rows x 128 B
 constexpr int OFF_G = OFF_P + TILE / 2;   // two sets of gates
 constexpr int OFF_MISC = OFF_G + 2 * 7 * C * 4;
 constexpr int ALLOC = OFF_MISC + 80;
 static_assert(2 * (ALLOC + 1024) <= 228 * 1024, "two CTAs per SM");
-constexpr uint32_t TM_S = 0, TM_B = 128, TM_D = 192, TM_COLS = 256;
+constexpr uint32_t TM_S = 0, TM_B = 128, TM_D = 192, TM_SMALL = 128, TM_COLS = 256;
 constexpr int FIT = 2 * 148;           // CTAs that run at once
 constexpr int STATE = D * D;
 
@@ -223,18 +224,10 @@ __global__ void __launch_bounds__(THREADS, 2)
   const int qd = warp & 3, ch = warp >> 2;
   const int L = 32 * qd + lane;   // this thread's tensor-memory lane
   const uint32_t lane_bits = (uint32_t)(32 * qd) << 16;
-  const int pair = blockIdx.x / seg.count, part = blockIdx.x % seg.count;
-  const int row = pair / a.heads, h = pair % a.heads;
-  const int stop = a.real ? min(max(a.real[row], 0), a.n) : a.n;
-  const int begin = part * seg.chunks * C, end = min(begin + seg.chunks * C, a.n);
-  const int work = min(end, stop);   // tokens past it are padding: zeros out, the state stays
-  const int chunks = begin < work ? (work - begin + C - 1) / C : 0;
   if (smem_u32(sm) & 1023) {         // the swizzled tiles' base
     if (tid == 0) atomicCAS(err, 0, JB_DEV_LAUNCH | 50);
     return;
   }
-  auto start_of = [&](int i) { return begin + (OUT ? i : chunks - 1 - i) * C; };   // the first token of chunk i
-
   if (tid == 0) {
     for (int i = 0; i < 7; ++i) mbar_init(d_bar + i, 1);
     *abort_flag = 0;
@@ -244,16 +237,40 @@ __global__ void __launch_bounds__(THREADS, 2)
     tmem_alloc(tmem_slot, TM_COLS);
     tmem_relinquish();
   }
-  // tile loads, all issued by one lane of warp 0; without Q the V tiles alternate between two places
-  auto v_place = [&](int odd) { return !OUT && odd ? OFF_KQ + 8192 : OFF_V; };
-  auto v_step = [&](int odd) { return !OUT && odd ? 16384 : 8192; };   // between its atoms
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t s_at = tmem + lane_bits + TM_S + 64 * ch, b_at = tmem + lane_bits + TM_B + 32 * ch;
+  const uint32_t kq_a = smem_u32(kq), pt_a = smem_u32(pt);
+  if (OUT)   // P's upper right block is never anything else
+    for (int i = tid; i < 32 * 4; i += THREADS)
+      *reinterpret_cast<uint4*>(swz(pt, i >> 2, 4 + (i & 3))) = make_uint4(0, 0, 0, 0);
+
   int k_issued = 0, q_issued = 0, v_issued = 0;
+  const int pair = blockIdx.x / seg.count, part = blockIdx.x % seg.count;
+  const int row = pair / a.heads, h = pair % a.heads;
+  const int stop = a.real ? min(max(a.real[row], 0), a.n) : a.n;
+  const int begin = part * seg.chunks * C, end = min(begin + seg.chunks * C, a.n);
+  const int work = min(end, stop);   // tokens past it are padding: zeros out, the state stays
+  const int chunks = begin < work ? (work - begin + C - 1) / C : 0;
+  auto start_of = [&](int i) { return begin + (OUT ? i : chunks - 1 - i) * C; };   // the first token of chunk i
+  // tile loads, all issued by one lane of warp 0; without Q the K and V tiles alternate between two places, K's with
+  // Q's, the first part of Kd over it
+  auto k_place = [&](int odd) { return !OUT && odd ? OFF_KQ + 8192 : OFF_KQ; };
+  auto v_place = [&](int odd) { return !OUT && odd ? OFF_K0 : OFF_V; };
+  // chunk i's barriers of those tiles and the parity of its phase: with two places a barrier for each, since the next
+  // tile may have landed before a warp looks for this one
+  auto k_ready = [&](int i) { return !OUT && (i & 1) ? q_bar : k_bar; };
+  auto v_ready = [&](int i) { return !OUT && (i & 1) ? d_bar : v_bar; };
+  auto parity = [&](int i) { return (uint32_t)(OUT ? i : i >> 1) & 1; };
   auto load_k = [&](int i, bool me) {
     ++k_issued;
     if (!me) return;
-    mbar_arrive_expect_tx(k_bar, TILE);
-    tma_load_4d(kq, &tm_k, k_bar, 0, h, start_of(i), row);
-    tma_load_4d(kq + 16384, &tm_k, k_bar, 64, h, start_of(i), row);
+    uint8_t* to = sm + k_place(i & 1);
+    mbar_arrive_expect_tx(k_ready(i), TILE);
+    tma_load_4d(to, &tm_k, k_ready(i), 0, h, start_of(i), row);
+    tma_load_4d(to + 16384, &tm_k, k_ready(i), 64, h, start_of(i), row);
   };
   auto load_q = [&](int i, bool me) {
     ++q_issued;
@@ -266,9 +283,9 @@ __global__ void __launch_bounds__(THREADS, 2)
     ++v_issued;
     if (!me) return;
     uint8_t* to = sm + v_place(i & 1);
-    mbar_arrive_expect_tx(v_bar, TILE);
-    tma_load_4d(to, &tm_v, v_bar, 0, h, start_of(i), row);
-    tma_load_4d(to + v_step(i & 1), &tm_v, v_bar, 64, h, start_of(i), row);
+    mbar_arrive_expect_tx(v_ready(i), TILE);
+    tma_load_4d(to, &tm_v, v_ready(i), 0, h, start_of(i), row);
+    tma_load_4d(to + 8192, &tm_v, v_ready(i), 64, h, start_of(i), row);
   };
   const float* gp = a.g + row * a.g_row + h;
   float g0 = 0.f, g1 = 0.f;   // warps 0 and 4: the log-decays of the next chunk's tokens, 0 past the row's end
@@ -279,7 +296,6 @@ __global__ void __launch_bounds__(THREADS, 2)
   };
   double carry = 0.0;         // the same warps: log-decays so far
   if (qd == 0) gates_of(0);
-  __syncthreads();
   if (warp == 0 && chunks) {
     const bool me = elect_one();
     load_k(0, me);
@@ -290,50 +306,50 @@ __global__ void __launch_bounds__(THREADS, 2)
   // the state ahead of the segment, its loads in flight while the first gates are formed
   const float* in = MODE == WHOLE ? lin::state_in(a.pool, row, h)
                     : MODE == OUTPUTS ? seg.states + ((int64_t)pair * seg.count + part) * STATE : nullptr;
-  uint32_t r[32];
+  uint32_t r[32], r2[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) r[i] = in ? __float_as_uint(in[(ch * 64 + i) * D + L]) : 0u;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r2[i] = in ? __float_as_uint(in[(ch * 64 + 32 + i) * D + L]) : 0u;
   if (qd == 0) {
     form_gates<!OUT>(gates[0], ch, g0, g1, lane, whole, carry);
     gates_of(1);
   }
-  if (OUT)   // P's upper right block is never anything else
-    for (int i = tid; i < 32 * 4; i += THREADS)
-      *reinterpret_cast<uint4*>(swz(pt, i >> 2, 4 + (i & 3))) = make_uint4(0, 0, 0, 0);
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
   // lane = value column, columns = key rows: into tensor memory, scaled for the first chunk, and its bf16 copy
-  const uint32_t s_at = tmem + lane_bits + TM_S + 64 * ch, b_at = tmem + lane_bits + TM_B + 32 * ch;
-  auto put_state = [&](int half, float el) {
+  auto put_state = [&](int half, uint32_t (&x)[32], float el) {
     if (OUT) {
       uint32_t b[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) b[e] = pack_bf2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+      for (int e = 0; e < 16; ++e) b[e] = pack_bf2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
       tmem_st16(b_at + 16 * half, b);
 #pragma unroll
-      for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * el);
+      for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * el);
     }
-    tmem_st32(s_at + 32 * half, r);
+    tmem_st32(s_at + 32 * half, x);
+    if (!OUT) tmem_st32(s_at + TM_SMALL + 32 * half, x);
   };
   {
     const float el = OUT && chunks ? whole[0] : 1.f;
-    put_state(0, el);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) r[i] = in ? __float_as_uint(in[(ch * 64 + 32 + i) * D + L]) : 0u;
-    put_state(1, el);
+    put_state(0, r, el);
+    put_state(1, r2, el);
     tc_wait_st();
   }
   tc_fence_before();
   __syncthreads();
 
-  const uint32_t kq_a = smem_u32(kq), kd_a = smem_u32(sm + OFF_K0), pt_a = smem_u32(pt);
-  uint32_t phase = 0;
-  for (int c = 0; c < chunks; ++c, phase ^= 1) {
+  for (int c = 0; c < chunks; ++c) {
+    const uint32_t phase = (uint32_t)c & 1;
     const int set = c & 1, live = min(C, work - start_of(c));
     const bool more = c + 1 < chunks;
     const Gates& gt = gates[set];
+    // ---- without outputs the next tiles now: the last chunk's products have read the other places
+    if (!OUT && warp == 0 && more) {
+      const bool me = elect_one();
+      load_k(c + 1, me);
+      load_v(c + 1, me);
+      __syncwarp();
+    }
     // ---- MMA1, then, where it has read the state's copy, MMA2
     if (OUT && warp == 1) {
       mbar_wait(q_bar, phase, abort_flag, err, 53);
@@ -348,7 +364,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       }
       if (issuer) tc_commit(d_bar);
       __syncwarp();
-      mbar_wait(k_bar, phase, abort_flag, err, 52);
+      mbar_wait(k_ready(c), parity(c), abort_flag, err, 52);
       mbar_wait(d_bar, phase, abort_flag, err, 55);
       __syncwarp();
       tc_fence_after();
@@ -367,21 +383,22 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
     // values past the row's end may be anything: zeros, so that a zero weight keeps them out
     if (live < C) {
-      mbar_wait(v_bar, phase, abort_flag, err, 54);
+      mbar_wait(v_ready(c), parity(c), abort_flag, err, 54);
       for (int i = tid; i < (C - live) * 16; i += THREADS) {
         const int t = live + (i >> 4), x = i & 15;
-        *reinterpret_cast<uint4*>(swz(sm + v_place(set) + (x >> 3) * v_step(set), t, x & 7)) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(swz(sm + v_place(set) + (x >> 3) * 8192, t, x & 7)) = make_uint4(0, 0, 0, 0);
       }
     }
     // ---- Kd, 16-byte pieces of the tokens' keys: five a thread of the warps that form P, six of warps 1 and 5
+    auto kd_place = [&](int u) { return sm + (!OUT && u == 0 ? k_place(set) : OFF_K0 + u * (int)TILE); };
     auto form_kd = [&](auto count, int first, int step) {   // its loads ahead of its stores
       constexpr int N = decltype(count)::value;
-      mbar_wait(k_bar, phase, abort_flag, err, 52);
+      mbar_wait(k_ready(c), parity(c), abort_flag, err, 52);
       uint4 x[N];
 #pragma unroll
       for (int it = 0; it < N; ++it) {
         const int i = min(first + it * step, C * 16 - 1), t = i >> 4, p = i & 15;
-        x[it] = *reinterpret_cast<const uint4*>(swz(kq + (p >> 3) * 16384, t, p & 7));
+        x[it] = *reinterpret_cast<const uint4*>(swz(sm + k_place(set) + (p >> 3) * 16384, t, p & 7));
       }
 #pragma unroll
       for (int it = 0; it < N; ++it) {
@@ -392,7 +409,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         if (i < C * 16)
 #pragma unroll
           for (int u = 0; u < PARTS; ++u)
-            *reinterpret_cast<uint4*>(swz(sm + OFF_K0 + u * TILE + (p >> 3) * 8192, t, p & 7)) =
+            *reinterpret_cast<uint4*>(swz(kd_place(u) + (p >> 3) * (!OUT && u == 0 ? 16384 : 8192), t, p & 7)) =
                 t < live ? y[u] : make_uint4(0, 0, 0, 0);
       }
     };
@@ -449,31 +466,25 @@ __global__ void __launch_bounds__(THREADS, 2)
     tc_fence_before();
     __syncthreads();
     if (*abort_flag) break;
-    // ---- the next tiles, each once its place has been read: K by every thread and by MMA2, Q by MMA1 and MMA2, the
-    // other V by the last chunk's products
-    if (warp == 0 && more) {
+    // ---- the next tiles, each once its place has been read: K by every thread and by MMA2, Q by MMA1 and MMA2
+    if (OUT && warp == 0 && more) {
       const bool me = elect_one();
       load_k(c + 1, me);
-      if (OUT) load_q(c + 1, me);
-      if (!OUT) {
-        mbar_wait(v_bar, phase, abort_flag, err, 54);   // one load at a time on a barrier
-        load_v(c + 1, me);
-      }
+      load_q(c + 1, me);
       __syncwarp();
     }
     // ---- MMA3, MMA4
     if (warp == 1) {
-      mbar_wait(v_bar, phase, abort_flag, err, 54);
+      mbar_wait(v_ready(c), parity(c), abort_flag, err, 54);
       __syncwarp();
       tc_fence_after();
       const bool issuer = elect_one();
       const uint32_t v_a = smem_u32(sm + v_place(set));
-      const uint32_t step = v_step(set);
       if (OUT) {
         constexpr uint32_t id3 = idesc_bf16(128, 64) | A_MN;
 #pragma unroll
         for (int kk = 0; kk < C / 16; ++kk) {
-          const uint64_t av = mn_desc(v_a + kk * 2048, step), b = sw128_desc(pt_a + 32 * kk);
+          const uint64_t av = mn_desc(v_a + kk * 2048, 8192), b = sw128_desc(pt_a + 32 * kk);
           if (issuer) tc_mma_bf16(tmem + TM_B, av, b, id3, kk != 0);
         }
         if (EARLY && issuer) tc_commit(e_bar);
@@ -482,11 +493,11 @@ __global__ void __launch_bounds__(THREADS, 2)
       constexpr uint32_t id4 = idesc_bf16(128, 128) | A_MN | B_MN;
 #pragma unroll
       for (int kk = 0; kk < C / 16; ++kk) {
-        const uint64_t av = mn_desc(v_a + kk * 2048, step);
+        const uint64_t av = mn_desc(v_a + kk * 2048, 8192);
 #pragma unroll
         for (int p = PARTS - 1; p >= 0; --p) {   // the small parts first
-          const uint64_t b = mn_desc(kd_a + p * TILE + kk * 2048, 8192);
-          if (issuer) tc_mma_bf16(tmem + TM_S, av, b, id4, 1);
+          const uint64_t b = mn_desc(smem_u32(kd_place(p)) + kk * 2048, !OUT && p == 0 ? 16384 : 8192);
+          if (issuer) tc_mma_bf16(tmem + (!OUT && p > 0 ? TM_SMALL : TM_S), av, b, id4, 1);
         }
       }
       if (issuer) tc_commit(all_bar);
@@ -553,7 +564,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         for (int half = 0; half < 2; ++half) {
           tmem_ld32(s_at + 32 * half, r);
           tc_wait_ld();
-          put_state(half, el);
+          put_state(half, r, el);
         }
         tc_wait_st();
         if (tid == 0) tma_store_wait_read();   // the output tile's place is Kd's, or the next tile's
@@ -563,16 +574,6 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
   }
   const bool ok = *abort_flag == 0;
-  if (OUT && tid == 0) tma_store_wait_all();
-  if (!ok && warp == 0) {
-    // a CTA that gave up waits (bounded) for the copies it issued before its shared memory goes away
-    const uint64_t t0 = global_ns();
-    while (((k_issued && !mbar_try_wait(k_bar, (k_issued - 1) & 1)) ||
-            (q_issued && !mbar_try_wait(q_bar, (q_issued - 1) & 1)) ||
-            (v_issued && !mbar_try_wait(v_bar, (v_issued - 1) & 1))) &&
-           global_ns() - t0 < kWaitNs) {
-    }
-  }
   if (OUT) {   // chunks that hold padding only
     const int first = max(begin, (work + C - 1) / C * C);
     for (int i = first * 16 + tid; i < end * 16; i += THREADS)
@@ -585,11 +586,28 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       tmem_ld32(s_at + 32 * half, r);
+      if (!OUT) tmem_ld32(s_at + TM_SMALL + 32 * half, r2);
       tc_wait_ld();
 #pragma unroll
-      for (int i = 0; i < 32; ++i) out[(ch * 64 + half * 32 + i) * D + L] = __uint_as_float(r[i]);
+      for (int i = 0; i < 32; ++i)
+        out[(ch * 64 + half * 32 + i) * D + L] =
+            OUT ? __uint_as_float(r[i]) : __uint_as_float(r[i]) + __uint_as_float(r2[i]);
     }
     if (MODE == STATES && tid == 0) seg.decay[(int64_t)pair * seg.count + part] = exp2_fast((float)carry);
+  }
+  if (OUT && tid == 0) tma_store_wait_all();
+  if (!ok && warp == 0) {
+    // a CTA that gave up waits (bounded) for the copies it issued before its shared memory goes away: those of the last
+    // tile or two, the others having landed before these were issued
+    const uint64_t t0 = global_ns();
+    auto landed = [&]() {
+      bool all = !q_issued || mbar_try_wait(q_bar, (q_issued - 1) & 1);
+      for (int i = max(0, k_issued - (OUT ? 1 : 2)); i < k_issued; ++i) all = all && mbar_try_wait(k_ready(i), parity(i));
+      for (int i = max(0, v_issued - (OUT ? 1 : 2)); i < v_issued; ++i) all = all && mbar_try_wait(v_ready(i), parity(i));
+      return all;
+    };
+    while (!landed() && global_ns() - t0 < kWaitNs) {
+    }
   }
   tc_fence_before();
   __syncthreads();
