@@ -167,6 +167,7 @@ __global__ void __launch_bounds__(TAB_THREADS) tables_kernel(const TabParams p) 
 // and cosine, so positions of any size keep full accuracy.
 
 constexpr int NQ = 8, NKV = 2, HD = 256, ROT = 64;
+constexpr int PREP_MANY = 1;
 
 struct PrepParams {
   const __nv_bfloat16* pr;
@@ -238,6 +239,100 @@ __global__ void __launch_bounds__(384) prep_axes_kernel(const PrepParams p) {
   }
 }
 
+// The same with a warp per token, all twelve heads of a lane's dimensions loaded at once (6 KB in flight a warp), the
+// weights in registers over a warp's tokens, and no barrier. The eight query heads' sums are reduced together: each
+// step of the first three halves the number of values a lane carries (9 exchanges and 8 to hand them back, not 40).
+__device__ __forceinline__ void load8(const float* w, float (&x)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(w)[0], b = reinterpret_cast<const float4*>(w)[1];
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+
+__global__ void __launch_bounds__(256, 2) prep_tokens_kernel(const PrepParams p) {
+  pdl_begin();
+  constexpr int N = NQ + 2 * NKV;
+  const int lane = threadIdx.x & 31;
+  float wq[8], wk[8], wqo[8], wko[8];   // this lane's weights, and of the dimensions its first eight are turned with
+  load8(p.q_w1 + lane * 8, wq);
+  load8(p.k_w1 + lane * 8, wk);
+  load8(p.q_w1 + (lane ^ 4) * 8, wqo);
+  load8(p.k_w1 + (lane ^ 4) * 8, wko);
+  for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < p.t; t += gridDim.x * 8) {
+    const __nv_bfloat16* src = p.pr + (int64_t)t * p.ldpr;
+    uint4 x[N];
+#pragma unroll
+    for (int h = 0; h < N; ++h)
+      x[h] = reinterpret_cast<const uint4*>(src + (h < NQ ? h * 2 * HD : NQ * 2 * HD + (h - NQ) * HD))[lane];
+    float mc, ms, c[8], s[8];
+    turn_of(p, t, lane, mc, ms);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      c[e] = __shfl_sync(0xffffffffu, mc, (lane & 3) * 8 + e);
+      s[e] = __shfl_sync(0xffffffffu, ms, (lane & 3) * 8 + e);
+      if (!(lane & 4)) s[e] = -s[e];   // dimensions 0-31 subtract
+    }
+    float ss[NQ + NKV];
+#pragma unroll
+    for (int h = 0; h < NQ + NKV; ++h) {
+      float f[8];
+      ew::unpack8(x[h], f);
+      ss[h] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss[h] += f[e] * f[e];
+    }
+    float v[4];   // lanes with bit 16, 8, 4 set keep the odd heads of what is left at each step
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float keep = lane & 16 ? ss[2 * i + 1] : ss[2 * i], give = lane & 16 ? ss[2 * i] : ss[2 * i + 1];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float keep = lane & 8 ? v[2 * i + 1] : v[2 * i], give = lane & 8 ? v[2 * i] : v[2 * i + 1];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
+    }
+    {
+      const float keep = lane & 4 ? v[1] : v[0], give = lane & 4 ? v[0] : v[1];
+      v[0] = keep + __shfl_xor_sync(0xffffffffu, give, 4);
+    }
+    v[0] += __shfl_xor_sync(0xffffffffu, v[0], 2);
+    v[0] += __shfl_xor_sync(0xffffffffu, v[0], 1);
+    const float mine = rsqrtf(v[0] / HD + ew::EPS);   // of head 4 (lane bit 4) + 2 (bit 8) + (bit 16)
+#pragma unroll
+    for (int h = 0; h < NQ; ++h)
+      ss[h] = __shfl_sync(0xffffffffu, mine, (h & 1) * 16 + (h >> 1 & 1) * 8 + (h >> 2) * 4);
+#pragma unroll
+    for (int h = NQ; h < NQ + NKV; ++h) ss[h] = rsqrtf(ew::warp_sum(ss[h]) / HD + ew::EPS);
+#pragma unroll
+    for (int h = 0; h < NQ + NKV; ++h) {
+      const uint4 o = make_uint4(__shfl_xor_sync(0xffffffffu, x[h].x, 4), __shfl_xor_sync(0xffffffffu, x[h].y, 4),
+                                 __shfl_xor_sync(0xffffffffu, x[h].z, 4), __shfl_xor_sync(0xffffffffu, x[h].w, 4));
+      float f[8], g[8];
+      ew::unpack8(x[h], f);
+      ew::unpack8(o, g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f[e] *= ss[h] * (h < NQ ? wq[e] : wk[e]);
+        g[e] *= ss[h] * (h < NQ ? wqo[e] : wko[e]);
+        if (lane < ROT / 8) f[e] = f[e] * c[e] + g[e] * s[e];
+      }
+      x[h] = ew::pack8(f);
+    }
+#pragma unroll
+    for (int h = 0; h < NQ; ++h) reinterpret_cast<uint4*>(p.q + ((int64_t)t * NQ + h) * HD)[lane] = x[h];
+    const int64_t slot = p.kv ? p.slots[t] : -1, page = slot / PAGE;
+#pragma unroll
+    for (int i = 0; i < 2 * NKV; ++i) {
+      const int head = i % NKV, half = i / NKV;   // half 0: keys, 1: values
+      __nv_bfloat16* flat = half ? p.vn : p.kn;
+      if (flat) reinterpret_cast<uint4*>(flat + ((int64_t)t * NKV + head) * HD)[lane] = x[NQ + i];
+      if (slot >= 0 && page < p.pages)
+        reinterpret_cast<uint4*>(p.kv + page * p.page_bytes +
+                                 (((int64_t)half * PAGE + slot % PAGE) * NKV + head) * HD * 2)[lane] = x[NQ + i];
+    }
+  }
+}
+
 // ------------------------------------------------------------------ attention of one new token per row
 //
 // o = sum_j softmax_j(scale q . k_j) v_j over the row's cached tokens j < lengths[r], in one pass over the pages with
@@ -291,24 +386,31 @@ struct DecParams {
 
 __device__ __forceinline__ int dec_length(const DecParams& p, int r) { return min(max(p.lengths[r], 0), p.most); }
 
-// Units (steps of one key/value head) of the rows before `row`, and with row = b of all; warp-collective.
+// Units (steps of one key/value head) of the rows before `row`, and of all; warp-collective.
 template <int STEP>
-__device__ long long dec_units_before(const DecParams& p, int row) {
+__device__ void dec_units(const DecParams& p, int row, long long& before, long long& total) {
   const int lane = threadIdx.x & 31;
-  long long sum = 0;
-  for (int r0 = 0; r0 < row; r0 += 128) {
+  long long some = 0, all = 0;
+  for (int r0 = 0; r0 < p.b; r0 += 128) {
     int n[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = r0 + 32 * i + lane;
-      n[i] = r < row ? dec_length(p, r) : 0;
+      n[i] = r < p.b ? (dec_length(p, r) + STEP - 1) / STEP : 0;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum += (n[i] + STEP - 1) / STEP;
+    for (int i = 0; i < 4; ++i) {
+      all += n[i];
+      if (r0 + 32 * i + lane < row) some += n[i];
+    }
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum * p.kv_heads;
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    some += __shfl_xor_sync(0xffffffffu, some, o);
+  }
+  before = some * p.kv_heads;
+  total = all * p.kv_heads;
 }
 
 struct Cursor {   // a unit: a step of a row's head
@@ -371,7 +473,8 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
   extern __shared__ __align__(16) uint8_t sm[];
   __shared__ float s_m[L::WARPS][16], s_l[L::WARPS][16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, tq = lane & 3;
-  const long long total = dec_units_before<L::STEP>(p, p.b);
+  long long none, total;
+  dec_units<L::STEP>(p, 0, none, total);
   const long long shares = min((long long)SHARES, total);   // none of them empty
   if (blockIdx.x >= shares) return;
   const long long u0 = total * blockIdx.x / shares, u1 = total * (blockIdx.x + 1) / shares;
@@ -607,42 +710,63 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
   }
 }
 
-// CTA per (row, query head), thread = dimension: the parts of a row that shares cut, in share order; rows without
-// tokens are zeros; nothing to do for a row that one share held in full.
+// CTA per (row, query head): the parts of a row that shares cut, joined in share order; rows without tokens are zeros;
+// nothing to do for a row that one share held in full. The parts' factors first, a thread each, then their sums.
 template <int D>
-__global__ void __launch_bounds__(D) join_kernel(const DecParams p) {
+__global__ void __launch_bounds__(256) join_kernel(const DecParams p) {
   pdl_begin();
   constexpr int STEP = Dec<D>::STEP;
+  __shared__ float s_w[SHARES], s_red[32], s_v[256];
   const int heads = p.kv_heads * p.group;
   const int row = blockIdx.x / heads, head = blockIdx.x % heads, g = head / p.group, h = head % p.group;
-  const int d = threadIdx.x;
   const int steps = (dec_length(p, row) + STEP - 1) / STEP;
-  __nv_bfloat16* y = p.y + row * p.ldy + (int64_t)head * D + d;
+  __nv_bfloat16* y = p.y + row * p.ldy + (int64_t)head * D;
   if (steps == 0) {
-    *y = f2bf(0.f);
+    if (threadIdx.x < D) y[threadIdx.x] = f2bf(0.f);
     return;
   }
-  const long long total = dec_units_before<STEP>(p, p.b);
-  const long long a = dec_units_before<STEP>(p, row) + (long long)g * steps, z = a + steps - 1;
+  long long before, total;
+  dec_units<STEP>(p, row, before, total);
   const long long shares = min((long long)SHARES, total);
+  const long long a = before + (long long)g * steps, z = a + steps - 1;
   const long long c0 = ((a + 1) * shares - 1) / total, c1 = ((z + 1) * shares - 1) / total;   // unit u's: the last c
   if (c0 == c1) return;                                                      // with total * c / shares <= u
-  const int stride = p.group * (D + 2);
-  const float* first = p.scratch + (2 * c0 + (total * c0 / shares == a ? 0 : 1)) * stride + h * (D + 2);
-  float mx = first[0];
-  for (long long c = c0 + 1; c <= c1; ++c) mx = fmaxf(mx, p.scratch[2 * c * stride + h * (D + 2)]);
-  float sum = 0.f, v = 0.f;
-#pragma unroll 4
-  for (long long c = c0; c <= c1; ++c) {
-    const float* part = c == c0 ? first : p.scratch + 2 * c * stride + h * (D + 2);
-    const bool none = part[0] == -INFINITY && part[1] == 0.f;
-    const float w = none ? 0.f : exp2f(part[0] - finite(mx));
-    sum += w * part[1];
-    v += w * part[2 + d];
+  const int stride = p.group * (D + 2), count = (int)(c1 - c0) + 1;
+  // share c0 + i's part: its slot 0 holds what began with the share
+  const float* parts = p.scratch + 2 * c0 * stride + h * (D + 2);
+  const int first = total * c0 / shares == a ? 0 : stride;
+  auto part = [&](int i) { return parts + (int64_t)2 * i * stride + (i == 0 ? first : 0); };
+  float m = -INFINITY, l = 0.f;
+  if ((int)threadIdx.x < count) {
+    m = part(threadIdx.x)[0];
+    l = part(threadIdx.x)[1];
+  }
+  const float mx = ew::block_max(m, s_red);
+  const float w = (int)threadIdx.x < count && !(m == -INFINITY && l == 0.f) ? exp2f(m - finite(mx)) : 0.f;
+  if ((int)threadIdx.x < count) s_w[threadIdx.x] = w;
+  const float sum = ew::block_sum(w == 0.f ? 0.f : w * l, s_red);   // its barriers order s_w too
+  // thread = (one of 256 / D interleaved sets of parts, dimension), eight loads in flight
+  constexpr int SETS = 256 / D;
+  const int d = threadIdx.x % D, set = threadIdx.x / D;
+  float v = 0.f;
+  for (int i0 = set; i0 < count; i0 += 8 * SETS) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = i0 + j * SETS < count ? part(i0 + j * SETS)[2 + d] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + j * SETS < count && s_w[i0 + j * SETS] != 0.f) v += s_w[i0 + j * SETS] * x[j];
+  }
+  if (SETS > 1) {
+    s_v[threadIdx.x] = v;
+    __syncthreads();
+    if (set > 0) return;
+#pragma unroll
+    for (int i = 1; i < SETS; ++i) v += s_v[i * D + d];
   }
   v = mx == -INFINITY && sum == 0.f ? 0.f : v / sum;
   if (p.pr) v *= ew::sigmoid(bf2f(p.pr[row * p.ldpr + ((int64_t)2 * head + 1) * D + d]));
-  *y = f2bf(v);
+  y[d] = f2bf(v);
 }
 
 template <int D, int NT, bool PAIR>
@@ -659,7 +783,7 @@ int dec_launch(const DecParams& p, cudaStream_t stream) {
   }
   launch_pdl(decode_kernel<D, NT, PAIR>, SHARES, Dec<D>::WARPS * 32, Dec<D>::SMEM, stream, p);
   if (int r = check_launch("decode_kernel")) return r;
-  launch_pdl(join_kernel<D>, p.b * p.kv_heads * p.group, D, 0, stream, p);
+  launch_pdl(join_kernel<D>, p.b * p.kv_heads * p.group, 256, 0, stream, p);
   return check_launch("join_kernel");
 }
 
@@ -716,6 +840,10 @@ extern "C" int jb_attn_prep_axes(const uint16_t* pr, int64_t ldpr, int t, const 
                              reinterpret_cast<__nv_bfloat16*>(kn), reinterpret_cast<__nv_bfloat16*>(vn),
                              kv ? static_cast<uint8_t*>(kv) + attn_layer * layer_bytes : nullptr, pages, page_bytes,
                              slots};
+  if (t >= dec::PREP_MANY) {
+    launch_pdl(dec::prep_tokens_kernel, min((t + 7) / 8, 2 * dec::SHARES), 256, 0, (cudaStream_t)stream, p);
+    return check_launch("prep_tokens_kernel");
+  }
   launch_pdl(dec::prep_axes_kernel, t, 384, 0, (cudaStream_t)stream, p);
   return check_launch("prep_axes_kernel");
 }

@@ -364,14 +364,14 @@ def kv_scatter(kn: torch.Tensor, vn: torch.Tensor, n: int, real: torch.Tensor, p
 def _rows_of(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, ...], inner: int,
              device: torch.device) -> None:
     """`t` (shape) of `dtype` on `device`, its last `inner` dimensions packed and the others strided as they like."""
+    if t.dtype is dtype and t.shape == shape and t.device == device and t.is_cuda and t.is_contiguous():
+        return   # what nearly every call brings: these checks are most of a small call's host time
     if t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name}: expected {dtype} of shape {shape}, got {t.dtype} {tuple(t.shape)}")
     if not t.is_cuda:
         raise ValueError(f"{name}: expected a CUDA tensor, got one on {t.device}")
     if t.device != device:
         raise ValueError(f"{name}: expected a tensor on {device} as the others, got one on {t.device}")
-    if t.is_contiguous():
-        return
     step = 1
     for size, stride in zip(reversed(shape[len(shape) - inner:]), reversed(t.stride()[len(shape) - inner:])):
         if stride != step and size != 1:
@@ -380,10 +380,12 @@ def _rows_of(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, .
 
 
 def _tables_of(tables: torch.Tensor, name: str, rows: int, width: int, device: torch.device) -> None:
-    if tables.dim() != 2 or tables.shape[0] < rows or tables.shape[1] < width or tables.dtype != torch.int32 or \
-            tables.stride(1) != 1:
+    """Block tables of at least `rows` rows and `width` entries, packed or with their rows apart."""
+    shape = tables.shape
+    if len(shape) != 2 or shape[0] < rows or shape[1] < width or tables.dtype is not torch.int32 or \
+            not (tables.is_contiguous() or tables.stride(1) == 1):
         raise ValueError(f"{name}: expected int32 (rows >= {rows}, width >= {width}) with packed rows, got "
-                         f"{tuple(tables.shape)} {tables.dtype}, strides {tables.stride()}")
+                         f"{tuple(shape)} {tables.dtype}, strides {tables.stride()}")
     if tables.device != device:
         raise ValueError(f"{name}: expected a tensor on {device}, got one on {tables.device}")
 
@@ -392,7 +394,7 @@ def _cache_of(kv: torch.Tensor, attn_layer: int, device: torch.device) -> tuple[
     """(key/value heads, their width) of a cache of pages kv[page, layer, K|V, 32 tokens, head, dim]."""
     if kv.dim() != 6 or kv.dtype != DT or kv.shape[2:4] != (2, 32):
         raise ValueError(f"kv: expected bf16 pages (page, layer, 2, 32, heads, dim), got {kv.dtype} {tuple(kv.shape)}")
-    _rows_of(kv, "kv", DT, tuple(kv.shape), 5, device)
+    _rows_of(kv, "kv", DT, kv.shape, 5, device)
     if not 0 <= attn_layer < kv.shape[1]:
         raise ValueError(f"attn_layer {attn_layer}: the pages hold {kv.shape[1]} layers")
     return kv.shape[4], kv.shape[5]
@@ -437,16 +439,18 @@ def block_tables(lengths: torch.Tensor, new: torch.Tensor, free: torch.Tensor, t
     _rows_of(free, "free", torch.int32, tuple(free.shape), 1, dev)
     _tables_of(tables, "tables", b, kv_entry + 1, dev)
     if out is None:
-        buf = torch.empty(4 * tokens + 2 * (b + 1), dtype=torch.int32, device=dev)
-        out = SlotMap(buf[:2 * tokens].view(torch.int64), buf[2 * tokens:3 * tokens], buf[3 * tokens:4 * tokens],
-                      buf[4 * tokens:4 * tokens + b + 1], buf[4 * tokens + b + 1:])
+        parts = torch.empty(4 * tokens + 2 * (b + 1), dtype=torch.int32, device=dev).split(
+            (2 * tokens, tokens, tokens, b + 1, b + 1))
+        out = SlotMap(parts[0].view(torch.int64), *parts[1:])
     else:
         for name, dtype, size in (("slots", torch.int64, tokens), ("rows", torch.int32, tokens),
                                   ("positions", torch.int32, tokens), ("starts", torch.int32, b + 1),
                                   ("taken", torch.int32, b + 1)):
             _rows_of(getattr(out, name), name, dtype, (size,), 1, dev)
-    _on(dev, "jb_block_tables", ptr(lengths), ptr(new), b, ptr(free), free.shape[0], ptr(tables), tables.stride(0),
-        tables.shape[1], kv_entry, page_tokens, 1 if fixed else 0, tokens, *map(ptr, out))
+    slots, rows, positions, starts, taken = out
+    _on(dev, "jb_block_tables", lengths.data_ptr(), new.data_ptr(), b, free.data_ptr(), free.shape[0],
+        tables.data_ptr(), tables.stride(0), tables.shape[1], kv_entry, page_tokens, 1 if fixed else 0, tokens,
+        slots.data_ptr(), rows.data_ptr(), positions.data_ptr(), starts.data_ptr(), taken.data_ptr())
     return out
 
 
@@ -485,7 +489,7 @@ def attn_prep_axes(pr: torch.Tensor, q_w1: torch.Tensor, k_w1: torch.Tensor, inv
     dev, t = pr.device, pr.shape[0]
     if pr.dim() != 2 or pr.shape[1] < C.ATTN_PROJ:
         raise ValueError(f"pr: expected (tokens, at least {C.ATTN_PROJ}), got {tuple(pr.shape)}")
-    _rows_of(pr, "pr", DT, tuple(pr.shape), 1, dev)
+    _rows_of(pr, "pr", DT, pr.shape, 1, dev)
     _rows_of(q_w1, "q_w1", torch.float32, (C.HD,), 1, dev)
     _rows_of(k_w1, "k_w1", torch.float32, (C.HD,), 1, dev)
     _rows_of(inv_freq, "inv_freq", torch.float32, (C.ROT // 2,), 1, dev)
@@ -504,10 +508,11 @@ def attn_prep_axes(pr: torch.Tensor, q_w1: torch.Tensor, k_w1: torch.Tensor, inv
         out = torch.empty(t, C.NQ, C.HD, dtype=DT, device=dev)
     else:
         _rows_of(out, "out", DT, (t, C.NQ, C.HD), 3, dev)
-    _on(dev, "jb_attn_prep_axes", ptr(pr), pr.stride(0), t, ptr(q_w1), ptr(k_w1), ptr(inv_freq), ptr(positions),
-        positions.stride(0), axes - (1 << 64) if axes >> 63 else axes, ptr(out), ptr(kn), ptr(vn), ptr(kv),
-        0 if kv is None else kv.shape[0], 0 if kv is None else 2 * kv.stride(0), attn_layer,
-        0 if kv is None else kv.shape[1], ptr(slots))
+    pages = (None, 0, 0, attn_layer, 0) if kv is None else (kv.data_ptr(), kv.shape[0], 2 * kv.stride(0), attn_layer,
+                                                            kv.shape[1])
+    _on(dev, "jb_attn_prep_axes", pr.data_ptr(), pr.stride(0), t, q_w1.data_ptr(), k_w1.data_ptr(),
+        inv_freq.data_ptr(), positions.data_ptr(), positions.stride(0), axes - (1 << 64) if axes >> 63 else axes,
+        out.data_ptr(), ptr(kn), ptr(vn), *pages, ptr(slots))
     return out
 
 
@@ -545,10 +550,10 @@ def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, at
                               device=dev)
     else:
         _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), dev)
-    _on(dev, "jb_decode_attention", ptr(q), q.stride(0), ptr(kv), kv.shape[0], 2 * kv.stride(0), attn_layer,
-        kv.shape[1], ptr(tables), tables.stride(0), tables.shape[1], kv_entry, ptr(lengths), b, heads, kv_heads, dim,
-        dim ** -0.5 if scale is None else scale, ptr(pr), 0 if pr is None else pr.stride(0), ptr(out), out.stride(0),
-        ptr(scratch), scratch.numel())
+    _on(dev, "jb_decode_attention", q.data_ptr(), q.stride(0), kv.data_ptr(), kv.shape[0], 2 * kv.stride(0), attn_layer,
+        kv.shape[1], tables.data_ptr(), tables.stride(0), tables.shape[1], kv_entry, lengths.data_ptr(), b, heads,
+        kv_heads, dim, dim ** -0.5 if scale is None else scale, ptr(pr), 0 if pr is None else pr.stride(0),
+        out.data_ptr(), out.stride(0), scratch.data_ptr(), scratch.numel())
     return out
 
 
@@ -559,30 +564,36 @@ def _linear_of(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
                tables: torch.Tensor, layer: int, out_tables: torch.Tensor | None,
                out: torch.Tensor | None) -> tuple[torch.Tensor, tuple]:
     """What linear_scan and linear_step check alike; (o, the states' arguments)."""
-    dev = q.device
-    b, heads = q.shape[0], q.shape[-2]
-    shape = (*q.shape[:-1], C.DK)
-    for name, x in (("q", q), ("k", k), ("v", v)):
-        _rows_of(x, name, DT, shape, 2, dev)
+    dev, shape = q.device, q.shape
+    b, heads = shape[0], shape[-2]
+    if shape[-1] != C.DK:
+        raise ValueError(f"q: expected heads of {C.DK}, got {tuple(shape)}")
+    if not (q.shape == shape and k.shape == shape and v.shape == shape and q.dtype is DT and k.dtype is DT and
+            v.dtype is DT and q.is_cuda and k.device == dev and v.device == dev and q.is_contiguous() and
+            k.is_contiguous() and v.is_contiguous()):
+        for name, x in (("q", q), ("k", k), ("v", v)):
+            _rows_of(x, name, DT, shape, 2, dev)
     if g.dim() == 1:
         _rows_of(g, "g", torch.float32, (heads,), 1, dev)
     else:
         _rows_of(g, "g", torch.float32, shape[:-1], 1, dev)
-    if state.dim() != 4 or state.shape[2:] != (C.DK, C.DV):
-        raise ValueError(f"state: expected pages (page, heads per page, {C.DK}, {C.DV}), got {tuple(state.shape)}")
-    _rows_of(state, "state", torch.float32, tuple(state.shape), 3, dev)
+    held = state.shape
+    if len(held) != 4 or held[2:] != (C.DK, C.DV):
+        raise ValueError(f"state: expected pages (page, heads per page, {C.DK}, {C.DV}), got {tuple(held)}")
+    _rows_of(state, "state", torch.float32, held, 3, dev)
     if layer < 0:
         raise ValueError(f"layer {layer}: layers count from 0")
-    width = (layer * heads + heads - 1) // state.shape[1] + 1
+    width = (layer * heads + heads - 1) // held[1] + 1
     _tables_of(tables, "tables", b, width, dev)
-    if out_tables is not None:
+    if out_tables is not None and out_tables is not tables:
         _tables_of(out_tables, "out_tables", b, width, dev)
     if out is None:
-        out = torch.empty(shape, dtype=DT, device=dev)
+        out = torch.empty_like(v, memory_format=torch.contiguous_format)
     else:
         _rows_of(out, "out", DT, shape, len(shape), dev)
-    return out, (ptr(state), state.shape[0], 4 * state.stride(0), state.shape[1], layer * heads, ptr(tables),
-                 tables.stride(0), ptr(out_tables), 0 if out_tables is None else out_tables.stride(0))
+    return out, (state.data_ptr(), held[0], 4 * state.stride(0), held[1], layer * heads,
+                 tables.data_ptr(), tables.stride(0), ptr(out_tables),
+                 0 if out_tables is None else out_tables.stride(0))
 
 
 def linear_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor,
@@ -608,9 +619,9 @@ def linear_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     else:
         _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), q.device)
     steps = (0, 0) if g.dim() == 1 else g.stride()[:2]
-    _on(q.device, "jb_linear_scan", ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(v),
-        v.stride(0), v.stride(1), ptr(g), *steps, ptr(real), ptr(o), b, n, heads, *pool, ptr(scratch),
-        0 if scratch is None else scratch.numel())
+    _on(q.device, "jb_linear_scan", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+        v.data_ptr(), v.stride(0), v.stride(1), g.data_ptr(), *steps, ptr(real), o.data_ptr(), b, n, heads, *pool,
+        ptr(scratch), 0 if scratch is None else scratch.numel())
     return o
 
 
@@ -626,6 +637,6 @@ def linear_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     o, pool = _linear_of(q, k, v, g, state, tables, layer, tables if out_tables is None else out_tables, out)
     if beta is not None:
         _rows_of(beta, "beta", DT, (b, heads), 2, q.device)
-    _on(q.device, "jb_linear_step", ptr(q), q.stride(0), ptr(k), k.stride(0), ptr(v), v.stride(0), ptr(g),
-        0 if g.dim() == 1 else g.stride(0), ptr(beta), ptr(o), b, heads, *pool)
+    _on(q.device, "jb_linear_step", q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+        g.data_ptr(), 0 if g.dim() == 1 else g.stride(0), ptr(beta), o.data_ptr(), b, heads, *pool)
     return o
