@@ -44,8 +44,9 @@ __device__ __forceinline__ TabRow tab_row(const TabParams& p, int r) {
   t.len = max(p.lengths[r], 0);
   t.add = min(max(p.added[r], 0), 0x7fffffff - t.len);
   const int most = p.width - p.kv_entry;
-  const int need = (int)min(((long long)t.len + t.add + p.page - 1) / p.page, (long long)most);
-  t.held = (int)min(((long long)t.len + p.page - 1) / p.page, (long long)most);
+  const unsigned page = p.page;   // the sums stay below 2^32
+  const int need = (int)min(((unsigned)t.len + t.add + (page - 1)) / page, (unsigned)most);
+  t.held = (int)min(((unsigned)t.len + (page - 1)) / page, (unsigned)most);
   t.head = p.fixed && t.len == 0 && t.add > 0 ? p.kv_entry : 0;
   t.take = need - t.held + t.head;
   return t;
@@ -64,11 +65,12 @@ __global__ void __launch_bounds__(TAB_THREADS) tables_kernel(const TabParams p) 
     const int count = min(TAB_ROWS, p.b - r0);
     TabRow mine[TAB_PER];
     long long a = 0, k = 0;
+    const int rows_each = (count + TAB_THREADS - 1) / TAB_THREADS;
 #pragma unroll
     for (int i = 0; i < TAB_PER; ++i) {
-      const int j = tid * TAB_PER + i;
+      const int j = tid * rows_each + i;
       mine[i].add = mine[i].take = 0;
-      if (j < count) mine[i] = tab_row(p, r0 + j);
+      if (i < rows_each && j < count) mine[i] = tab_row(p, r0 + j);
       a += mine[i].add;
       k += mine[i].take;
     }
@@ -100,8 +102,10 @@ __global__ void __launch_bounds__(TAB_THREADS) tables_kernel(const TabParams p) 
     }
 #pragma unroll
     for (int i = 0; i < TAB_PER; ++i) {
-      s_add[tid * TAB_PER + i] = ea;
-      s_take[tid * TAB_PER + i] = ek;
+      if (i < rows_each) {
+        s_add[tid * rows_each + i] = ea;
+        s_take[tid * rows_each + i] = ek;
+      }
       ea += mine[i].add;
       ek += mine[i].take;
     }
@@ -248,7 +252,7 @@ __device__ __forceinline__ void load8(const float* w, float (&x)[8]) {
   x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
 }
 
-__global__ void __launch_bounds__(256, 2) prep_tokens_kernel(const PrepParams p) {
+__global__ void __launch_bounds__(128, 3) prep_tokens_kernel(const PrepParams p) {
   pdl_begin();
   constexpr int N = NQ + 2 * NKV;
   const int lane = threadIdx.x & 31;
@@ -257,7 +261,7 @@ __global__ void __launch_bounds__(256, 2) prep_tokens_kernel(const PrepParams p)
   load8(p.k_w1 + lane * 8, wk);
   load8(p.q_w1 + (lane ^ 4) * 8, wqo);
   load8(p.k_w1 + (lane ^ 4) * 8, wko);
-  for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < p.t; t += gridDim.x * 8) {
+  for (int t = blockIdx.x * 4 + (threadIdx.x >> 5); t < p.t; t += gridDim.x * 4) {
     const __nv_bfloat16* src = p.pr + (int64_t)t * p.ldpr;
     uint4 x[N];
 #pragma unroll
@@ -344,9 +348,9 @@ __global__ void __launch_bounds__(256, 2) prep_tokens_kernel(const PrepParams p)
 // CTA finishes what it holds in full; of a row cut by a share's border each part leaves its unnormalised sum, maximum
 // and weight in scratch, and join_kernel adds a row's parts in order.
 //
-// In a CTA each warp takes one 16-token tile of a step, with a ring of its own in shared memory (cp.async, rows past the
-// end filled with zeros) and no barrier with the other warps until a row ends, when the warps' sums are joined in
-// shared memory. Scores and output are taken transposed, S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16: the 16
+// In a CTA each warp takes one 16-token tile of a step, with a ring of its own in shared memory (cp.async of a tile's
+// keys, then its values, tokens past the row's end as zeros) and no barrier with the other warps until a row ends, when
+// the warps' sums are joined in shared memory. Scores and output are taken transposed, S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16: the 16
 // rows of the tile are keys (then 16 of the head's dimensions), the 8 columns the query heads, so 4 query heads cost
 // half of what a 16-row query tile would. (tcgen05 has no use here: its 128-row tile would be filled with 4 rows.)
 // The weights are held as two bf16 parts, p = hi + lo to 2^-17: with at most 4 query heads the lo parts ride in
@@ -354,14 +358,14 @@ __global__ void __launch_bounds__(256, 2) prep_tokens_kernel(const PrepParams p)
 
 template <int D>
 struct Dec {
-  static constexpr int WARPS = D == 256 ? 4 : 8;
-  static constexpr int STAGES = D == 64 ? 5 : 3;
+  static constexpr int WARPS = D == 64 ? 16 : 8;
+  static constexpr int HALVES = D == 256 ? 3 : D == 128 ? 6 : 5;   // a warp's ring, in tiles' keys or values
   static constexpr int STEP = WARPS * 16;         // tokens
   static constexpr int PITCH = D * 2 + 16;        // bytes of a key in shared memory: ldmatrix without conflicts
-  static constexpr int SLOT = 2 * 16 * PITCH;     // a tile's keys, then its values; a warp's output at a row's end
-  static constexpr int SMEM = WARPS * STAGES * SLOT;
+  static constexpr int SLOT = 16 * PITCH;         // a tile's keys or its values; eight heads' outputs at a row's end
+  static constexpr int SMEM = WARPS * HALVES * SLOT;
   static constexpr int OPITCH = D + 8;            // floats of a head's output there
-  static_assert(16 * OPITCH * 4 <= SLOT, "sixteen heads' outputs fit a slot");
+  static_assert(8 * OPITCH * 4 <= SLOT, "eight heads' outputs fit a slot");
   static_assert(SMEM + 4096 <= 227 * 1024, "shared memory");
 };
 
@@ -478,7 +482,7 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
   const long long shares = min((long long)SHARES, total);   // none of them empty
   if (blockIdx.x >= shares) return;
   const long long u0 = total * blockIdx.x / shares, u1 = total * (blockIdx.x + 1) / shares;
-  uint8_t* ring = sm + warp * L::STAGES * L::SLOT;
+  uint8_t* ring = sm + warp * L::HALVES * L::SLOT;
   Cursor c = dec_find<L::STEP>(p, u0), f = c;
   const int half_bytes = PAGE * p.kv_heads * D * 2;   // a page's keys of one layer, then its values
 
@@ -488,37 +492,46 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
     const int page = p.tables[(int64_t)x.row * p.table_stride + p.kv_entry + j / PAGE];
     return page >= 0 && page < p.pages ? page : -1;
   };
-  auto fetch = [&](const Cursor& x, int page, int slot) {
-    if (page >= 0) {
-      const int j0 = x.step * L::STEP + warp * 16;
-      const int live = min(16, dec_length(p, x.row) - j0);
-      const uint8_t* src = p.kv + (int64_t)page * p.page_bytes + ((j0 % PAGE) * p.kv_heads + x.head) * D * 2;
-      const uint32_t dst = smem_u32(ring + slot * L::SLOT);
+  // the fetches' cursor, half a tile at a time: the unit, its page (loaded one unit ahead, so that its load never stands
+  // in a fetch's way), keys or values, and the slot; `valid` has a bit for each tile fetched and not yet used
+  long long uf = u0;
+  int page = page_of(f), value = 0, fslot = 0, ahead = 0;
+  uint32_t valid = 0;
+  auto fetch = [&]() {
+    if (uf < u1) {
+      if (page >= 0) {
+        const int j0 = f.step * L::STEP + warp * 16;
+        const int live = min(16, dec_length(p, f.row) - j0);
+        const uint8_t* src = p.kv + (int64_t)page * p.page_bytes + (int64_t)value * half_bytes +
+                             ((j0 % PAGE) * p.kv_heads + f.head) * D * 2;
+        const uint32_t dst = smem_u32(ring + fslot * L::SLOT);
+        const int row_bytes = p.kv_heads * D * 2;
+        if (live == 16) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {   // 32 keys and values x CH chunks: consecutive lanes along a row
-        const int idx = i * 32 + lane, r = idx / CH, ch = idx % CH;   // row 0-15 of the keys, 16-31 of the values
-        const int key = r & 15;
-        const uint8_t* s = src + (int64_t)(r >> 4) * half_bytes + key * (p.kv_heads * D * 2) + ch * 16;
-        attn::cp_async16(dst + r * L::PITCH + ch * 16, key < live ? s : p.kv, key < live);
+          for (int i = 0; i < CH / 2; ++i) {   // 16 keys x CH chunks: consecutive lanes along a key
+            const int idx = i * 32 + lane, r = idx / CH, ch = idx % CH;
+            attn::cp_async16(dst + r * L::PITCH + ch * 16, src + r * row_bytes + ch * 16, true);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < CH / 2; ++i) {   // zeros past the row's end
+            const int idx = i * 32 + lane, r = idx / CH, ch = idx % CH;
+            attn::cp_async16(dst + r * L::PITCH + ch * 16, r < live ? src + r * row_bytes + ch * 16 : p.kv, r < live);
+          }
+        }
       }
+      if (value == 0) valid |= (page >= 0 ? 1u : 0u) << ahead++;
+      else if (++uf < u1) {
+        dec_next<L::STEP>(p, f);
+        page = page_of(f);
+      }
+      value ^= 1;
+      fslot = fslot + 1 == L::HALVES ? 0 : fslot + 1;
     }
     attn::cp_async_commit();
   };
-
-  // the ring's first tiles; `page` runs one tile ahead of the fetches, so that its load never stands in their way
-  long long uf = u0;   // the next unit to fetch
-  int page = page_of(f);
-  int pages_in[L::STAGES];
 #pragma unroll
-  for (int s = 0; s < L::STAGES; ++s) {
-    pages_in[s] = uf < u1 ? page : -1;
-    fetch(f, pages_in[s], s);
-    ++uf;
-    if (uf < u1) {
-      dec_next<L::STEP>(p, f);
-      page = page_of(f);
-    }
-  }
+  for (int s = 0; s < L::HALVES; ++s) fetch();
 
   uint32_t qf[NT][KS][2];
   float o[NT][KS][4], m[NT][2], l[NT][2];
@@ -543,14 +556,16 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
   bool from_start = true;   // the current row's head began at the share's first unit
   int first_step = c.step;
   for (long long u = u0; u < u1; ++u) {
-    attn::cp_async_wait<L::STAGES - 1>();
+    const bool mine = valid & 1, ends = c.step + 1 == c.steps || u + 1 == u1;
+    valid >>= 1;
+    --ahead;
+    uint8_t* keys = ring + slot * L::SLOT;
+    const int vslot = slot + 1 == L::HALVES ? 0 : slot + 1;
+    uint8_t* values = ring + vslot * L::SLOT;
+    uint32_t hi[NT][2], lo[NT][2];
+    attn::cp_async_wait<L::HALVES - 1>();
     __syncwarp();
-    int mine = -1;
-#pragma unroll
-    for (int s = 0; s < L::STAGES; ++s)
-      if (s == slot) mine = pages_in[s];
-    uint8_t* tile = ring + slot * L::SLOT;
-    if (mine >= 0) {
+    if (mine) {
       const int j0 = c.step * L::STEP + warp * 16;
       const int live = dec_length(p, c.row) - j0;
       // S^T: 16 keys x 8 heads, four chains of products
@@ -559,7 +574,7 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[nt][i][0] = s[nt][i][1] = s[nt][i][2] = s[nt][i][3] = 0.f;
-      const uint32_t ka = smem_u32(tile) + ((lane & 7) + (lane & 8)) * L::PITCH + (lane >> 4) * 16;
+      const uint32_t ka = smem_u32(keys) + ((lane & 7) + (lane & 8)) * L::PITCH + (lane >> 4) * 16;
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {
         uint32_t a0, a1, a2, a3;
@@ -567,7 +582,6 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) attn::mma16816(s[nt][kk & 3], a0, a1, a2, a3, qf[nt][kk][0], qf[nt][kk][1]);
       }
-      uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float x[4];
@@ -614,9 +628,19 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
           }
         }
       }
+    }
+    // the keys' slot is free; at a row's end it is kept for the outputs
+    __syncwarp();
+    if (!ends) {
+      fetch();
+      attn::cp_async_wait<L::HALVES - 1>();
+    } else {
+      attn::cp_async_wait<L::HALVES - 2>();
+    }
+    __syncwarp();
+    if (mine) {
       // O^T += V^T P^T, 16 dimensions at a time
-      const uint32_t va =
-          smem_u32(tile) + 16 * L::PITCH + ((lane & 7) + ((lane >> 4) << 3)) * L::PITCH + ((lane >> 3) & 1) * 16;
+      const uint32_t va = smem_u32(values) + ((lane & 7) + ((lane >> 4) << 3)) * L::PITCH + ((lane >> 3) & 1) * 16;
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {
         uint32_t a0, a1, a2, a3;
@@ -629,10 +653,8 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
       }
     }
     __syncwarp();
-    const bool ends = c.step + 1 == c.steps || u + 1 == u1;
     if (ends) {
-      // the warps' sums into the slots just read, then joined: thread = one dimension of a head
-      float* mo = reinterpret_cast<float*>(tile);
+      // the warps' sums into the slots just read, eight heads each, then joined: thread = one dimension of a head
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -641,13 +663,14 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
           for (int off = 4; off < 32; off <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
         }
         const int h = nt * 8 + 2 * tq;
+        float* mo = reinterpret_cast<float*>(nt == 0 ? values : keys);
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float v = o[nt][kk][e];
             if (PAIR) v += __shfl_xor_sync(0xffffffffu, v, 2);   // the lo parts' product
-            if (!PAIR || tq < 2) mo[(h + (e & 1)) * L::OPITCH + kk * 16 + gr + (e >> 1) * 8] = v;
+            if (!PAIR || tq < 2) mo[(2 * tq + (e & 1)) * L::OPITCH + kk * 16 + gr + (e >> 1) * 8] = v;
           }
         }
         if (gr == 0) {
@@ -671,7 +694,8 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
           if (s_m[w][h] == -INFINITY && s_l[w][h] == 0.f) continue;   // a warp without keys of this row
           const float a = exp2f(s_m[w][h] - finite(mx));
           sum += a * s_l[w][h];
-          v += a * reinterpret_cast<const float*>(sm + (w * L::STAGES + slot) * L::SLOT)[h * L::OPITCH + d];
+          v += a * reinterpret_cast<const float*>(sm + (w * L::HALVES + (h < 8 ? vslot : slot)) * L::SLOT)[
+                       (h & 7) * L::OPITCH + d];
         }
         if (whole) {
           const int head = c.head * p.group + h;
@@ -688,17 +712,9 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
       }
       __syncthreads();
     }
-    // the slot is free: the tile STAGES units on
-#pragma unroll
-    for (int s = 0; s < L::STAGES; ++s)
-      if (s == slot) pages_in[s] = uf < u1 ? page : -1;
-    fetch(f, uf < u1 ? page : -1, slot);
-    ++uf;
-    if (uf < u1) {
-      dec_next<L::STEP>(p, f);
-      page = page_of(f);
-    }
-    slot = slot + 1 == L::STAGES ? 0 : slot + 1;
+    if (ends) fetch();
+    fetch();
+    slot = vslot + 1 == L::HALVES ? 0 : vslot + 1;
     if (u + 1 < u1) {
       dec_next<L::STEP>(p, c);
       if (ends) {
@@ -841,7 +857,7 @@ extern "C" int jb_attn_prep_axes(const uint16_t* pr, int64_t ldpr, int t, const 
                              kv ? static_cast<uint8_t*>(kv) + attn_layer * layer_bytes : nullptr, pages, page_bytes,
                              slots};
   if (t >= dec::PREP_MANY) {
-    launch_pdl(dec::prep_tokens_kernel, min((t + 7) / 8, 2 * dec::SHARES), 256, 0, (cudaStream_t)stream, p);
+    launch_pdl(dec::prep_tokens_kernel, min((t + 3) / 4, 3 * dec::SHARES), 128, 0, (cudaStream_t)stream, p);
     return check_launch("prep_tokens_kernel");
   }
   launch_pdl(dec::prep_axes_kernel, t, 384, 0, (cudaStream_t)stream, p);
