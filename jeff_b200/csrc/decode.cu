@@ -343,12 +343,12 @@ __global__ void __launch_bounds__(128, 3) prep_tokens_kernel(const PrepParams p)
 // a running maximum and sum. Every key and value is read once, for all query heads of its head: 4 operations a byte
 // with 4 of them, so the bound is HBM.
 //
-// Shares: a (row, key/value head) is cut into steps of WARPS x 16 tokens, all steps of the call into as many equal
+// Shares: a (row, key/value head) is cut into steps of WARPS x TILE tokens, all steps of the call into as many equal
 // shares as there are CTAs (one per SM), in row order: a share's work does not depend on how the lengths are spread. A
 // CTA finishes what it holds in full; of a row cut by a share's border each part leaves its unnormalised sum, maximum
 // and weight in scratch, and join_kernel adds a row's parts in order.
 //
-// In a CTA each warp takes one 16-token tile of a step, with a ring of its own in shared memory (cp.async of a tile's
+// In a CTA each warp takes one tile (16 or 32 tokens) of a step, with a ring of its own in shared memory (cp.async of a tile's
 // keys, then its values, tokens past the row's end as zeros) and no barrier with the other warps until a row ends, when
 // the warps' sums are joined in shared memory. Scores and output are taken transposed, S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16: the 16
 // rows of the tile are keys (then 16 of the head's dimensions), the 8 columns the query heads, so 4 query heads cost
@@ -358,11 +358,12 @@ __global__ void __launch_bounds__(128, 3) prep_tokens_kernel(const PrepParams p)
 
 template <int D>
 struct Dec {
-  static constexpr int WARPS = D == 64 ? 16 : 8;
-  static constexpr int HALVES = D == 256 ? 3 : D == 128 ? 6 : 5;   // a warp's ring, in tiles' keys or values
-  static constexpr int STEP = WARPS * 16;         // tokens
+  static constexpr int WARPS = 8;
+  static constexpr int TILE = D == 256 ? 16 : 32; // tokens of a warp's tile
+  static constexpr int HALVES = D == 64 ? 5 : 3;  // a warp's ring, in tiles' keys or values
+  static constexpr int STEP = WARPS * TILE;       // tokens
   static constexpr int PITCH = D * 2 + 16;        // bytes of a key in shared memory: ldmatrix without conflicts
-  static constexpr int SLOT = 16 * PITCH;         // a tile's keys or its values; eight heads' outputs at a row's end
+  static constexpr int SLOT = TILE * PITCH;       // a tile's keys or its values; eight heads' outputs at a row's end
   static constexpr int SMEM = WARPS * HALVES * SLOT;
   static constexpr int OPITCH = D + 8;            // floats of a head's output there
   static_assert(8 * OPITCH * 4 <= SLOT, "eight heads' outputs fit a slot");
@@ -370,6 +371,7 @@ struct Dec {
 };
 
 constexpr int SHARES = 148;   // one CTA per SM
+constexpr int HELD = 1024;    // rows whose lengths a CTA holds
 
 struct DecParams {
   const __nv_bfloat16* q;
@@ -391,8 +393,8 @@ struct DecParams {
 __device__ __forceinline__ int dec_length(const DecParams& p, int r) { return min(max(p.lengths[r], 0), p.most); }
 
 // Units (steps of one key/value head) of the rows before `row`, and of all; warp-collective.
-template <int STEP>
-__device__ void dec_units(const DecParams& p, int row, long long& before, long long& total) {
+template <int STEP, class Len>
+__device__ void dec_units(const DecParams& p, const Len& len, int row, long long& before, long long& total) {
   const int lane = threadIdx.x & 31;
   long long some = 0, all = 0;
   for (int r0 = 0; r0 < p.b; r0 += 128) {
@@ -400,7 +402,7 @@ __device__ void dec_units(const DecParams& p, int row, long long& before, long l
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = r0 + 32 * i + lane;
-      n[i] = r < p.b ? (dec_length(p, r) + STEP - 1) / STEP : 0;
+      n[i] = r < p.b ? (len(r) + STEP - 1) / STEP : 0;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -417,17 +419,17 @@ __device__ void dec_units(const DecParams& p, int row, long long& before, long l
   total = all * p.kv_heads;
 }
 
-struct Cursor {   // a unit: a step of a row's head
-  int row, head, step, steps;
+struct Cursor {   // a unit: a step of a row's head, and the row's tokens
+  int row, head, step, steps, len;
 };
 
 // The unit `u` (below the total); warp-collective.
-template <int STEP>
-__device__ Cursor dec_find(const DecParams& p, long long u) {
+template <int STEP, class Len>
+__device__ Cursor dec_find(const DecParams& p, const Len& len, long long u) {
   const int lane = threadIdx.x & 31;
   long long before = 0;
   for (int r0 = 0; r0 < p.b; r0 += 32) {
-    const int steps = r0 + lane < p.b ? (dec_length(p, r0 + lane) + STEP - 1) / STEP : 0;
+    const int n = r0 + lane < p.b ? len(r0 + lane) : 0, steps = (n + STEP - 1) / STEP;
     long long upto = (long long)steps * p.kv_heads;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -438,24 +440,25 @@ __device__ Cursor dec_find(const DecParams& p, long long u) {
     const unsigned over = __ballot_sync(0xffffffffu, upto > u);
     if (over) {
       const int l = __ffs(over) - 1;
-      const int n = __shfl_sync(0xffffffffu, steps, l);
-      const long long in = u - (__shfl_sync(0xffffffffu, upto, l) - (long long)n * p.kv_heads);
-      return {r0 + l, (int)(in / n), (int)(in % n), n};
+      const int ln = __shfl_sync(0xffffffffu, n, l), ls = __shfl_sync(0xffffffffu, steps, l);
+      const int in = (int)(u - (__shfl_sync(0xffffffffu, upto, l) - (long long)ls * p.kv_heads));
+      return {r0 + l, in / ls, in % ls, ls, ln};
     }
     before = __shfl_sync(0xffffffffu, upto, 31);
   }
-  return {p.b, 0, 0, 0};
+  return {p.b, 0, 0, 1, 0};
 }
 
-template <int STEP>
-__device__ __forceinline__ void dec_next(const DecParams& p, Cursor& c) {
+template <int STEP, class Len>
+__device__ __forceinline__ void dec_next(const DecParams& p, const Len& len, Cursor& c) {
   if (++c.step < c.steps) return;
   c.step = 0;
   if (++c.head < p.kv_heads) return;
   c.head = 0;
   do {
     ++c.row;
-    c.steps = c.row < p.b ? (dec_length(p, c.row) + STEP - 1) / STEP : 1;
+    c.len = c.row < p.b ? len(c.row) : 1;
+    c.steps = (c.len + STEP - 1) / STEP;
   } while (c.steps == 0);
 }
 
@@ -474,21 +477,29 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
   pdl_begin();
   using L = Dec<D>;
   constexpr int KS = D / 16, CH = D / 8;   // 16-wide k steps, 16-byte chunks of a key
+  constexpr int TILE = L::TILE, MT = TILE / 16, CHAINS = 4 / MT;
   extern __shared__ __align__(16) uint8_t sm[];
   __shared__ float s_m[L::WARPS][16], s_l[L::WARPS][16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, tq = lane & 3;
+  // the rows' lengths are asked for again and again: from shared memory where they fit there
+  __shared__ int s_len[HELD];
+  if (p.b <= HELD) {
+    for (int r = threadIdx.x; r < p.b; r += L::WARPS * 32) s_len[r] = dec_length(p, r);
+    __syncthreads();
+  }
+  auto length = [&](int r) { return p.b <= HELD ? s_len[r] : dec_length(p, r); };
   long long none, total;
-  dec_units<L::STEP>(p, 0, none, total);
+  dec_units<L::STEP>(p, length, 0, none, total);
   const long long shares = min((long long)SHARES, total);   // none of them empty
   if (blockIdx.x >= shares) return;
   const long long u0 = total * blockIdx.x / shares, u1 = total * (blockIdx.x + 1) / shares;
   uint8_t* ring = sm + warp * L::HALVES * L::SLOT;
-  Cursor c = dec_find<L::STEP>(p, u0), f = c;
+  Cursor c = dec_find<L::STEP>(p, length, u0), f = c;
   const int half_bytes = PAGE * p.kv_heads * D * 2;   // a page's keys of one layer, then its values
 
   auto page_of = [&](const Cursor& x) -> int {   // the page of this warp's tile of a unit, -1: none
-    const int j = x.step * L::STEP + warp * 16;
-    if (x.row >= p.b || j >= dec_length(p, x.row)) return -1;
+    const int j = x.step * L::STEP + warp * TILE;
+    if (j >= x.len) return -1;
     const int page = p.tables[(int64_t)x.row * p.table_stride + p.kv_entry + j / PAGE];
     return page >= 0 && page < p.pages ? page : -1;
   };
@@ -500,21 +511,21 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
   auto fetch = [&]() {
     if (uf < u1) {
       if (page >= 0) {
-        const int j0 = f.step * L::STEP + warp * 16;
-        const int live = min(16, dec_length(p, f.row) - j0);
+        const int j0 = f.step * L::STEP + warp * TILE;
+        const int live = min(TILE, f.len - j0);
         const uint8_t* src = p.kv + (int64_t)page * p.page_bytes + (int64_t)value * half_bytes +
                              ((j0 % PAGE) * p.kv_heads + f.head) * D * 2;
         const uint32_t dst = smem_u32(ring + fslot * L::SLOT);
         const int row_bytes = p.kv_heads * D * 2;
-        if (live == 16) {
+        if (live == TILE) {
 #pragma unroll
-          for (int i = 0; i < CH / 2; ++i) {   // 16 keys x CH chunks: consecutive lanes along a key
+          for (int i = 0; i < TILE * CH / 32; ++i) {   // TILE keys x CH chunks: consecutive lanes along a key
             const int idx = i * 32 + lane, r = idx / CH, ch = idx % CH;
             attn::cp_async16(dst + r * L::PITCH + ch * 16, src + r * row_bytes + ch * 16, true);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < CH / 2; ++i) {   // zeros past the row's end
+          for (int i = 0; i < TILE * CH / 32; ++i) {   // zeros past the row's end
             const int idx = i * 32 + lane, r = idx / CH, ch = idx % CH;
             attn::cp_async16(dst + r * L::PITCH + ch * 16, r < live ? src + r * row_bytes + ch * 16 : p.kv, r < live);
           }
@@ -522,7 +533,7 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
       }
       if (value == 0) valid |= (page >= 0 ? 1u : 0u) << ahead++;
       else if (++uf < u1) {
-        dec_next<L::STEP>(p, f);
+        dec_next<L::STEP>(p, length, f);
         page = page_of(f);
       }
       value ^= 1;
@@ -562,35 +573,47 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
     uint8_t* keys = ring + slot * L::SLOT;
     const int vslot = slot + 1 == L::HALVES ? 0 : slot + 1;
     uint8_t* values = ring + vslot * L::SLOT;
-    uint32_t hi[NT][2], lo[NT][2];
+    uint32_t hi[NT][MT][2], lo[NT][MT][2];
     attn::cp_async_wait<L::HALVES - 1>();
     __syncwarp();
     if (mine) {
-      const int j0 = c.step * L::STEP + warp * 16;
-      const int live = dec_length(p, c.row) - j0;
-      // S^T: 16 keys x 8 heads, four chains of products
-      float s[NT][4][4];
+      const int j0 = c.step * L::STEP + warp * TILE;
+      const int live = c.len - j0;
+      // S^T: TILE keys x 8 heads, four chains of products
+      float s[NT][MT][CHAINS][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[nt][i][0] = s[nt][i][1] = s[nt][i][2] = s[nt][i][3] = 0.f;
+        for (int i = 0; i < MT * CHAINS; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][i / CHAINS][i % CHAINS][e] = 0.f;
       const uint32_t ka = smem_u32(keys) + ((lane & 7) + (lane & 8)) * L::PITCH + (lane >> 4) * 16;
 #pragma unroll
-      for (int kk = 0; kk < KS; ++kk) {
-        uint32_t a0, a1, a2, a3;
-        attn::ldsm_x4(ka + kk * 32, a0, a1, a2, a3);
+      for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) attn::mma16816(s[nt][kk & 3], a0, a1, a2, a3, qf[nt][kk][0], qf[nt][kk][1]);
-      }
+        for (int mt = 0; mt < MT; ++mt) {
+          uint32_t a0, a1, a2, a3;
+          attn::ldsm_x4(ka + mt * 16 * L::PITCH + kk * 32, a0, a1, a2, a3);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            attn::mma16816(s[nt][mt][kk % CHAINS], a0, a1, a2, a3, qf[nt][kk][0], qf[nt][kk][1]);
+        }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float x[4];
+        float x[MT][4];
+        float n0 = -INFINITY, n1 = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = ((s[nt][0][e] + s[nt][1][e]) + (s[nt][2][e] + s[nt][3][e])) * p.scale_log2;
-          if (gr + (e >> 1) * 8 >= live) x[e] = -INFINITY;
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float sum = s[nt][mt][0][e];
+#pragma unroll
+            for (int i = 1; i < CHAINS; ++i) sum += s[nt][mt][i][e];
+            x[mt][e] = mt * 16 + gr + (e >> 1) * 8 < live ? sum * p.scale_log2 : -INFINITY;
+          }
+          n0 = fmaxf(n0, fmaxf(x[mt][0], x[mt][2]));
+          n1 = fmaxf(n1, fmaxf(x[mt][1], x[mt][3]));
         }
-        float n0 = fmaxf(x[0], x[2]), n1 = fmaxf(x[1], x[3]);
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
           n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, off));
@@ -612,19 +635,21 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
             o[nt][kk][3] *= a1;
           }
         }
+        const float b0 = finite(m[nt][0]), b1 = finite(m[nt][1]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = exp2f(x[e] - finite(m[nt][e & 1]));
-          l[nt][e & 1] += x[e];
-        }
+        for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-        for (int e2 = 0; e2 < 2; ++e2) {
-          const uint32_t h = pack_bf2(x[2 * e2], x[2 * e2 + 1]);
-          const uint32_t r = pack_bf2(x[2 * e2] - bf_lo(h), x[2 * e2 + 1] - bf_hi(h));
-          if (PAIR) hi[nt][e2] = transpose8x8(tq < 2 ? h : r);
-          else {
-            hi[nt][e2] = transpose8x8(h);
-            lo[nt][e2] = transpose8x8(r);
+          for (int e2 = 0; e2 < 2; ++e2) {
+            const float p0 = exp2f(x[mt][2 * e2] - b0), p1 = exp2f(x[mt][2 * e2 + 1] - b1);
+            l[nt][0] += p0;
+            l[nt][1] += p1;
+            const uint32_t h = pack_bf2(p0, p1);
+            const uint32_t r = pack_bf2(p0 - bf_lo(h), p1 - bf_hi(h));
+            if (PAIR) hi[nt][mt][e2] = transpose8x8(tq < 2 ? h : r);
+            else {
+              hi[nt][mt][e2] = transpose8x8(h);
+              lo[nt][mt][e2] = transpose8x8(r);
+            }
           }
         }
       }
@@ -642,15 +667,17 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
       // O^T += V^T P^T, 16 dimensions at a time
       const uint32_t va = smem_u32(values) + ((lane & 7) + ((lane >> 4) << 3)) * L::PITCH + ((lane >> 3) & 1) * 16;
 #pragma unroll
-      for (int kk = 0; kk < KS; ++kk) {
-        uint32_t a0, a1, a2, a3;
-        attn::ldsm_x4_trans(va + kk * 32, a0, a1, a2, a3);
+      for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          attn::mma16816(o[nt][kk], a0, a1, a2, a3, hi[nt][0], hi[nt][1]);
-          if (!PAIR) attn::mma16816(o[nt][kk], a0, a1, a2, a3, lo[nt][0], lo[nt][1]);
+        for (int mt = 0; mt < MT; ++mt) {
+          uint32_t a0, a1, a2, a3;
+          attn::ldsm_x4_trans(va + mt * 16 * L::PITCH + kk * 32, a0, a1, a2, a3);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            attn::mma16816(o[nt][kk], a0, a1, a2, a3, hi[nt][mt][0], hi[nt][mt][1]);
+            if (!PAIR) attn::mma16816(o[nt][kk], a0, a1, a2, a3, lo[nt][mt][0], lo[nt][mt][1]);
+          }
         }
-      }
     }
     __syncwarp();
     if (ends) {
@@ -716,7 +743,7 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
     fetch();
     slot = vslot + 1 == L::HALVES ? 0 : vslot + 1;
     if (u + 1 < u1) {
-      dec_next<L::STEP>(p, c);
+      dec_next<L::STEP>(p, length, c);
       if (ends) {
         begin();
         from_start = false;
@@ -727,22 +754,25 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
 }
 
 // CTA per (row, query head): the parts of a row that shares cut, joined in share order; rows without tokens are zeros;
-// nothing to do for a row that one share held in full. The parts' factors first, a thread each, then their sums.
+// nothing to do for a row that one share held in full. Bound by its chain of reads (lengths, the parts' maxima and
+// sums, their values), so a warp does all of it for 32 dimensions, without a barrier.
 template <int D>
-__global__ void __launch_bounds__(256) join_kernel(const DecParams p) {
+__global__ void __launch_bounds__(D) join_kernel(const DecParams p) {
   pdl_begin();
-  constexpr int STEP = Dec<D>::STEP;
-  __shared__ float s_w[SHARES], s_red[32], s_v[256];
+  constexpr int STEP = Dec<D>::STEP, EACH = (SHARES + 31) / 32;
   const int heads = p.kv_heads * p.group;
   const int row = blockIdx.x / heads, head = blockIdx.x % heads, g = head / p.group, h = head % p.group;
-  const int steps = (dec_length(p, row) + STEP - 1) / STEP;
-  __nv_bfloat16* y = p.y + row * p.ldy + (int64_t)head * D;
+  const int d = threadIdx.x, lane = d & 31;
+  auto length = [&](int r) { return dec_length(p, r); };
+  const int steps = (length(row) + STEP - 1) / STEP;
+  __nv_bfloat16* y = p.y + row * p.ldy + (int64_t)head * D + d;
   if (steps == 0) {
-    if (threadIdx.x < D) y[threadIdx.x] = f2bf(0.f);
+    *y = f2bf(0.f);
     return;
   }
+  const float gate = p.pr ? bf2f(p.pr[row * p.ldpr + ((int64_t)2 * head + 1) * D + d]) : 0.f;
   long long before, total;
-  dec_units<STEP>(p, row, before, total);
+  dec_units<STEP>(p, length, row, before, total);
   const long long shares = min((long long)SHARES, total);
   const long long a = before + (long long)g * steps, z = a + steps - 1;
   const long long c0 = ((a + 1) * shares - 1) / total, c1 = ((z + 1) * shares - 1) / total;   // unit u's: the last c
@@ -752,37 +782,34 @@ __global__ void __launch_bounds__(256) join_kernel(const DecParams p) {
   const float* parts = p.scratch + 2 * c0 * stride + h * (D + 2);
   const int first = total * c0 / shares == a ? 0 : stride;
   auto part = [&](int i) { return parts + (int64_t)2 * i * stride + (i == 0 ? first : 0); };
-  float m = -INFINITY, l = 0.f;
-  if ((int)threadIdx.x < count) {
-    m = part(threadIdx.x)[0];
-    l = part(threadIdx.x)[1];
-  }
-  const float mx = ew::block_max(m, s_red);
-  const float w = (int)threadIdx.x < count && !(m == -INFINITY && l == 0.f) ? exp2f(m - finite(mx)) : 0.f;
-  if ((int)threadIdx.x < count) s_w[threadIdx.x] = w;
-  const float sum = ew::block_sum(w == 0.f ? 0.f : w * l, s_red);   // its barriers order s_w too
-  // thread = (one of 256 / D interleaved sets of parts, dimension), eight loads in flight
-  constexpr int SETS = 256 / D;
-  const int d = threadIdx.x % D, set = threadIdx.x / D;
-  float v = 0.f;
-  for (int i0 = set; i0 < count; i0 += 8 * SETS) {
-    float x[8];
+  float m[EACH], l[EACH], mx = -INFINITY, sum = 0.f, v = 0.f;   // lane i of a warp: parts i, i + 32, ...
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = i0 + j * SETS < count ? part(i0 + j * SETS)[2 + d] : 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (i0 + j * SETS < count && s_w[i0 + j * SETS] != 0.f) v += s_w[i0 + j * SETS] * x[j];
+  for (int j = 0; j < EACH; ++j) {
+    const int i = lane + 32 * j;
+    m[j] = i < count ? part(i)[0] : -INFINITY;
+    l[j] = i < count ? part(i)[1] : 0.f;
+    mx = fmaxf(mx, m[j]);
   }
-  if (SETS > 1) {
-    s_v[threadIdx.x] = v;
-    __syncthreads();
-    if (set > 0) return;
+  mx = ew::warp_max(mx);
 #pragma unroll
-    for (int i = 1; i < SETS; ++i) v += s_v[i * D + d];
+  for (int j = 0; j < EACH; ++j) {
+    const float w = m[j] == -INFINITY && l[j] == 0.f ? 0.f : exp2f(m[j] - finite(mx));
+    if (w != 0.f) sum += w * l[j];
+    for (int i0 = 0; i0 < 32 && 32 * j + i0 < count; i0 += 8) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = 32 * j + i0 + i < count ? part(32 * j + i0 + i)[2 + d] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, i0 + i);
+        if (wi != 0.f) v += wi * x[i];
+      }
+    }
   }
+  sum = ew::warp_sum(sum);
   v = mx == -INFINITY && sum == 0.f ? 0.f : v / sum;
-  if (p.pr) v *= ew::sigmoid(bf2f(p.pr[row * p.ldpr + ((int64_t)2 * head + 1) * D + d]));
-  y[d] = f2bf(v);
+  if (p.pr) v *= ew::sigmoid(gate);
+  *y = f2bf(v);
 }
 
 template <int D, int NT, bool PAIR>
@@ -799,7 +826,7 @@ int dec_launch(const DecParams& p, cudaStream_t stream) {
   }
   launch_pdl(decode_kernel<D, NT, PAIR>, SHARES, Dec<D>::WARPS * 32, Dec<D>::SMEM, stream, p);
   if (int r = check_launch("decode_kernel")) return r;
-  launch_pdl(join_kernel<D>, p.b * p.kv_heads * p.group, 256, 0, stream, p);
+  launch_pdl(join_kernel<D>, p.b * p.kv_heads * p.group, D, 0, stream, p);
   return check_launch("join_kernel");
 }
 
