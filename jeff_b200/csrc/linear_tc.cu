@@ -185,6 +185,19 @@ __device__ __forceinline__ void split8_pairs(const uint4& x, uint2 f, uint4& y0,
   y0 = make_uint4(p0[0], p0[1], p0[2], p0[3]);
   y1 = make_uint4(p1[0], p1[1], p1[2], p1[3]);
 }
+// an untiled copy of whole 16-byte pieces
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(reinterpret_cast<uint64_t>(dst)),
+               "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+
 template <int N>
 struct Count {
   static constexpr int value = N;
@@ -216,9 +229,10 @@ __global__ void __launch_bounds__(THREADS, 2)
   uint64_t* k_bar = d_bar + 4;
   uint64_t* q_bar = d_bar + 5;
   uint64_t* v_bar = d_bar + 6;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + OFF_MISC + 56);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + OFF_MISC + 60);
-  volatile float* whole = reinterpret_cast<volatile float*>(sm + OFF_MISC + 64);   // [2] the chunks' decay factors
+  uint64_t* s_bar = d_bar + 7;                                    // the state's copy
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + OFF_MISC + 64);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + OFF_MISC + 68);
+  volatile float* whole = reinterpret_cast<volatile float*>(sm + OFF_MISC + 72);   // [2] the chunks' decay factors
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int qd = warp & 3, ch = warp >> 2;
@@ -229,7 +243,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     return;
   }
   if (tid == 0) {
-    for (int i = 0; i < 7; ++i) mbar_init(d_bar + i, 1);
+    for (int i = 0; i < 8; ++i) mbar_init(d_bar + i, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -296,21 +310,23 @@ __global__ void __launch_bounds__(THREADS, 2)
   };
   double carry = 0.0;         // the same warps: log-decays so far
   if (qd == 0) gates_of(0);
-  if (warp == 0 && chunks) {
-    const bool me = elect_one();
-    load_k(0, me);
-    if (OUT) load_q(0, me);
-    load_v(0, me);
-    __syncwarp();
-  }
-  // the state ahead of the segment, its loads in flight while the first gates are formed
+  // the state ahead of the segment: one copy over Kd's and V's places, which nothing needs yet
   const float* in = MODE == WHOLE ? lin::state_in(a.pool, row, h)
                     : MODE == OUTPUTS ? seg.states + ((int64_t)pair * seg.count + part) * STATE : nullptr;
-  uint32_t r[32], r2[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) r[i] = in ? __float_as_uint(in[(ch * 64 + i) * D + L]) : 0u;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) r2[i] = in ? __float_as_uint(in[(ch * 64 + 32 + i) * D + L]) : 0u;
+  float* state = reinterpret_cast<float*>(sm + OFF_K0);
+  if (warp == 0) {
+    const bool me = elect_one();
+    if (in && me) {
+      mbar_arrive_expect_tx(s_bar, STATE * 4);
+      bulk_load(state, in, STATE * 4, s_bar);
+    }
+    if (chunks) {
+      load_k(0, me);
+      if (OUT) load_q(0, me);
+      else load_v(0, me);
+    }
+    __syncwarp();
+  }
   if (qd == 0) {
     form_gates<!OUT>(gates[0], ch, g0, g1, lane, whole, carry);
     gates_of(1);
@@ -329,14 +345,26 @@ __global__ void __launch_bounds__(THREADS, 2)
     tmem_st32(s_at + 32 * half, x);
     if (!OUT) tmem_st32(s_at + TM_SMALL + 32 * half, x);
   };
+  uint32_t r[32];
   {
     const float el = OUT && chunks ? whole[0] : 1.f;
-    put_state(0, r, el);
-    put_state(1, r2, el);
+    if (in) mbar_wait(s_bar, 0, abort_flag, err, 58);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        r[i] = in ? __float_as_uint(state[(ch * 64 + half * 32 + i) * D + L]) : 0u;
+      put_state(half, r, el);
+    }
     tc_wait_st();
   }
+  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
+  if (OUT && warp == 0 && chunks) {
+    load_v(0, elect_one());
+    __syncwarp();
+  }
 
   for (int c = 0; c < chunks; ++c) {
     const uint32_t phase = (uint32_t)c & 1;
@@ -582,26 +610,35 @@ __global__ void __launch_bounds__(THREADS, 2)
   }
   float* out = MODE == WHOLE ? lin::state_out(a.pool, row, h)
                : MODE == STATES ? seg.states + ((int64_t)pair * seg.count + part) * STATE : nullptr;
-  if (ok && out) {
+  if (ok && out) {   // through shared memory, Kd's and V's places again, as one copy
+    if (tid == 0) tma_store_wait_read();
+    __syncthreads();
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
+      uint32_t small[32];
       tmem_ld32(s_at + 32 * half, r);
-      if (!OUT) tmem_ld32(s_at + TM_SMALL + 32 * half, r2);
+      if (!OUT) tmem_ld32(s_at + TM_SMALL + 32 * half, small);
       tc_wait_ld();
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        out[(ch * 64 + half * 32 + i) * D + L] =
-            OUT ? __uint_as_float(r[i]) : __uint_as_float(r[i]) + __uint_as_float(r2[i]);
+        state[(ch * 64 + half * 32 + i) * D + L] =
+            OUT ? __uint_as_float(r[i]) : __uint_as_float(r[i]) + __uint_as_float(small[i]);
+    }
+    fence_proxy_async_smem();
+    __syncthreads();
+    if (tid == 0) {
+      bulk_store(out, state, STATE * 4);
+      tma_store_commit();
     }
     if (MODE == STATES && tid == 0) seg.decay[(int64_t)pair * seg.count + part] = exp2_fast((float)carry);
   }
-  if (OUT && tid == 0) tma_store_wait_all();
+  if (tid == 0) tma_store_wait_all();
   if (!ok && warp == 0) {
     // a CTA that gave up waits (bounded) for the copies it issued before its shared memory goes away: those of the last
     // tile or two, the others having landed before these were issued
     const uint64_t t0 = global_ns();
     auto landed = [&]() {
-      bool all = !q_issued || mbar_try_wait(q_bar, (q_issued - 1) & 1);
+      bool all = (!in || mbar_try_wait(s_bar, 0)) && (!q_issued || mbar_try_wait(q_bar, (q_issued - 1) & 1));
       for (int i = max(0, k_issued - (OUT ? 1 : 2)); i < k_issued; ++i) all = all && mbar_try_wait(k_ready(i), parity(i));
       for (int i = max(0, v_issued - (OUT ? 1 : 2)); i < v_issued; ++i) all = all && mbar_try_wait(v_ready(i), parity(i));
       return all;
@@ -655,12 +692,23 @@ int tile_map(CUtensorMap* map, const void* base, const Args& a, int b, int64_t t
   return make_tmap_nd(map, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Segments of a (row, head): as many as let every CTA that fits run at once, none shorter than a chunk.
+// Segments of a (row, head). Measured on a B200, in us: one segment takes 4 + 3.5 a chunk; segments of `per` chunks, all
+// of them at once, 9 + 4.7 per + 0.045 for each segment of the call, whose states are written, joined, and read again.
+// So 8 rows of 256 tokens stay whole (20.8 us, 30.5 in two segments a head), one row of 1,001 takes segments of two
+// chunks (21.2; 24.8 of one, 66 whole), one of 8,192 as many as run at once.
 inline Seg segments(int b, int heads, int n) {
   const int chunks = (n + C - 1) / C;
   const int64_t pairs = (int64_t)b * heads;
-  const int most = (int)max((int64_t)1, FIT / pairs);
-  const int per = (chunks + most - 1) / most;
+  const int64_t most = FIT / pairs;
+  int64_t best = 4000 + 3500ll * chunks;   // ns
+  int per = chunks;
+  for (int64_t p = most ? (chunks + most - 1) / most : chunks; p < chunks && 4700 * p < best; ++p) {
+    const int64_t cost = 9000 + 4700 * p + 45 * pairs * ((chunks + p - 1) / p);
+    if (cost < best) {
+      best = cost;
+      per = (int)p;
+    }
+  }
   return {(chunks + per - 1) / per, per, nullptr, nullptr};
 }
 inline int64_t scratch_floats(int b, int heads, int n) {

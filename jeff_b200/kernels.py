@@ -390,14 +390,15 @@ def _tables_of(tables: torch.Tensor, name: str, rows: int, width: int, device: t
         raise ValueError(f"{name}: expected a tensor on {device}, got one on {tables.device}")
 
 
-def _cache_of(kv: torch.Tensor, attn_layer: int, device: torch.device) -> tuple[int, int]:
-    """(key/value heads, their width) of a cache of pages kv[page, layer, K|V, 32 tokens, head, dim]."""
-    if kv.dim() != 6 or kv.dtype != DT or kv.shape[2:4] != (2, 32):
-        raise ValueError(f"kv: expected bf16 pages (page, layer, 2, 32, heads, dim), got {kv.dtype} {tuple(kv.shape)}")
-    _rows_of(kv, "kv", DT, kv.shape, 5, device)
-    if not 0 <= attn_layer < kv.shape[1]:
-        raise ValueError(f"attn_layer {attn_layer}: the pages hold {kv.shape[1]} layers")
-    return kv.shape[4], kv.shape[5]
+def _cache_of(kv: torch.Tensor, attn_layer: int, device: torch.device) -> torch.Size:
+    """The shape of a cache of pages kv[page, layer, K|V, 32 tokens, head, dim]."""
+    shape = kv.shape
+    if len(shape) != 6 or shape[2] != 2 or shape[3] != 32:
+        raise ValueError(f"kv: expected bf16 pages (page, layer, 2, 32, heads, dim), got {kv.dtype} {tuple(shape)}")
+    _rows_of(kv, "kv", DT, shape, 5, device)
+    if not 0 <= attn_layer < shape[1]:
+        raise ValueError(f"attn_layer {attn_layer}: the pages hold {shape[1]} layers")
+    return shape
 
 
 def _on(device: torch.device, name: str, *args) -> None:
@@ -502,7 +503,7 @@ def attn_prep_axes(pr: torch.Tensor, q_w1: torch.Tensor, k_w1: torch.Tensor, inv
             _rows_of(x, name, DT, (t, C.NKV, C.HD), 3, dev)
     if slots is not None:
         _rows_of(slots, "slots", torch.int64, (t,), 1, dev)
-    if kv is not None and _cache_of(kv, attn_layer, dev) != (C.NKV, C.HD):
+    if kv is not None and _cache_of(kv, attn_layer, dev)[4:] != (C.NKV, C.HD):
         raise ValueError(f"kv: expected pages of {C.NKV} heads of {C.HD}, got {tuple(kv.shape)}")
     if out is None:
         out = torch.empty(t, C.NQ, C.HD, dtype=DT, device=dev)
@@ -516,6 +517,11 @@ def attn_prep_axes(pr: torch.Tensor, q_w1: torch.Tensor, k_w1: torch.Tensor, inv
     return out
 
 
+@functools.lru_cache(maxsize=64)
+def _decode_scratch(heads: int, kv_heads: int, dim: int) -> int:
+    return _lib.load().jb_decode_attention_scratch(heads, kv_heads, dim)
+
+
 def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, attn_layer: int, lengths: torch.Tensor,
                      kv_entry: int, *, scale: float | None = None, pr: torch.Tensor | None = None,
                      out: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
@@ -527,11 +533,12 @@ def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, at
     the SMs, whatever the lengths; scratch (fp32, jb_decode_attention_scratch of them, overwritten by every call)
     holds the cut rows' parts and is allocated unless given."""
     dev = q.device
-    if q.dim() != 3:
-        raise ValueError(f"q: expected (rows, heads, dim), got {tuple(q.shape)}")
-    b, heads, dim = q.shape
-    _rows_of(q, "q", DT, (b, heads, dim), 2, dev)
-    kv_heads, kv_dim = _cache_of(kv, attn_layer, dev)
+    shape = q.shape
+    if len(shape) != 3:
+        raise ValueError(f"q: expected (rows, heads, dim), got {tuple(shape)}")
+    b, heads, dim = shape
+    _rows_of(q, "q", DT, shape, 2, dev)
+    pages, layers, _, _, kv_heads, kv_dim = _cache_of(kv, attn_layer, dev)
     if kv_dim != dim:
         raise ValueError(f"q: heads of {dim}, the pages' keys are {kv_dim} wide")
     _tables_of(tables, "tables", b, kv_entry, dev)
@@ -540,18 +547,17 @@ def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, at
         if pr.dim() != 2 or pr.shape[1] < 2 * heads * dim:
             raise ValueError(f"pr: expected (rows, at least {2 * heads * dim}), got {tuple(pr.shape)}")
         _rows_of(pr, "pr", DT, (b, pr.shape[1]), 1, dev)
-    shape = (b, heads, dim) if pr is None else (b, heads * dim)
+        shape = (b, heads * dim)
     if out is None:
         out = torch.empty(shape, dtype=DT, device=dev)
     else:
         _rows_of(out, "out", DT, shape, len(shape) - 1, dev)
     if scratch is None:
-        scratch = torch.empty(_lib.load().jb_decode_attention_scratch(heads, kv_heads, dim), dtype=torch.float32,
-                              device=dev)
+        scratch = torch.empty(_decode_scratch(heads, kv_heads, dim), dtype=torch.float32, device=dev)
     else:
         _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), dev)
-    _on(dev, "jb_decode_attention", q.data_ptr(), q.stride(0), kv.data_ptr(), kv.shape[0], 2 * kv.stride(0), attn_layer,
-        kv.shape[1], tables.data_ptr(), tables.stride(0), tables.shape[1], kv_entry, lengths.data_ptr(), b, heads,
+    _on(dev, "jb_decode_attention", q.data_ptr(), q.stride(0), kv.data_ptr(), pages, 2 * kv.stride(0), attn_layer,
+        layers, tables.data_ptr(), tables.stride(0), tables.shape[1], kv_entry, lengths.data_ptr(), b, heads,
         kv_heads, dim, dim ** -0.5 if scale is None else scale, ptr(pr), 0 if pr is None else pr.stride(0),
         out.data_ptr(), out.stride(0), scratch.data_ptr(), scratch.numel())
     return out
@@ -596,6 +602,11 @@ def _linear_of(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
                  0 if out_tables is None else out_tables.stride(0))
 
 
+@functools.lru_cache(maxsize=256)
+def _scan_scratch(b: int, heads: int, n: int) -> int:
+    return _lib.load().jb_linear_scan_scratch(b, heads, n)
+
+
 def linear_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor,
                 tables: torch.Tensor, layer: int, *, real: torch.Tensor | None = None,
                 out_tables: torch.Tensor | None = None, out: torch.Tensor | None = None,
@@ -614,7 +625,7 @@ def linear_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     if real is not None:
         _rows_of(real, "real", torch.int32, (b,), 1, q.device)
     if scratch is None:
-        need = _lib.load().jb_linear_scan_scratch(b, heads, n)
+        need = _scan_scratch(b, heads, n)
         scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
     else:
         _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), q.device)
