@@ -624,8 +624,8 @@ def linear_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     o, pool = _linear_of(q, k, v, g, state, tables, layer, out_tables, out)
     if real is not None:
         _rows_of(real, "real", torch.int32, (b,), 1, q.device)
+    need = _scan_scratch(b, heads, n)
     if scratch is None:
-        need = _scan_scratch(b, heads, n)
         scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
     else:
         _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), q.device)
@@ -633,6 +633,8 @@ def linear_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     _on(q.device, "jb_linear_scan", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
         v.data_ptr(), v.stride(0), v.stride(1), g.data_ptr(), *steps, ptr(real), o.data_ptr(), b, n, heads, *pool,
         ptr(scratch), 0 if scratch is None else scratch.numel())
+    if need:
+        _lib.launches += 2   # in segments: their states, the join, the outputs
     return o
 
 
@@ -640,8 +642,8 @@ def linear_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
                 tables: torch.Tensor, layer: int, *, beta: torch.Tensor | None = None,
                 out_tables: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """linear_scan's recurrence for one token per row, q, k, v (b, heads, 128), g (b, heads) or (heads,): o (b, heads,
-    128), the new states written in place, or to out_tables' pages. beta (b, heads) bf16: the gated delta rule of
-    gdn_scan, v replaced by beta (v - (e^g S)^T k)."""
+    128), the new states written in place, or to out_tables' pages (rows must not share them). beta (b, heads) bf16: the
+    gated delta rule of gdn_scan, v replaced by beta (v - (e^g S)^T k)."""
     if q.dim() != 3:
         raise ValueError(f"q: expected (rows, heads, {C.DK}), got {tuple(q.shape)}")
     b, heads = q.shape[:2]

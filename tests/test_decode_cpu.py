@@ -30,9 +30,9 @@ def _tables(lib, **over):
 
 
 def _prep(lib, **over):
-    a = dict(pr=P, ldpr=5120, t=3, stride=3, kn=P, vn=P, kv=None, pages=0, page_bytes=0, layer=0, layers=0,
+    a = dict(pr=P, w1=P, ldpr=5120, t=3, stride=3, kn=P, vn=P, kv=None, pages=0, page_bytes=0, layer=0, layers=0,
              slots=None) | over
-    return lib.jb_attn_prep_axes(a["pr"], a["ldpr"], a["t"], P, P, P, P, a["stride"], 0, P, a["kn"], a["vn"], a["kv"],
+    return lib.jb_attn_prep_axes(a["pr"], a["ldpr"], a["t"], a["w1"], P, P, P, a["stride"], 0, P, a["kn"], a["vn"], a["kv"],
                                  a["pages"], a["page_bytes"], a["layer"], a["layers"], a["slots"], None)
 
 
@@ -70,6 +70,7 @@ def _step(lib, **over):
     (_prep, {"ldpr": 5112}, b"ldpr 5112"),
     (_prep, {"ldpr": 5121}, b"ldpr 5121"),
     (_prep, {"pr": ODD}, b"aligned"),
+    (_prep, {"w1": ODD}, b"aligned"),
     (_prep, {"vn": None}, b"keys and values"),
     (_prep, {"kn": None, "vn": None}, b"keys and values"),
     (_prep, {"kv": P, "pages": 4, "page_bytes": 393216, "layers": 6}, b"keys and values"),
@@ -86,10 +87,12 @@ def _step(lib, **over):
     (_decode, {"ldq": 2044}, b"row strides"),
     (_decode, {"pr": P, "ldpr": 2048}, b"row strides"),
     (_decode, {"q": ODD}, b"aligned"),
+    (_decode, {"heads": 8}, b"a scratch of 0 floats"),
     (_scan, {"n": 0}, b"0 tokens"),
     (_scan, {"heads": 0}, b"0 heads"),
     (_scan, {"tok": 2044}, b"multiples of 8"),
     (_scan, {"q": ODD}, b"aligned"),
+    (_scan, {"n": 1000}, b"a scratch of 0 floats"),
     (_scan, {"per": 7}, b"7 heads per page"),
     (_scan, {"first": 285}, b"past the block table"),
     (_scan, {"out": P, "out_stride": 2}, b"past the block table"),
@@ -99,6 +102,19 @@ def _step(lib, **over):
 def test_bad_arguments_are_refused_before_any_launch(lib, call, over, says) -> None:
     assert call(lib, **over) == -1
     assert says in lib.jb_last_error()
+
+
+def test_scratch_sizes(lib) -> None:
+    """Two cut rows' parts a share; a state and its decay for each of a long row's segments, which all run at once, and
+    none for rows that stay whole."""
+    assert lib.jb_decode_attention_scratch(8, 2, 256) == 2 * 148 * 4 * 258
+    assert lib.jb_decode_attention_scratch(34, 2, 256) == lib.jb_decode_attention_scratch(8, 0, 256) == 0
+    for b, heads, n in ((1, 16, 1000), (2, 16, 8192), (1, 1, 100000), (100, 1, 4096)):
+        floats = lib.jb_linear_scan_scratch(b, heads, n)
+        count, rest = divmod(floats, b * heads * (128 * 128 + 1))
+        assert rest == 0 and 2 <= count and b * heads * count <= 296
+    for b, heads, n in ((1, 16, 1), (1, 16, 64), (64, 16, 128), (300, 1, 8192), (0, 16, 64)):
+        assert lib.jb_linear_scan_scratch(b, heads, n) == 0
 
 
 def test_rope_axes() -> None:

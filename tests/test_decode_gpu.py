@@ -150,7 +150,8 @@ def plain_prep(pr, q_w1, k_w1, inv_freq, positions, axis_of):
 
 
 @pytest.mark.parametrize(("t", "sections", "interleaved", "reach"), [
-    (1, (32,), False, 5), (3, (11, 11, 10), True, 100), (31, (8, 12, 12), False, 9000),
+    (1, (32,), False, 5), (3, (11, 11, 10), True, 100), (31, (8, 12, 12), False, 9000), (255, (11, 11, 10), True, 8192),
+    (256, (32,), False, 8192), (257, (16, 8, 8), True, 8192),
     (64, (16, 16), False, 2 ** 31 - 1), (1000, (8, 8, 8, 8), True, 300000), (1217, (0, 32, 0), False, 60),
 ])
 def test_attn_prep_axes(t, sections, interleaved, reach) -> None:
@@ -190,6 +191,20 @@ def test_attn_prep_axes(t, sections, interleaved, reach) -> None:
     only = torch.full_like(kv, 7.0)   # the pages alone, and kn and vn alone, give the same
     q2 = kernels.attn_prep_axes(pr, q_w1, k_w1, inv_freq, positions, axes, kv=only, attn_layer=1, slots=slots)
     assert torch.equal(only, kv) and torch.equal(q2, got)
+
+
+def test_attn_prep_axes_shares_positions() -> None:
+    """Text: one row of positions standing for all axes (expanded) is the same as its copies."""
+    g = gen(3)
+    pr, w = normal(g, 70, C.ATTN_PROJ), torch.ones(256, device="cuda")
+    f = torch.rand(32, generator=g, device="cuda")
+    one = torch.arange(70, dtype=torch.int32, device="cuda")
+    axes = kernels.rope_axes([11, 11, 10], True)
+    outs = []
+    for positions in (one.expand(3, -1), one.repeat(3, 1)):
+        kn, vn = (torch.empty(70, 2, 256, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        outs.append((kernels.attn_prep_axes(pr, w, w, f, positions, axes, kn=kn, vn=vn), kn, vn))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
 
 
 def test_attn_prep_axes_agrees_with_the_text_form() -> None:
@@ -293,6 +308,9 @@ def plain_decode(q, dense, scale, pr=None):
     ([129, 16], 1, 1, 256, False),
     ([250, 47, 400, 3], 32, 8, 128, False),   # other head layouts
     ([500, 33], 16, 1, 128, True),            # sixteen query heads to one
+    ([129, 700, 16], 9, 1, 256, True),
+    ([64, 2000], 16, 1, 64, False),
+    ([300, 5], 5, 1, 256, False),
     ([40, 41, 700], 5, 1, 64, False),
     ([99, 1500], 12, 12, 64, True),
     ([64] * 200, 8, 2, 256, False),           # more rows than SMs
@@ -511,6 +529,47 @@ def test_linear_scan_long_prompt_continues() -> None:
         close(got, o, HALF * o.abs() + (HALF + 2.0 ** -13) * mag)
     for got in (end, state[page, slot]):
         close(got, s, (2.0 ** -20 + (n / 4 + 64) * ULP) * m + 1e-30)
+
+
+def test_linear_scan_broadcast_inputs() -> None:
+    """One key and value row for all rows, one token for all tokens, decays of one row for all (strides of zero)."""
+    q, k, v, g, state, tables, _, begin = linear_case(13, 3, 70, 2, 2, 0, "mixed")
+    for kk, vv, gg in ((k[:1].expand(3, -1, -1, -1), v[:1].expand(3, -1, -1, -1), g[:1].expand(3, -1, -1)),
+                       (k[:, :1].expand(-1, 70, -1, -1), v, g[:, :1].expand(-1, 70, -1))):
+        got = kernels.linear_scan(q, kk, vv, gg, state, tables, 0)
+        o, mag, _, _ = plain_linear(q, kk, vv, gg, begin, i32([70] * 3))
+        close(got, o, HALF * o.abs() + (HALF + 2.0 ** -13) * mag)
+
+
+@pytest.mark.parametrize(("b", "n", "heads"), [(1, 700, 16), (5, 130, 16)])
+def test_linear_scan_padding_holds_anything(b, n, heads) -> None:
+    """What stands past a row's end, NaN in q, k, v and g, changes nothing."""
+    q, k, v, g, state, tables, outs, _ = linear_case(14, b, n, heads, 6, 1, "mixed")
+    real = [n - 1 - 37 * r for r in range(b)]
+    want = kernels.linear_scan(q, k, v, g, state, tables, 1, real=i32(real), out_tables=outs)
+    page, slot = spots(outs, 1, heads, 6)
+    ends = state[page, slot].clone()
+    for r, count in enumerate(real):
+        for x in (q, k, v, g):
+            x[r, count:] = math.nan
+    got = kernels.linear_scan(q, k, v, g, state, tables, 1, real=i32(real), out_tables=outs)
+    assert torch.equal(got, want) and torch.equal(state[page, slot], ends)
+
+
+def test_linear_scan_captured() -> None:
+    """A captured scan of a long prompt, replayed on other inputs, gives the eager bits."""
+    q, k, v, g, state, tables, outs, _ = linear_case(15, 2, 600, 16, 6, 0, "mixed")
+    page, slot = spots(outs, 0, 16, 6)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = kernels.linear_scan(q, k, v, g, state, tables, 0, out_tables=outs)
+    for scale in (0.5, -2.0):
+        v *= scale
+        want = kernels.linear_scan(q, k, v, g, state, tables, 0, out_tables=outs).clone()
+        ends = state[page, slot].clone()
+        state[page, slot] = 0
+        graph.replay()
+        assert torch.equal(o, want) and torch.equal(state[page, slot], ends)
 
 
 def test_linear_bad_pages() -> None:
