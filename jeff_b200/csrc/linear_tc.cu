@@ -42,8 +42,8 @@ using lin::D;
 
 constexpr int C = 64, THREADS = 256;
 constexpr uint32_t TILE = C * D * 2;   // 16 KB: two 64-column atoms of 64 rows x 128 B
-constexpr int OFF_KQ = 0;              // atom a: K at a * 16384, Q (without outputs the second K) at + 8192
-constexpr int OFF_K0 = 32768;          // Kd's first part (atoms 8192 apart), then the output tile; the second V
+constexpr int OFF_KQ = 0;              // atom a: K at a * 16384, Q at + 8192
+constexpr int OFF_K0 = 32768;          // Kd's first part (atoms 8192 apart), then the output tile
 constexpr int OFF_K1 = OFF_K0 + TILE;
 constexpr int OFF_K2 = OFF_K1 + TILE;  // its third part, or with two parts the output tile
 constexpr int OFF_V = OFF_K2 + TILE;
@@ -56,7 +56,7 @@ constexpr uint32_t TM_S = 0, TM_B = 128, TM_D = 192, TM_SMALL = 128, TM_COLS = 2
 constexpr int FIT = 2 * 148;           // CTAs that run at once
 constexpr int STATE = D * D;
 
-enum Mode { WHOLE, STATES, OUTPUTS };
+enum Mode { WHOLE, OUTPUTS };
 
 struct Seg {
   int count, chunks;   // segments of a (row, head), chunks of a segment
@@ -185,6 +185,15 @@ __device__ __forceinline__ void split8_pairs(const uint4& x, uint2 f, uint4& y0,
   y0 = make_uint4(p0[0], p0[1], p0[2], p0[3]);
   y1 = make_uint4(p1[0], p1[1], p1[2], p1[3]);
 }
+// a tile's two boxes to L2
+__device__ __forceinline__ void prefetch_tile(const CUtensorMap* map, int h, int token, int row) {
+#pragma unroll
+  for (int x = 0; x < D; x += 64)
+    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(h), "r"(token), "r"(row)
+                 : "memory");
+}
 // an untiled copy of whole 16-byte pieces
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -213,7 +222,6 @@ __global__ void __launch_bounds__(THREADS, 2)
                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o, const Args a,
                 const Seg seg, int* err) {
   pdl_begin();
-  constexpr bool OUT = MODE != STATES;
   constexpr int PARTS = MODE == OUTPUTS ? 2 : 3;   // of Kd
   extern __shared__ __align__(1024) uint8_t sm[];
   uint8_t* kq = sm + OFF_KQ;
@@ -256,10 +264,9 @@ __global__ void __launch_bounds__(THREADS, 2)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t s_at = tmem + lane_bits + TM_S + 64 * ch, b_at = tmem + lane_bits + TM_B + 32 * ch;
-  const uint32_t kq_a = smem_u32(kq), pt_a = smem_u32(pt);
-  if (OUT)   // P's upper right block is never anything else
-    for (int i = tid; i < 32 * 4; i += THREADS)
-      *reinterpret_cast<uint4*>(swz(pt, i >> 2, 4 + (i & 3))) = make_uint4(0, 0, 0, 0);
+  const uint32_t kq_a = smem_u32(kq), kd_a = smem_u32(sm + OFF_K0), pt_a = smem_u32(pt);
+  for (int i = tid; i < 32 * 4; i += THREADS)   // P's upper right block is never anything else
+    *reinterpret_cast<uint4*>(swz(pt, i >> 2, 4 + (i & 3))) = make_uint4(0, 0, 0, 0);
 
   int k_issued = 0, q_issued = 0, v_issued = 0;
   const int pair = blockIdx.x / seg.count, part = blockIdx.x % seg.count;
@@ -268,39 +275,17 @@ __global__ void __launch_bounds__(THREADS, 2)
   const int begin = part * seg.chunks * C, end = min(begin + seg.chunks * C, a.n);
   const int work = min(end, stop);   // tokens past it are padding: zeros out, the state stays
   const int chunks = begin < work ? (work - begin + C - 1) / C : 0;
-  auto start_of = [&](int i) { return begin + (OUT ? i : chunks - 1 - i) * C; };   // the first token of chunk i
-  // tile loads, all issued by one lane of warp 0; without Q the K and V tiles alternate between two places, K's with
-  // Q's, the first part of Kd over it
-  auto k_place = [&](int odd) { return !OUT && odd ? OFF_KQ + 8192 : OFF_KQ; };
-  auto v_place = [&](int odd) { return !OUT && odd ? OFF_K0 : OFF_V; };
-  // chunk i's barriers of those tiles and the parity of its phase: with two places a barrier for each, since the next
-  // tile may have landed before a warp looks for this one
-  auto k_ready = [&](int i) { return !OUT && (i & 1) ? q_bar : k_bar; };
-  auto v_ready = [&](int i) { return !OUT && (i & 1) ? d_bar : v_bar; };
-  auto parity = [&](int i) { return (uint32_t)(OUT ? i : i >> 1) & 1; };
-  auto load_k = [&](int i, bool me) {
-    ++k_issued;
+  auto start_of = [&](int i) { return begin + i * C; };   // the first token of chunk i
+  // tile loads, all issued by one lane of warp 0
+  auto load = [&](const CUtensorMap* map, uint8_t* to, int step, uint64_t* bar, int i, bool me) {
     if (!me) return;
-    uint8_t* to = sm + k_place(i & 1);
-    mbar_arrive_expect_tx(k_ready(i), TILE);
-    tma_load_4d(to, &tm_k, k_ready(i), 0, h, start_of(i), row);
-    tma_load_4d(to + 16384, &tm_k, k_ready(i), 64, h, start_of(i), row);
+    mbar_arrive_expect_tx(bar, TILE);
+    tma_load_4d(to, map, bar, 0, h, start_of(i), row);
+    tma_load_4d(to + step, map, bar, 64, h, start_of(i), row);
   };
-  auto load_q = [&](int i, bool me) {
-    ++q_issued;
-    if (!me) return;
-    mbar_arrive_expect_tx(q_bar, TILE);
-    tma_load_4d(kq + 8192, &tm_q, q_bar, 0, h, start_of(i), row);
-    tma_load_4d(kq + 16384 + 8192, &tm_q, q_bar, 64, h, start_of(i), row);
-  };
-  auto load_v = [&](int i, bool me) {
-    ++v_issued;
-    if (!me) return;
-    uint8_t* to = sm + v_place(i & 1);
-    mbar_arrive_expect_tx(v_ready(i), TILE);
-    tma_load_4d(to, &tm_v, v_ready(i), 0, h, start_of(i), row);
-    tma_load_4d(to + 8192, &tm_v, v_ready(i), 64, h, start_of(i), row);
-  };
+  auto load_k = [&](int i, bool me) { ++k_issued, load(&tm_k, kq, 16384, k_bar, i, me); };
+  auto load_q = [&](int i, bool me) { ++q_issued, load(&tm_q, kq + 8192, 16384, q_bar, i, me); };
+  auto load_v = [&](int i, bool me) { ++v_issued, load(&tm_v, sm + OFF_V, 8192, v_bar, i, me); };
   const float* gp = a.g + row * a.g_row + h;
   float g0 = 0.f, g1 = 0.f;   // warps 0 and 4: the log-decays of the next chunk's tokens, 0 past the row's end
   auto gates_of = [&](int i) {
@@ -312,7 +297,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   if (qd == 0) gates_of(0);
   // the state ahead of the segment: one copy over Kd's and V's places, which nothing needs yet
   const float* in = MODE == WHOLE ? lin::state_in(a.pool, row, h)
-                    : MODE == OUTPUTS ? seg.states + ((int64_t)pair * seg.count + part) * STATE : nullptr;
+                                  : seg.states + ((int64_t)pair * seg.count + part) * STATE;
   float* state = reinterpret_cast<float*>(sm + OFF_K0);
   if (warp == 0) {
     const bool me = elect_one();
@@ -322,32 +307,28 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
     if (chunks) {
       load_k(0, me);
-      if (OUT) load_q(0, me);
-      else load_v(0, me);
+      load_q(0, me);
     }
     __syncwarp();
   }
   if (qd == 0) {
-    form_gates<!OUT>(gates[0], ch, g0, g1, lane, whole, carry);
+    form_gates<false>(gates[0], ch, g0, g1, lane, whole, carry);
     gates_of(1);
   }
   __syncthreads();
   // lane = value column, columns = key rows: into tensor memory, scaled for the first chunk, and its bf16 copy
   auto put_state = [&](int half, uint32_t (&x)[32], float el) {
-    if (OUT) {
-      uint32_t b[16];
+    uint32_t b[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) b[e] = pack_bf2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-      tmem_st16(b_at + 16 * half, b);
+    for (int e = 0; e < 16; ++e) b[e] = pack_bf2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+    tmem_st16(b_at + 16 * half, b);
 #pragma unroll
-      for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * el);
-    }
+    for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * el);
     tmem_st32(s_at + 32 * half, x);
-    if (!OUT) tmem_st32(s_at + TM_SMALL + 32 * half, x);
   };
   uint32_t r[32];
   {
-    const float el = OUT && chunks ? whole[0] : 1.f;
+    const float el = chunks ? whole[0] : 1.f;
     if (in) mbar_wait(s_bar, 0, abort_flag, err, 58);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -361,7 +342,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
-  if (OUT && warp == 0 && chunks) {
+  if (warp == 0 && chunks) {
     load_v(0, elect_one());
     __syncwarp();
   }
@@ -371,15 +352,8 @@ __global__ void __launch_bounds__(THREADS, 2)
     const int set = c & 1, live = min(C, work - start_of(c));
     const bool more = c + 1 < chunks;
     const Gates& gt = gates[set];
-    // ---- without outputs the next tiles now: the last chunk's products have read the other places
-    if (!OUT && warp == 0 && more) {
-      const bool me = elect_one();
-      load_k(c + 1, me);
-      load_v(c + 1, me);
-      __syncwarp();
-    }
     // ---- MMA1, then, where it has read the state's copy, MMA2
-    if (OUT && warp == 1) {
+    if (warp == 1) {
       mbar_wait(q_bar, phase, abort_flag, err, 53);
       __syncwarp();
       tc_fence_after();
@@ -392,7 +366,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       }
       if (issuer) tc_commit(d_bar);
       __syncwarp();
-      mbar_wait(k_ready(c), parity(c), abort_flag, err, 52);
+      mbar_wait(k_bar, phase, abort_flag, err, 52);
       mbar_wait(d_bar, phase, abort_flag, err, 55);
       __syncwarp();
       tc_fence_after();
@@ -406,27 +380,26 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
     // ---- warps 0 and 4: the next chunk's gates, and the decays of the one after it
     if (qd == 0 && more) {
-      form_gates<!OUT>(gates[set ^ 1], ch, g0, g1, lane, whole + (set ^ 1), carry);
+      form_gates<false>(gates[set ^ 1], ch, g0, g1, lane, whole + (set ^ 1), carry);
       gates_of(c + 2);
     }
     // values past the row's end may be anything: zeros, so that a zero weight keeps them out
     if (live < C) {
-      mbar_wait(v_ready(c), parity(c), abort_flag, err, 54);
+      mbar_wait(v_bar, phase, abort_flag, err, 54);
       for (int i = tid; i < (C - live) * 16; i += THREADS) {
         const int t = live + (i >> 4), x = i & 15;
-        *reinterpret_cast<uint4*>(swz(sm + v_place(set) + (x >> 3) * 8192, t, x & 7)) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(swz(sm + OFF_V + (x >> 3) * 8192, t, x & 7)) = make_uint4(0, 0, 0, 0);
       }
     }
     // ---- Kd, 16-byte pieces of the tokens' keys: five a thread of the warps that form P, six of warps 1 and 5
-    auto kd_place = [&](int u) { return sm + (!OUT && u == 0 ? k_place(set) : OFF_K0 + u * (int)TILE); };
     auto form_kd = [&](auto count, int first, int step) {   // its loads ahead of its stores
       constexpr int N = decltype(count)::value;
-      mbar_wait(k_ready(c), parity(c), abort_flag, err, 52);
+      mbar_wait(k_bar, phase, abort_flag, err, 52);
       uint4 x[N];
 #pragma unroll
       for (int it = 0; it < N; ++it) {
         const int i = min(first + it * step, C * 16 - 1), t = i >> 4, p = i & 15;
-        x[it] = *reinterpret_cast<const uint4*>(swz(sm + k_place(set) + (p >> 3) * 16384, t, p & 7));
+        x[it] = *reinterpret_cast<const uint4*>(swz(kq + (p >> 3) * 16384, t, p & 7));
       }
 #pragma unroll
       for (int it = 0; it < N; ++it) {
@@ -437,13 +410,11 @@ __global__ void __launch_bounds__(THREADS, 2)
         if (i < C * 16)
 #pragma unroll
           for (int u = 0; u < PARTS; ++u)
-            *reinterpret_cast<uint4*>(swz(kd_place(u) + (p >> 3) * (!OUT && u == 0 ? 16384 : 8192), t, p & 7)) =
+            *reinterpret_cast<uint4*>(swz(sm + OFF_K0 + u * TILE + (p >> 3) * 8192, t, p & 7)) =
                 t < live ? y[u] : make_uint4(0, 0, 0, 0);
       }
     };
-    if (!OUT) {
-      if (qd > 0) form_kd(Count<6>(), (warp - 1 - (warp > 4)) * 32 + lane, 192);
-    } else if (qd == 1) {
+    if (qd == 1) {
       form_kd(Count<6>(), 640 + ch * 32 + lane, 64);
     } else if (qd >= 2) {
       form_kd(Count<5>(), (2 * ch + qd - 2) * 32 + lane, 128);
@@ -495,7 +466,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     __syncthreads();
     if (*abort_flag) break;
     // ---- the next tiles, each once its place has been read: K by every thread and by MMA2, Q by MMA1 and MMA2
-    if (OUT && warp == 0 && more) {
+    if (warp == 0 && more) {
       const bool me = elect_one();
       load_k(c + 1, me);
       load_q(c + 1, me);
@@ -503,29 +474,27 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
     // ---- MMA3, MMA4
     if (warp == 1) {
-      mbar_wait(v_ready(c), parity(c), abort_flag, err, 54);
+      mbar_wait(v_bar, phase, abort_flag, err, 54);
       __syncwarp();
       tc_fence_after();
       const bool issuer = elect_one();
-      const uint32_t v_a = smem_u32(sm + v_place(set));
-      if (OUT) {
-        constexpr uint32_t id3 = idesc_bf16(128, 64) | A_MN;
+      const uint32_t v_a = smem_u32(sm + OFF_V);
+      constexpr uint32_t id3 = idesc_bf16(128, 64) | A_MN;
 #pragma unroll
-        for (int kk = 0; kk < C / 16; ++kk) {
-          const uint64_t av = mn_desc(v_a + kk * 2048, 8192), b = sw128_desc(pt_a + 32 * kk);
-          if (issuer) tc_mma_bf16(tmem + TM_B, av, b, id3, kk != 0);
-        }
-        if (EARLY && issuer) tc_commit(e_bar);
-        __syncwarp();
+      for (int kk = 0; kk < C / 16; ++kk) {
+        const uint64_t av = mn_desc(v_a + kk * 2048, 8192), b = sw128_desc(pt_a + 32 * kk);
+        if (issuer) tc_mma_bf16(tmem + TM_B, av, b, id3, kk != 0);
       }
+      if (EARLY && issuer) tc_commit(e_bar);
+      __syncwarp();
       constexpr uint32_t id4 = idesc_bf16(128, 128) | A_MN | B_MN;
 #pragma unroll
       for (int kk = 0; kk < C / 16; ++kk) {
         const uint64_t av = mn_desc(v_a + kk * 2048, 8192);
 #pragma unroll
         for (int p = PARTS - 1; p >= 0; --p) {   // the small parts first
-          const uint64_t b = mn_desc(smem_u32(kd_place(p)) + kk * 2048, !OUT && p == 0 ? 16384 : 8192);
-          if (issuer) tc_mma_bf16(tmem + (!OUT && p > 0 ? TM_SMALL : TM_S), av, b, id4, 1);
+          const uint64_t b = mn_desc(kd_a + p * TILE + kk * 2048, 8192);
+          if (issuer) tc_mma_bf16(tmem + TM_S, av, b, id4, 1);
         }
       }
       if (issuer) tc_commit(all_bar);
@@ -538,91 +507,84 @@ __global__ void __launch_bounds__(THREADS, 2)
       load_v(c + 1, elect_one());
       __syncwarp();
     }
-    if (OUT) {
-      // ---- O^T = e^gc D + E -> bf16 -> the output tile, laid out as the loads -> TMA store
-      const float scale = rsqrtf((float)D);
-      const int tq = lane & 3;
-      uint32_t pk[4][4];   // 8 tokens each: the warp's four groups of 8 channels
+    // ---- O^T = e^gc D + E -> bf16 -> the output tile, laid out as the loads -> TMA store
+    const float scale = rsqrtf((float)D);
+    const int tq = lane & 3;
+    uint32_t pk[4][4];   // 8 tokens each: the warp's four groups of 8 channels
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        uint32_t d[16], e[16];
-        const uint32_t ta = tmem + lane_bits + ((uint32_t)(16 * hf) << 16) + 32 * ch;
-        tmem_ld_frag(ta + TM_D, d);
-        tmem_ld_frag(ta + TM_B, e);
-        tc_wait_ld();
+    for (int hf = 0; hf < 2; ++hf) {
+      uint32_t d[16], e[16];
+      const uint32_t ta = tmem + lane_bits + ((uint32_t)(16 * hf) << 16) + 32 * ch;
+      tmem_ld_frag(ta + TM_D, d);
+      tmem_ld_frag(ta + TM_B, e);
+      tc_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = 32 * ch + 8 * i + 2 * tq;
-          const float2 f = *reinterpret_cast<const float2*>(&gt.from_start[t]);
+      for (int i = 0; i < 4; ++i) {
+        const int t = 32 * ch + 8 * i + 2 * tq;
+        const float2 f = *reinterpret_cast<const float2*>(&gt.from_start[t]);
 #pragma unroll
-          for (int g8 = 0; g8 < 2; ++g8) {
-            const float x = fmaf(f.x, __uint_as_float(d[4 * i + 2 * g8]), __uint_as_float(e[4 * i + 2 * g8])) * scale;
-            const float y =
-                fmaf(f.y, __uint_as_float(d[4 * i + 2 * g8 + 1]), __uint_as_float(e[4 * i + 2 * g8 + 1])) * scale;
-            pk[i][2 * hf + g8] = pack_bf2(t < live ? x : 0.f, t + 1 < live ? y : 0.f);
-          }
+        for (int g8 = 0; g8 < 2; ++g8) {
+          const float x = fmaf(f.x, __uint_as_float(d[4 * i + 2 * g8]), __uint_as_float(e[4 * i + 2 * g8])) * scale;
+          const float y =
+              fmaf(f.y, __uint_as_float(d[4 * i + 2 * g8 + 1]), __uint_as_float(e[4 * i + 2 * g8 + 1])) * scale;
+          pk[i][2 * hf + g8] = pack_bf2(t < live ? x : 0.f, t + 1 < live ? y : 0.f);
         }
       }
-      const int x = 32 * qd + 8 * (lane >> 3);
+    }
+    const int x = 32 * qd + 8 * (lane >> 3);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        st_frags_trans(smem_u32(swz(ot + (x >> 6) * 8192, 32 * ch + 8 * i + (lane & 7), (x & 63) >> 3)), pk[i][0],
-                       pk[i][1], pk[i][2], pk[i][3]);
-      fence_proxy_async_smem();
+    for (int i = 0; i < 4; ++i)
+      st_frags_trans(smem_u32(swz(ot + (x >> 6) * 8192, 32 * ch + 8 * i + (lane & 7), (x & 63) >> 3)), pk[i][0],
+                     pk[i][1], pk[i][2], pk[i][3]);
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) break;
+    if (tid == 0) {
+      tma_store_4d(&tm_o, ot, 0, h, start_of(c), row);
+      tma_store_4d(&tm_o, ot + 8192, 64, h, start_of(c), row);
+      tma_store_commit();
+    }
+    if (EARLY) {
+      mbar_wait(all_bar, phase, abort_flag, err, 57);
+      tc_fence_after();
+      if (warp == 0 && more) {
+        load_v(c + 1, elect_one());
+        __syncwarp();
+      }
+    }
+    if (more) {
+      // ---- the next chunk's copy of the state, and the state's decay over it
+      const float el = whole[set ^ 1];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        tmem_ld32(s_at + 32 * half, r);
+        tc_wait_ld();
+        put_state(half, r, el);
+      }
+      tc_wait_st();
+      if (tid == 0) tma_store_wait_read();   // the output tile's place is Kd's, or the next tile's
       tc_fence_before();
       __syncthreads();
-      if (*abort_flag) break;
-      if (tid == 0) {
-        tma_store_4d(&tm_o, ot, 0, h, start_of(c), row);
-        tma_store_4d(&tm_o, ot + 8192, 64, h, start_of(c), row);
-        tma_store_commit();
-      }
-      if (EARLY) {
-        mbar_wait(all_bar, phase, abort_flag, err, 57);
-        tc_fence_after();
-        if (warp == 0 && more) {
-          load_v(c + 1, elect_one());
-          __syncwarp();
-        }
-      }
-      if (more) {
-        // ---- the next chunk's copy of the state, and the state's decay over it
-        const float el = whole[set ^ 1];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          tmem_ld32(s_at + 32 * half, r);
-          tc_wait_ld();
-          put_state(half, r, el);
-        }
-        tc_wait_st();
-        if (tid == 0) tma_store_wait_read();   // the output tile's place is Kd's, or the next tile's
-        tc_fence_before();
-        __syncthreads();
-      }
     }
   }
   const bool ok = *abort_flag == 0;
-  if (OUT) {   // chunks that hold padding only
+  {   // chunks that hold padding only
     const int first = max(begin, (work + C - 1) / C * C);
     for (int i = first * 16 + tid; i < end * 16; i += THREADS)
       reinterpret_cast<uint4*>(a.o + row * a.o_row + (int64_t)(i >> 4) * a.o_tok + h * D)[i & 15] =
           make_uint4(0, 0, 0, 0);
   }
-  float* out = MODE == WHOLE ? lin::state_out(a.pool, row, h)
-               : MODE == STATES ? seg.states + ((int64_t)pair * seg.count + part) * STATE : nullptr;
+  float* out = MODE == WHOLE ? lin::state_out(a.pool, row, h) : nullptr;
   if (ok && out) {   // through shared memory, Kd's and V's places again, as one copy
     if (tid == 0) tma_store_wait_read();
     __syncthreads();
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      uint32_t small[32];
       tmem_ld32(s_at + 32 * half, r);
-      if (!OUT) tmem_ld32(s_at + TM_SMALL + 32 * half, small);
       tc_wait_ld();
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        state[(ch * 64 + half * 32 + i) * D + L] =
-            OUT ? __uint_as_float(r[i]) : __uint_as_float(r[i]) + __uint_as_float(small[i]);
+      for (int i = 0; i < 32; ++i) state[(ch * 64 + half * 32 + i) * D + L] = __uint_as_float(r[i]);
     }
     fence_proxy_async_smem();
     __syncthreads();
@@ -630,20 +592,241 @@ __global__ void __launch_bounds__(THREADS, 2)
       bulk_store(out, state, STATE * 4);
       tma_store_commit();
     }
-    if (MODE == STATES && tid == 0) seg.decay[(int64_t)pair * seg.count + part] = exp2_fast((float)carry);
   }
   if (tid == 0) tma_store_wait_all();
   if (!ok && warp == 0) {
-    // a CTA that gave up waits (bounded) for the copies it issued before its shared memory goes away: those of the last
-    // tile or two, the others having landed before these were issued
+    // a CTA that gave up waits (bounded) for the copies it issued before its shared memory goes away: the last tiles', the
+    // others having landed before these were issued
     const uint64_t t0 = global_ns();
     auto landed = [&]() {
-      bool all = (!in || mbar_try_wait(s_bar, 0)) && (!q_issued || mbar_try_wait(q_bar, (q_issued - 1) & 1));
-      for (int i = max(0, k_issued - (OUT ? 1 : 2)); i < k_issued; ++i) all = all && mbar_try_wait(k_ready(i), parity(i));
-      for (int i = max(0, v_issued - (OUT ? 1 : 2)); i < v_issued; ++i) all = all && mbar_try_wait(v_ready(i), parity(i));
+      return (!in || mbar_try_wait(s_bar, 0)) && (!k_issued || mbar_try_wait(k_bar, (k_issued - 1) & 1)) &&
+             (!q_issued || mbar_try_wait(q_bar, (q_issued - 1) & 1)) &&
+             (!v_issued || mbar_try_wait(v_bar, (v_issued - 1) & 1));
+    };
+    while (!landed() && global_ns() - t0 < kWaitNs) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TM_COLS);
+  }
+}
+
+// A segment's own contribution to the state, and its decay: S^T += V^T Kd over its chunks from the last to the first, Kd
+// with the decay to the segment's end, so that the sum in tensor memory is only added to. Kd's first part and its two
+// small ones go to accumulators of their own: the tensor core's sums truncate, and the small parts would make the large
+// sum truncate three times as often. Two halves of a chunk in turn: one's Kd is formed while the other's products run.
+constexpr int ST_K = 0;                // K tile of chunk i: atoms 16384 apart at 8192 (i % 2); Kd's first part over it
+constexpr int ST_V = 32768;            // V tile: TILE (i % 2)
+constexpr int ST_K1 = ST_V + 2 * TILE, ST_K2 = ST_K1 + TILE;   // Kd's other parts (atoms 8192 apart)
+
+__global__ void __launch_bounds__(THREADS, 2)
+    states_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Args a,
+                  const Seg seg, int* err) {
+  pdl_begin();
+  extern __shared__ __align__(1024) uint8_t sm[];
+  Gates* gates = reinterpret_cast<Gates*>(sm + OFF_G);
+  uint64_t* h_bar = reinterpret_cast<uint64_t*>(sm + OFF_MISC);   // [2] a half's products
+  uint64_t* k_bar = h_bar + 2;                                    // [2] a tile's copy, by the chunk's parity
+  uint64_t* v_bar = h_bar + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + OFF_MISC + 48);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + OFF_MISC + 52);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int qd = warp & 3, ch = warp >> 2;
+  const int L = 32 * qd + lane;
+  const uint32_t lane_bits = (uint32_t)(32 * qd) << 16;
+  if (smem_u32(sm) & 1023) {         // the swizzled tiles' base
+    if (tid == 0) atomicCAS(err, 0, JB_DEV_LAUNCH | 60);
+    return;
+  }
+  if (tid == 0) {
+    for (int i = 0; i < 6; ++i) mbar_init(h_bar + i, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TM_COLS);
+    tmem_relinquish();
+  }
+  const int pair = blockIdx.x / seg.count, part = blockIdx.x % seg.count;
+  const int row = pair / a.heads, h = pair % a.heads;
+  const int stop = a.real ? min(max(a.real[row], 0), a.n) : a.n;
+  const int begin = part * seg.chunks * C, work = min(min(begin + seg.chunks * C, a.n), stop);
+  const int chunks = begin < work ? (work - begin + C - 1) / C : 0;
+  auto start_of = [&](int i) { return begin + (chunks - 1 - i) * C; };   // the first token of the i-th chunk
+  auto k_place = [&](int i) { return sm + ST_K + (i & 1) * 8192; };
+  auto v_place = [&](int i) { return sm + ST_V + (i & 1) * TILE; };
+  int issued = 0;
+  auto load = [&](int i) {   // warp 0
+    ++issued;
+    if (elect_one()) {
+      mbar_arrive_expect_tx(k_bar + (i & 1), TILE);
+      tma_load_4d(k_place(i), &tm_k, k_bar + (i & 1), 0, h, start_of(i), row);
+      tma_load_4d(k_place(i) + 16384, &tm_k, k_bar + (i & 1), 64, h, start_of(i), row);
+      mbar_arrive_expect_tx(v_bar + (i & 1), TILE);
+      tma_load_4d(v_place(i), &tm_v, v_bar + (i & 1), 0, h, start_of(i), row);
+      tma_load_4d(v_place(i) + 8192, &tm_v, v_bar + (i & 1), 64, h, start_of(i), row);
+    }
+    __syncwarp();
+  };
+  auto ahead = [&](int i) {   // warp 4: to L2, since a tile's place is free only half a chunk before it is needed
+    if (i < chunks && elect_one()) {
+      prefetch_tile(&tm_k, h, start_of(i), row);
+      prefetch_tile(&tm_v, h, start_of(i), row);
+    }
+    __syncwarp();
+  };
+  const float* gp = a.g + row * a.g_row + h;
+  float g0 = 0.f, g1 = 0.f;   // warps 0 and 4: the log-decays of the next chunk's tokens, 0 past the row's end
+  auto gates_of = [&](int i) {
+    const int t = start_of(i) + lane;
+    g0 = i < chunks && t < work ? gp[t * a.g_tok] : 0.f;
+    g1 = i < chunks && t + 32 < work ? gp[(t + 32) * a.g_tok] : 0.f;
+  };
+  double carry = 0.0;         // the same warps: log-decays so far
+  if (qd == 0) gates_of(0);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) {
+    if (chunks > 0) load(0);
+    if (chunks > 1) load(1);
+  }
+  if (warp == 4) ahead(2);
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t s_at = tmem + lane_bits + TM_S + 64 * ch;
+  uint32_t r[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i] = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) tmem_st32(s_at + (i & 1) * 32 + (i >> 1) * TM_SMALL, r);
+  tc_wait_st();
+  if (qd == 0) {
+    form_gates<true>(gates[0], ch, g0, g1, lane, nullptr, carry);
+    gates_of(1);
+  }
+  tc_fence_before();
+  __syncthreads();
+
+  for (int c = 0; c < chunks; ++c) {
+    const int set = c & 1, live = min(C, work - start_of(c));
+    const uint32_t tile_phase = (uint32_t)(c >> 1) & 1, before = (uint32_t)(c - 1) & 1;
+    const Gates& gt = gates[set];
+    // values past the row's end may be anything: zeros, so that a zero weight keeps them out
+    if (live < C) {
+      mbar_wait(v_bar + set, tile_phase, abort_flag, err, 64);
+      for (int i = tid; i < (C - live) * 16; i += THREADS) {
+        const int t = live + (i >> 4), x = i & 15;
+        *reinterpret_cast<uint4*>(swz(v_place(c) + (x >> 3) * 8192, t, x & 7)) = make_uint4(0, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      // the half's places: free once the last chunk's products of this half are done
+      if (c > 0) {
+        mbar_wait(h_bar + half, before, abort_flag, err, 61);
+        tc_fence_after();
+      }
+      if (warp == 0 && half == 1 && c > 0 && c + 1 < chunks) load(c + 1);   // both halves of the last chunk are
+      if (warp == 4 && half == 1) ahead(c + 3);
+      if (qd == 0) {
+        if (half == 0 && c + 1 < chunks) {
+          form_gates<true>(gates[set ^ 1], ch, g0, g1, lane, nullptr, carry);
+          gates_of(c + 2);
+        }
+      } else {
+        // ---- Kd: 512 16-byte pieces over six warps, loads ahead of stores
+        mbar_wait(k_bar + set, tile_phase, abort_flag, err, 62);
+        const int me = (warp - 1 - (warp > 4)) * 32 + lane;
+        uint4 x[3];
+#pragma unroll
+        for (int it = 0; it < 3; ++it) {
+          const int i = min(me + it * 192, 511), t = 32 * half + (i >> 4), p = i & 15;
+          x[it] = *reinterpret_cast<const uint4*>(swz(k_place(c) + (p >> 3) * 16384, t, p & 7));
+        }
+#pragma unroll
+        for (int it = 0; it < 3; ++it) {
+          const int i = me + it * 192, t = 32 * half + (min(i, 511) >> 4), p = i & 15;
+          uint4 y[3];
+          split8(x[it], gt.to_end[t], y);
+          if (i < 512)
+#pragma unroll
+            for (int u = 0; u < 3; ++u)
+              *reinterpret_cast<uint4*>(swz(u == 0 ? k_place(c) + (p >> 3) * 16384
+                                                   : sm + (u == 1 ? ST_K1 : ST_K2) + (p >> 3) * 8192, t, p & 7)) =
+                  t < live ? y[u] : make_uint4(0, 0, 0, 0);
+        }
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncthreads();
+      if (*abort_flag) goto out;
+      if (warp == 1) {
+        mbar_wait(v_bar + set, tile_phase, abort_flag, err, 64);
+        __syncwarp();
+        tc_fence_after();
+        constexpr uint32_t id = idesc_bf16(128, 128) | A_MN | B_MN;
+        const bool issuer = elect_one();
+        const uint32_t v_a = smem_u32(v_place(c)), k_a = smem_u32(k_place(c)), p1 = smem_u32(sm + ST_K1),
+                       p2 = smem_u32(sm + ST_K2);
+#pragma unroll
+        for (int kk = 2 * half; kk < 2 * half + 2; ++kk) {
+          const uint64_t av = mn_desc(v_a + kk * 2048, 8192), b0 = mn_desc(k_a + kk * 2048, 16384),
+                         b1 = mn_desc(p1 + kk * 2048, 8192), b2 = mn_desc(p2 + kk * 2048, 8192);
+          if (issuer) {
+            tc_mma_bf16(tmem + TM_SMALL, av, b2, id, 1);
+            tc_mma_bf16(tmem + TM_SMALL, av, b1, id, 1);
+            tc_mma_bf16(tmem + TM_S, av, b0, id, 1);
+          }
+        }
+        if (issuer) tc_commit(h_bar + half);
+        __syncwarp();
+      }
+    }
+  }
+  if (chunks > 0) {
+    mbar_wait(h_bar, (uint32_t)(chunks - 1) & 1, abort_flag, err, 61);
+    mbar_wait(h_bar + 1, (uint32_t)(chunks - 1) & 1, abort_flag, err, 61);
+    tc_fence_after();
+  }
+out:
+  __syncthreads();
+  const bool ok = *abort_flag == 0;
+  if (!ok && warp == 0) {
+    // a CTA that gave up waits (bounded) for the copies it issued before its shared memory goes away: the last two tiles',
+    // the others having landed before these were issued
+    const uint64_t t0 = global_ns();
+    auto landed = [&]() {
+      bool all = true;
+      for (int i = max(0, issued - 2); i < issued; ++i)
+        all = all && mbar_try_wait(k_bar + (i & 1), (i >> 1) & 1) && mbar_try_wait(v_bar + (i & 1), (i >> 1) & 1);
       return all;
     };
     while (!landed() && global_ns() - t0 < kWaitNs) {
+    }
+  }
+  if (ok) {   // through shared memory as one copy
+    float* state = reinterpret_cast<float*>(sm);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t small[32];
+      tmem_ld32(s_at + 32 * half, r);
+      tmem_ld32(s_at + TM_SMALL + 32 * half, small);
+      tc_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        state[(ch * 64 + half * 32 + i) * D + L] = __uint_as_float(r[i]) + __uint_as_float(small[i]);
+    }
+    fence_proxy_async_smem();
+    __syncthreads();
+    if (tid == 0) {
+      bulk_store(seg.states + ((int64_t)pair * seg.count + part) * STATE, state, STATE * 4);
+      tma_store_commit();
+      tma_store_wait_all();
+      seg.decay[(int64_t)pair * seg.count + part] = exp2_fast((float)carry);
     }
   }
   tc_fence_before();
@@ -737,7 +920,9 @@ int scan(const Args& a, int b, float* scratch, cudaStream_t stream) {
   const int64_t parts = (int64_t)b * a.heads * seg.count;
   seg.states = scratch;
   seg.decay = scratch + parts * STATE;
-  if ((st = launch<STATES>(m, a, seg, b, stream))) return st;
+  if ((st = gdnc::configure(states_kernel, ALLOC, "linear states_kernel"))) return st;
+  launch_pdl(states_kernel, (unsigned)parts, THREADS, ALLOC, stream, m[1], m[2], a, seg, device_status_word());
+  if ((st = check_launch("linear states_kernel"))) return st;
   launch_pdl(join_kernel, dim3(b * a.heads, STATE / 4 / 256), 256, 0, stream, a, seg);
   if ((st = check_launch("linear join_kernel"))) return st;
   return launch<OUTPUTS>(m, a, seg, b, stream);
