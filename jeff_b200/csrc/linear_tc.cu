@@ -50,7 +50,7 @@ constexpr int OFF_V = OFF_K2 + TILE;
 constexpr int OFF_P = OFF_V + TILE;    // 64 rows x 128 B
 constexpr int OFF_G = OFF_P + TILE / 2;   // two sets of gates
 constexpr int OFF_MISC = OFF_G + 2 * 7 * C * 4;
-constexpr int ALLOC = OFF_MISC + 80;
+constexpr int ALLOC = OFF_MISC + 112;
 static_assert(2 * (ALLOC + 1024) <= 228 * 1024, "two CTAs per SM");
 constexpr uint32_t TM_S = 0, TM_B = 128, TM_D = 192, TM_SMALL = 128, TM_COLS = 256;
 constexpr int FIT = 2 * 148;           // CTAs that run at once
@@ -617,37 +617,40 @@ __global__ void __launch_bounds__(THREADS, 2)
 // A segment's own contribution to the state, and its decay: S^T += V^T Kd over its chunks from the last to the first, Kd
 // with the decay to the segment's end, so that the sum in tensor memory is only added to. Kd's first part and its two
 // small ones go to accumulators of their own: the tensor core's sums truncate, and the small parts would make the large
-// sum truncate three times as often. Two halves of a chunk in turn: one's Kd is formed while the other's products run.
+// sum truncate three times as often. Warps 0-7 form Kd, warp 8 fetches the tiles and issues the products, warp 9 forms
+// the gates a chunk ahead; two halves of a chunk in turn, one's Kd formed while the other's products run. They meet at
+// mbarriers only.
+constexpr int ST_THREADS = 320;
 constexpr int ST_K = 0;                // K tile of chunk i: atoms 16384 apart at 8192 (i % 2); Kd's first part over it
 constexpr int ST_V = 32768;            // V tile: TILE (i % 2)
 constexpr int ST_K1 = ST_V + 2 * TILE, ST_K2 = ST_K1 + TILE;   // Kd's other parts (atoms 8192 apart)
 
-__global__ void __launch_bounds__(THREADS, 2)
+__global__ void __launch_bounds__(ST_THREADS, 2)
     states_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Args a,
                   const Seg seg, int* err) {
   pdl_begin();
   extern __shared__ __align__(1024) uint8_t sm[];
   Gates* gates = reinterpret_cast<Gates*>(sm + OFF_G);
-  uint64_t* h_bar = reinterpret_cast<uint64_t*>(sm + OFF_MISC);   // [2] a half's products
-  uint64_t* k_bar = h_bar + 2;                                    // [2] a tile's copy, by the chunk's parity
-  uint64_t* v_bar = h_bar + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + OFF_MISC + 48);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + OFF_MISC + 52);
+  uint64_t* done = reinterpret_cast<uint64_t*>(sm + OFF_MISC);    // [2] a half's products
+  uint64_t* k_bar = done + 2;                                     // [2] a tile's copy, by the chunk's parity
+  uint64_t* v_bar = done + 4;
+  uint64_t* formed = done + 6;                                    // [2] a half's Kd: eight warps
+  uint64_t* g_bar = done + 8;                                     // [2] a chunk's gates, by its parity
+  uint64_t* g_read = done + 10;                                   // [2] that they have been read: eight warps
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + OFF_MISC + 96);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + OFF_MISC + 100);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int qd = warp & 3, ch = warp >> 2;
-  const int L = 32 * qd + lane;
-  const uint32_t lane_bits = (uint32_t)(32 * qd) << 16;
   if (smem_u32(sm) & 1023) {         // the swizzled tiles' base
     if (tid == 0) atomicCAS(err, 0, JB_DEV_LAUNCH | 60);
     return;
   }
   if (tid == 0) {
-    for (int i = 0; i < 6; ++i) mbar_init(h_bar + i, 1);
+    for (int i = 0; i < 12; ++i) mbar_init(done + i, i == 6 || i == 7 || i >= 10 ? 8 : 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 1) {
+  if (warp == 8) {
     tmem_alloc(tmem_slot, TM_COLS);
     tmem_relinquish();
   }
@@ -659,179 +662,178 @@ __global__ void __launch_bounds__(THREADS, 2)
   auto start_of = [&](int i) { return begin + (chunks - 1 - i) * C; };   // the first token of the i-th chunk
   auto k_place = [&](int i) { return sm + ST_K + (i & 1) * 8192; };
   auto v_place = [&](int i) { return sm + ST_V + (i & 1) * TILE; };
-  int issued = 0;
-  auto load = [&](int i) {   // warp 0
-    ++issued;
-    if (elect_one()) {
+  auto odd = [](int i) { return (uint32_t)i & 1; };          // a barrier that every chunk uses: chunk i's phase
+  auto odd2 = [](int i) { return (uint32_t)(i >> 1) & 1; };  // one that every other chunk uses
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < 8) {
+    // the accumulators' first values
+    uint32_t r[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = 0u;
+    const uint32_t s_at = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + TM_S + 64 * (warp >> 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tmem_st32(s_at + (i & 1) * 32 + (i >> 1) * TM_SMALL, r);
+    tc_wait_st();
+    for (int c = 0; c < chunks && !*abort_flag; ++c) {
+      const int live = min(C, work - start_of(c));
+      const Gates& gt = gates[c & 1];
+      // values past the row's end may be anything: zeros, so that a zero weight keeps them out
+      if (live < C) {
+        mbar_wait(v_bar + (c & 1), odd2(c), abort_flag, err, 64);
+        for (int i = tid; i < (C - live) * 16; i += 256) {
+          const int t = live + (i >> 4), x = i & 15;
+          *reinterpret_cast<uint4*>(swz(v_place(c) + (x >> 3) * 8192, t, x & 7)) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      mbar_wait(k_bar + (c & 1), odd2(c), abort_flag, err, 62);
+      mbar_wait(g_bar + (c & 1), odd2(c), abort_flag, err, 63);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (c > 0) mbar_wait(done + half, odd(c - 1), abort_flag, err, 61);   // the places of this half's Kd are free
+        uint4 x[2];
+#pragma unroll
+        for (int it = 0; it < 2; ++it) {
+          const int t = 32 * half + 16 * it + (tid >> 4), p = tid & 15;
+          x[it] = *reinterpret_cast<const uint4*>(swz(k_place(c) + (p >> 3) * 16384, t, p & 7));
+        }
+#pragma unroll
+        for (int it = 0; it < 2; ++it) {
+          const int t = 32 * half + 16 * it + (tid >> 4), p = tid & 15;
+          uint4 y[3];
+          split8(x[it], gt.to_end[t], y);
+#pragma unroll
+          for (int u = 0; u < 3; ++u)
+            *reinterpret_cast<uint4*>(swz(u == 0 ? k_place(c) + (p >> 3) * 16384
+                                                 : sm + (u == 1 ? ST_K1 : ST_K2) + (p >> 3) * 8192, t, p & 7)) =
+                t < live ? y[u] : make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(formed + half);
+      }
+      if (lane == 0) mbar_arrive(g_read + (c & 1));
+    }
+  } else if (warp == 8) {
+    const bool me = elect_one();
+    int issued = 0;
+    auto load = [&](int i) {
+      ++issued;
+      if (!me) return;
       mbar_arrive_expect_tx(k_bar + (i & 1), TILE);
       tma_load_4d(k_place(i), &tm_k, k_bar + (i & 1), 0, h, start_of(i), row);
       tma_load_4d(k_place(i) + 16384, &tm_k, k_bar + (i & 1), 64, h, start_of(i), row);
       mbar_arrive_expect_tx(v_bar + (i & 1), TILE);
       tma_load_4d(v_place(i), &tm_v, v_bar + (i & 1), 0, h, start_of(i), row);
       tma_load_4d(v_place(i) + 8192, &tm_v, v_bar + (i & 1), 64, h, start_of(i), row);
-    }
-    __syncwarp();
-  };
-  auto ahead = [&](int i) {   // warp 4: to L2, since a tile's place is free only half a chunk before it is needed
-    if (i < chunks && elect_one()) {
-      prefetch_tile(&tm_k, h, start_of(i), row);
-      prefetch_tile(&tm_v, h, start_of(i), row);
-    }
-    __syncwarp();
-  };
-  const float* gp = a.g + row * a.g_row + h;
-  float g0 = 0.f, g1 = 0.f;   // warps 0 and 4: the log-decays of the next chunk's tokens, 0 past the row's end
-  auto gates_of = [&](int i) {
-    const int t = start_of(i) + lane;
-    g0 = i < chunks && t < work ? gp[t * a.g_tok] : 0.f;
-    g1 = i < chunks && t + 32 < work ? gp[(t + 32) * a.g_tok] : 0.f;
-  };
-  double carry = 0.0;         // the same warps: log-decays so far
-  if (qd == 0) gates_of(0);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  if (warp == 0) {
+    };
+    auto ahead = [&](int i) {   // to L2, since a tile's place is free only half a chunk before it is needed
+      if (i < chunks && me) {
+        prefetch_tile(&tm_k, h, start_of(i), row);
+        prefetch_tile(&tm_v, h, start_of(i), row);
+      }
+    };
     if (chunks > 0) load(0);
     if (chunks > 1) load(1);
-  }
-  if (warp == 4) ahead(2);
-  const uint32_t tmem = *tmem_slot;
-  const uint32_t s_at = tmem + lane_bits + TM_S + 64 * ch;
-  uint32_t r[32];
+    ahead(2);
+    constexpr uint32_t id = idesc_bf16(128, 128) | A_MN | B_MN;
+    for (int c = 0; c < chunks && !*abort_flag; ++c) {
+      mbar_wait(v_bar + (c & 1), odd2(c), abort_flag, err, 64);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) r[i] = 0u;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) tmem_st32(s_at + (i & 1) * 32 + (i >> 1) * TM_SMALL, r);
-  tc_wait_st();
-  if (qd == 0) {
-    form_gates<true>(gates[0], ch, g0, g1, lane, nullptr, carry);
-    gates_of(1);
-  }
-  tc_fence_before();
-  __syncthreads();
-
-  for (int c = 0; c < chunks; ++c) {
-    const int set = c & 1, live = min(C, work - start_of(c));
-    const uint32_t tile_phase = (uint32_t)(c >> 1) & 1, before = (uint32_t)(c - 1) & 1;
-    const Gates& gt = gates[set];
-    // values past the row's end may be anything: zeros, so that a zero weight keeps them out
-    if (live < C) {
-      mbar_wait(v_bar + set, tile_phase, abort_flag, err, 64);
-      for (int i = tid; i < (C - live) * 16; i += THREADS) {
-        const int t = live + (i >> 4), x = i & 15;
-        *reinterpret_cast<uint4*>(swz(v_place(c) + (x >> 3) * 8192, t, x & 7)) = make_uint4(0, 0, 0, 0);
-      }
-    }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      // the half's places: free once the last chunk's products of this half are done
-      if (c > 0) {
-        mbar_wait(h_bar + half, before, abort_flag, err, 61);
-        tc_fence_after();
-      }
-      if (warp == 0 && half == 1 && c > 0 && c + 1 < chunks) load(c + 1);   // both halves of the last chunk are
-      if (warp == 4 && half == 1) ahead(c + 3);
-      if (qd == 0) {
-        if (half == 0 && c + 1 < chunks) {
-          form_gates<true>(gates[set ^ 1], ch, g0, g1, lane, nullptr, carry);
-          gates_of(c + 2);
+      for (int half = 0; half < 2; ++half) {
+        if (half == 1 && c > 0 && c + 1 < chunks) {   // the last chunk's products are done: its places are the next's
+          mbar_wait(done + 1, odd(c - 1), abort_flag, err, 61);
+          load(c + 1);
         }
-      } else {
-        // ---- Kd: 512 16-byte pieces over six warps, loads ahead of stores
-        mbar_wait(k_bar + set, tile_phase, abort_flag, err, 62);
-        const int me = (warp - 1 - (warp > 4)) * 32 + lane;
-        uint4 x[3];
-#pragma unroll
-        for (int it = 0; it < 3; ++it) {
-          const int i = min(me + it * 192, 511), t = 32 * half + (i >> 4), p = i & 15;
-          x[it] = *reinterpret_cast<const uint4*>(swz(k_place(c) + (p >> 3) * 16384, t, p & 7));
-        }
-#pragma unroll
-        for (int it = 0; it < 3; ++it) {
-          const int i = me + it * 192, t = 32 * half + (min(i, 511) >> 4), p = i & 15;
-          uint4 y[3];
-          split8(x[it], gt.to_end[t], y);
-          if (i < 512)
-#pragma unroll
-            for (int u = 0; u < 3; ++u)
-              *reinterpret_cast<uint4*>(swz(u == 0 ? k_place(c) + (p >> 3) * 16384
-                                                   : sm + (u == 1 ? ST_K1 : ST_K2) + (p >> 3) * 8192, t, p & 7)) =
-                  t < live ? y[u] : make_uint4(0, 0, 0, 0);
-        }
-      }
-      fence_proxy_async_smem();
-      tc_fence_before();
-      __syncthreads();
-      if (*abort_flag) goto out;
-      if (warp == 1) {
-        mbar_wait(v_bar + set, tile_phase, abort_flag, err, 64);
+        if (half == 1) ahead(c + 3);
+        mbar_wait(formed + half, odd(c), abort_flag, err, 65);
         __syncwarp();
         tc_fence_after();
-        constexpr uint32_t id = idesc_bf16(128, 128) | A_MN | B_MN;
-        const bool issuer = elect_one();
         const uint32_t v_a = smem_u32(v_place(c)), k_a = smem_u32(k_place(c)), p1 = smem_u32(sm + ST_K1),
                        p2 = smem_u32(sm + ST_K2);
 #pragma unroll
         for (int kk = 2 * half; kk < 2 * half + 2; ++kk) {
           const uint64_t av = mn_desc(v_a + kk * 2048, 8192), b0 = mn_desc(k_a + kk * 2048, 16384),
                          b1 = mn_desc(p1 + kk * 2048, 8192), b2 = mn_desc(p2 + kk * 2048, 8192);
-          if (issuer) {
+          if (me) {
             tc_mma_bf16(tmem + TM_SMALL, av, b2, id, 1);
             tc_mma_bf16(tmem + TM_SMALL, av, b1, id, 1);
             tc_mma_bf16(tmem + TM_S, av, b0, id, 1);
           }
         }
-        if (issuer) tc_commit(h_bar + half);
+        if (me) tc_commit(done + half);
         __syncwarp();
       }
     }
+    if (*abort_flag) {
+      // a CTA that gave up waits (bounded) for the copies it issued before its shared memory goes away: the last two
+      // tiles', the others having landed before these were issued
+      const uint64_t t0 = global_ns();
+      auto landed = [&]() {
+        bool all = true;
+        for (int i = max(0, issued - 2); i < issued; ++i)
+          all = all && mbar_try_wait(k_bar + (i & 1), odd2(i)) && mbar_try_wait(v_bar + (i & 1), odd2(i));
+        return all;
+      };
+      while (!landed() && global_ns() - t0 < kWaitNs) {
+      }
+    }
+  } else {
+    const float* gp = a.g + row * a.g_row + h;
+    auto gate = [&](int i, int t) { return i < chunks && t < work ? gp[t * a.g_tok] : 0.f; };   // 0 past the row's end
+    double carry = 0.0;
+    float g0 = gate(0, start_of(0) + lane), g1 = gate(0, start_of(0) + 32 + lane);
+    for (int c = 0; c < chunks && !*abort_flag; ++c) {
+      const float x0 = g0, x1 = g1;
+      g0 = gate(c + 1, start_of(c + 1) + lane);
+      g1 = gate(c + 1, start_of(c + 1) + 32 + lane);
+      if (c > 1) mbar_wait(g_read + (c & 1), odd2(c - 2), abort_flag, err, 66);
+      double before = carry;
+      form_gates<true>(gates[c & 1], 0, x0, x1, lane, nullptr, before);
+      form_gates<true>(gates[c & 1], 1, x0, x1, lane, nullptr, carry);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(g_bar + (c & 1));
+    }
+    if (lane == 0) seg.decay[(int64_t)pair * seg.count + part] = exp2_fast((float)carry);
   }
   if (chunks > 0) {
-    mbar_wait(h_bar, (uint32_t)(chunks - 1) & 1, abort_flag, err, 61);
-    mbar_wait(h_bar + 1, (uint32_t)(chunks - 1) & 1, abort_flag, err, 61);
-    tc_fence_after();
+    mbar_wait(done, odd(chunks - 1), abort_flag, err, 61);
+    mbar_wait(done + 1, odd(chunks - 1), abort_flag, err, 61);
   }
-out:
+  tc_fence_before();
   __syncthreads();
-  const bool ok = *abort_flag == 0;
-  if (!ok && warp == 0) {
-    // a CTA that gave up waits (bounded) for the copies it issued before its shared memory goes away: the last two tiles',
-    // the others having landed before these were issued
-    const uint64_t t0 = global_ns();
-    auto landed = [&]() {
-      bool all = true;
-      for (int i = max(0, issued - 2); i < issued; ++i)
-        all = all && mbar_try_wait(k_bar + (i & 1), (i >> 1) & 1) && mbar_try_wait(v_bar + (i & 1), (i >> 1) & 1);
-      return all;
-    };
-    while (!landed() && global_ns() - t0 < kWaitNs) {
-    }
-  }
-  if (ok) {   // through shared memory as one copy
+  tc_fence_after();
+  if (*abort_flag == 0) {   // through shared memory as one copy
     float* state = reinterpret_cast<float*>(sm);
+    if (warp < 8) {
+      const int L = 32 * (warp & 3) + lane, ch = warp >> 2;
+      const uint32_t s_at = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + TM_S + 64 * ch;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      uint32_t small[32];
-      tmem_ld32(s_at + 32 * half, r);
-      tmem_ld32(s_at + TM_SMALL + 32 * half, small);
-      tc_wait_ld();
+      for (int half = 0; half < 2; ++half) {
+        uint32_t r[32], small[32];
+        tmem_ld32(s_at + 32 * half, r);
+        tmem_ld32(s_at + TM_SMALL + 32 * half, small);
+        tc_wait_ld();
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        state[(ch * 64 + half * 32 + i) * D + L] = __uint_as_float(r[i]) + __uint_as_float(small[i]);
+        for (int i = 0; i < 32; ++i)
+          state[(ch * 64 + half * 32 + i) * D + L] = __uint_as_float(r[i]) + __uint_as_float(small[i]);
+      }
+      fence_proxy_async_smem();
     }
-    fence_proxy_async_smem();
+    tc_fence_before();
     __syncthreads();
     if (tid == 0) {
       bulk_store(seg.states + ((int64_t)pair * seg.count + part) * STATE, state, STATE * 4);
       tma_store_commit();
       tma_store_wait_all();
-      seg.decay[(int64_t)pair * seg.count + part] = exp2_fast((float)carry);
     }
   }
-  tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tmem, TM_COLS);
   }
@@ -921,7 +923,7 @@ int scan(const Args& a, int b, float* scratch, cudaStream_t stream) {
   seg.states = scratch;
   seg.decay = scratch + parts * STATE;
   if ((st = gdnc::configure(states_kernel, ALLOC, "linear states_kernel"))) return st;
-  launch_pdl(states_kernel, (unsigned)parts, THREADS, ALLOC, stream, m[1], m[2], a, seg, device_status_word());
+  launch_pdl(states_kernel, (unsigned)parts, ST_THREADS, ALLOC, stream, m[1], m[2], a, seg, device_status_word());
   if ((st = check_launch("linear states_kernel"))) return st;
   launch_pdl(join_kernel, dim3(b * a.heads, STATE / 4 / 256), 256, 0, stream, a, seg);
   if ((st = check_launch("linear join_kernel"))) return st;
