@@ -79,8 +79,7 @@ def stream_ptr(stream: torch.cuda.Stream | None = None) -> int:
     return s.cuda_stream
 
 
-# Kernel launches each entry point makes (the product with LoRA makes two: shrink, then the fused GEMM; the decode
-# attention two: the shares, then the join); counted
+# Kernel launches each entry point makes (the product with LoRA makes two: shrink, then the fused GEMM); counted
 # by `call` so a caller can report how many of this library's kernels a recorded pass launches.
 _NO_LAUNCH = {"jb_abi_version", "jb_last_error", "jb_device_status", "jb_decode_attention_scratch",
               "jb_linear_scan_scratch"}
@@ -94,7 +93,7 @@ def call(name: str, *args) -> None:
     global launches
     lib = _lib if _lib is not None else load()
     if name not in _NO_LAUNCH:
-        launches += 2 if (name in _PRODUCTS and args[11]) or name == "jb_decode_attention" else 1   # args[11]: rank
+        launches += 2 if (name in _PRODUCTS and args[11]) else 1   # args[11]: rank
     status = getattr(lib, name)(*args)
     if status != 0:
         msg = lib.jb_last_error().decode(errors="replace")

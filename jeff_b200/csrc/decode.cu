@@ -1,6 +1,8 @@
 // Single tokens over the prefix pool: block tables and slot maps from request lengths, the attention input side with
 // several rotary axes writing straight into the cache, and the attention of one new token per row over its pages.
 
+#include <atomic>
+
 namespace jb {
 namespace dec {
 
@@ -349,7 +351,8 @@ __global__ void __launch_bounds__(128, 3) prep_tokens_kernel(const PrepParams p)
 // Shares: a (row, key/value head) is cut into steps of WARPS x TILE tokens, all steps of the call into as many equal
 // shares as there are CTAs (one per SM), in row order: a share's work does not depend on how the lengths are spread. A
 // CTA finishes what it holds in full; of a row cut by a share's border each part leaves its unnormalised sum, maximum
-// and weight in scratch, and join_kernel adds a row's parts in order.
+// and weight in scratch, and the CTA that leaves the last of them adds the row's parts, in share order whoever it is
+// (one launch instead of a second one of 5 to 7 us for the sums).
 //
 // In a CTA each warp takes one tile (16 or 32 tokens) of a step, with a ring of its own in shared memory (cp.async of a tile's
 // keys, then its values, tokens past the row's end as zeros) and no barrier with the other warps until a row ends, when
@@ -371,10 +374,20 @@ struct Dec {
   static constexpr int SLOT = TILE * PITCH;       // a tile's keys or its values; eight heads' outputs at a row's end
   static constexpr int SMEM = WARPS * HALVES * SLOT;
   static_assert(8 * D * 4 <= SLOT, "eight heads' outputs fit a slot");
-  static_assert(SMEM + 4096 <= 227 * 1024, "shared memory");
+  static_assert(SMEM + 16384 <= 227 * 1024, "shared memory");
 };
 
 constexpr int SHARES = 148;   // one CTA per SM
+__host__ __device__ constexpr int dec_part(int group, int dim) { return (group * (dim + 2) + 3) & ~3; }   // floats
+inline int64_t dec_scratch(int group, int dim) { return 4 * SHARES + (int64_t)2 * SHARES * dec_part(group, dim); }
+// a call's tag: 64 bits that memory does not hold by chance
+inline unsigned long long dec_tag() {
+  static std::atomic<unsigned long long> calls{0};
+  unsigned long long x = (calls.fetch_add(1, std::memory_order_relaxed) + 1) * 0x9e3779b97f4a7c15ull;
+  x ^= x >> 29;
+  x *= 0xd1342543de82ef95ull;
+  return x | 1;
+}
 constexpr int HELD = 1024;    // rows whose lengths a CTA holds
 
 struct DecParams {
@@ -391,7 +404,12 @@ struct DecParams {
   int64_t ldpr;
   __nv_bfloat16* y;
   int64_t ldy;
-  float* scratch;
+  // what cut rows leave: two flags a share, then two parts a share. A part is there when its flag holds the call's tag:
+  // the memory may hold anything before a call, and who joins a row's parts clears their flags, so that a replay of the
+  // call (the same tag) starts without them too
+  volatile unsigned long long* flags;
+  unsigned long long tag;
+  float* parts;
 };
 
 __device__ __forceinline__ int dec_length(const DecParams& p, int r) { return min(max(p.lengths[r], 0), p.most); }
@@ -475,6 +493,70 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return r;
 }
 
+// The parts of a cut row's key/value head, joined in share order: share c0's part, whose slot is its first if it began
+// with the row, and the following shares' first slots. A part: the group's values, then their maxima, then their sums.
+// First the parts' factors, a warp a head; then the values, four of them a lane.
+constexpr int WEIGHTS = 16 * (SHARES + 1);
+
+template <int D>
+__device__ void dec_join(const DecParams& p, int row, int kv_head, int c0, int count, bool first, float* s_w) {
+  constexpr int EACH = (SHARES + 31) / 32, AHEAD = 8;   // parts in flight
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t stride = dec_part(p.group, D);
+  auto part = [&](int i) { return p.parts + (2 * (c0 + i) + (i == 0 && !first ? 1 : 0)) * stride; };
+  for (int h = warp; h < p.group; h += 8) {
+    float m[EACH], l[EACH], mx = -INFINITY, sum = 0.f;   // lane i: parts i, i + 32, ...
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int i = lane + 32 * j;
+      m[j] = i < count ? __ldcg(part(i) + p.group * D + h) : -INFINITY;
+      l[j] = i < count ? __ldcg(part(i) + p.group * (D + 1) + h) : 0.f;
+      mx = fmaxf(mx, m[j]);
+    }
+    mx = ew::warp_max(mx);
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const float w = m[j] == -INFINITY && l[j] == 0.f ? 0.f : exp2f(m[j] - finite(mx));
+      if (w != 0.f) sum += w * l[j];
+      if (lane + 32 * j < SHARES) s_w[h * (SHARES + 1) + lane + 32 * j] = w;
+    }
+    sum = ew::warp_sum(sum);
+    if (lane == 0) s_w[h * (SHARES + 1) + SHARES] = mx == -INFINITY && sum == 0.f ? INFINITY : sum;
+  }
+  __syncthreads();
+  for (int i4 = threadIdx.x; i4 < p.group * D / 4; i4 += 256) {
+    const int h = i4 * 4 / D, d = i4 * 4 % D, head = kv_head * p.group + h;
+    const float* w = s_w + h * (SHARES + 1);
+    uint2 gate = make_uint2(0, 0);
+    if (p.pr) gate = *reinterpret_cast<const uint2*>(p.pr + row * p.ldpr + ((int64_t)2 * head + 1) * D + d);
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < count; i0 += AHEAD) {
+      float4 x[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        x[i] = __ldcg(reinterpret_cast<const float4*>(part(min(i0 + i, count - 1))) + i4);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const float f = i0 + i < count ? w[i0 + i] : 0.f;
+        if (f == 0.f) continue;   // a part without keys may hold anything
+        v[0] += f * x[i].x;
+        v[1] += f * x[i].y;
+        v[2] += f * x[i].z;
+        v[3] += f * x[i].w;
+      }
+    }
+    const float sum = w[SHARES];
+    const float g[4] = {bf_lo(gate.x), bf_hi(gate.x), bf_lo(gate.y), bf_hi(gate.y)};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] /= sum;
+      if (p.pr) v[e] *= ew::sigmoid(g[e]);
+    }
+    *reinterpret_cast<uint2*>(p.y + row * p.ldy + (int64_t)head * D + d) =
+        make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
+  }
+}
+
 // NT: 8-column tiles of query heads; PAIR: at most 4 query heads, the weights' lo parts in columns 4-7
 template <int D, int NT, bool PAIR>
 __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const DecParams p) {
@@ -484,6 +566,7 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
   constexpr int TILE = L::TILE, MT = TILE / 16, CHAINS = 4 / MT;
   extern __shared__ __align__(16) uint8_t sm[];
   __shared__ float s_m[L::WARPS][16], s_l[L::WARPS][16];
+  __shared__ float s_w[WEIGHTS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, tq = lane & 3;
   // the rows' lengths are asked for again and again: from shared memory where they fit there
   __shared__ int s_len[HELD];
@@ -494,6 +577,9 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
   auto length = [&](int r) { return p.b <= HELD ? s_len[r] : dec_length(p, r); };
   long long none, total;
   dec_units<L::STEP>(p, length, 0, none, total);
+  for (int r = blockIdx.x; r < p.b; r += gridDim.x)   // rows without tokens
+    if (length(r) == 0)
+      for (int i = threadIdx.x; i < p.kv_heads * p.group * D; i += L::WARPS * 32) p.y[r * p.ldy + i] = f2bf(0.f);
   const long long shares = min((long long)SHARES, total);   // none of them empty
   if (blockIdx.x >= shares) return;
   const long long u0 = total * blockIdx.x / shares, u1 = total * (blockIdx.x + 1) / shares;
@@ -714,7 +800,7 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
       }
       __syncthreads();
       const bool whole = first_step == 0 && c.step + 1 == c.steps;
-      float* part = p.scratch + (2 * (int64_t)blockIdx.x + (from_start ? 0 : 1)) * p.group * (D + 2);
+      float* part = p.parts + (2 * (int64_t)blockIdx.x + (from_start ? 0 : 1)) * dec_part(p.group, D);
       for (int i = threadIdx.x; i < p.group * D; i += L::WARPS * 32) {
         const int h = i / D, d = i % D;
         float mx = -INFINITY;
@@ -735,11 +821,36 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
           if (p.pr) v *= ew::sigmoid(bf2f(p.pr[c.row * p.ldpr + ((int64_t)2 * head + 1) * D + d]));
           p.y[c.row * p.ldy + (int64_t)head * D + d] = f2bf(v);
         } else {
-          part[h * (D + 2) + 2 + d] = v;
+          part[i] = v;
           if (d == 0) {
-            part[h * (D + 2)] = mx;
-            part[h * (D + 2) + 1] = sum;
+            part[p.group * D + h] = mx;
+            part[p.group * (D + 1) + h] = sum;
           }
+        }
+      }
+      if (!whole) {
+        // the row's units a .. z and their shares c0 .. c1 (unit u's: the last c with total * c / shares <= u)
+        const long long a = u - c.step, z = a + c.steps - 1;
+        const int c0 = (int)(((a + 1) * shares - 1) / total), c1 = (int)(((z + 1) * shares - 1) / total);
+        const int count = c1 - c0 + 1;
+        const bool first = total * c0 / shares == a;
+        auto slot_of = [&](int i) { return 2 * (c0 + i) + (i == 0 && !first ? 1 : 0); };
+        // the part, then its flag, then the others' flags: of the CTAs whose fences come in this order, the last sees
+        // all of them (a second one may, and then joins the same parts to the same values)
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          p.flags[slot_of(blockIdx.x - c0)] = p.tag;
+          __threadfence();
+        }
+        __syncthreads();
+        bool there = true;
+        for (int i = threadIdx.x; i < count; i += L::WARPS * 32) there &= p.flags[slot_of(i)] == p.tag;
+        if (__syncthreads_and(there)) {
+          __threadfence();
+          dec_join<D>(p, c.row, c.head, c0, count, first, s_w);
+          __syncthreads();
+          for (int i = threadIdx.x; i < count; i += L::WARPS * 32) p.flags[slot_of(i)] = 0;
         }
       }
       __syncthreads();
@@ -758,72 +869,11 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
   }
 }
 
-// CTA per (row, query head): the parts of a row that shares cut, joined in share order; rows without tokens are zeros;
-// nothing to do for a row that one share held in full. Bound by its chain of reads (lengths, the parts' maxima and
-// sums, their values), so a warp does all of it for 32 dimensions, without a barrier.
-template <int D>
-__global__ void __launch_bounds__(D) join_kernel(const DecParams p) {
-  pdl_begin();
-  constexpr int STEP = Dec<D>::STEP, EACH = (SHARES + 31) / 32;
-  const int heads = p.kv_heads * p.group;
-  const int row = blockIdx.x / heads, head = blockIdx.x % heads, g = head / p.group, h = head % p.group;
-  const int d = threadIdx.x, lane = d & 31;
-  auto length = [&](int r) { return dec_length(p, r); };
-  const int steps = (length(row) + STEP - 1) / STEP;
-  __nv_bfloat16* y = p.y + row * p.ldy + (int64_t)head * D + d;
-  if (steps == 0) {
-    *y = f2bf(0.f);
-    return;
-  }
-  const float gate = p.pr ? bf2f(p.pr[row * p.ldpr + ((int64_t)2 * head + 1) * D + d]) : 0.f;
-  long long before, total;
-  dec_units<STEP>(p, length, row, before, total);
-  const long long shares = min((long long)SHARES, total);
-  const long long a = before + (long long)g * steps, z = a + steps - 1;
-  const long long c0 = ((a + 1) * shares - 1) / total, c1 = ((z + 1) * shares - 1) / total;   // unit u's: the last c
-  if (c0 == c1) return;                                                      // with total * c / shares <= u
-  const int stride = p.group * (D + 2), count = (int)(c1 - c0) + 1;
-  // share c0 + i's part: its slot 0 holds what began with the share
-  const float* parts = p.scratch + 2 * c0 * stride + h * (D + 2);
-  const int first = total * c0 / shares == a ? 0 : stride;
-  auto part = [&](int i) { return parts + (int64_t)2 * i * stride + (i == 0 ? first : 0); };
-  float m[EACH], l[EACH], mx = -INFINITY, sum = 0.f, v = 0.f;   // lane i of a warp: parts i, i + 32, ...
-#pragma unroll
-  for (int j = 0; j < EACH; ++j) {
-    const int i = lane + 32 * j;
-    m[j] = i < count ? part(i)[0] : -INFINITY;
-    l[j] = i < count ? part(i)[1] : 0.f;
-    mx = fmaxf(mx, m[j]);
-  }
-  mx = ew::warp_max(mx);
-#pragma unroll
-  for (int j = 0; j < EACH; ++j) {
-    const float w = m[j] == -INFINITY && l[j] == 0.f ? 0.f : exp2f(m[j] - finite(mx));
-    if (w != 0.f) sum += w * l[j];
-    for (int i0 = 0; i0 < 32 && 32 * j + i0 < count; i0 += 8) {
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 32 * j + i0 + i < count ? part(32 * j + i0 + i)[2 + d] : 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float wi = __shfl_sync(0xffffffffu, w, i0 + i);
-        if (wi != 0.f) v += wi * x[i];
-      }
-    }
-  }
-  sum = ew::warp_sum(sum);
-  v = mx == -INFINITY && sum == 0.f ? 0.f : v / sum;
-  if (p.pr) v *= ew::sigmoid(gate);
-  *y = f2bf(v);
-}
-
 template <int D, int NT, bool PAIR>
 int dec_launch(const DecParams& p, cudaStream_t stream) {
   if (int r = gdnc::configure(decode_kernel<D, NT, PAIR>, Dec<D>::SMEM, "decode_kernel: cudaFuncSetAttribute")) return r;
   launch_pdl(decode_kernel<D, NT, PAIR>, SHARES, Dec<D>::WARPS * 32, Dec<D>::SMEM, stream, p);
-  if (int r = check_launch("decode_kernel")) return r;
-  launch_pdl(join_kernel<D>, p.b * p.kv_heads * p.group, D, 0, stream, p);
-  return check_launch("join_kernel");
+  return check_launch("decode_kernel");
 }
 
 template <int D>
@@ -913,21 +963,22 @@ extern "C" int jb_decode_attention(const uint16_t* q, int64_t ldq, const void* k
              "jb_decode_attention: q, the pages, pr and y must be 16-byte aligned");
   const int group = heads / kv_heads;
   JB_REQUIRE((int64_t)b * heads <= 0x7fffffff, "jb_decode_attention: %d rows of %d heads", b, heads);
-  JB_REQUIRE(scratch && scratch_floats >= (int64_t)2 * dec::SHARES * group * (dim + 2),
-             "jb_decode_attention: a scratch of %lld floats, %lld are needed", (long long)scratch_floats,
-             (long long)2 * dec::SHARES * group * (dim + 2));
+  JB_REQUIRE(scratch && scratch_floats >= dec::dec_scratch(group, dim) && dec::aligned16(scratch),
+             "jb_decode_attention: a scratch of %lld floats (16-byte aligned), %lld are needed",
+             (long long)scratch_floats, (long long)dec::dec_scratch(group, dim));
   const int64_t most = min((int64_t)(width - kv_entry) * dec::PAGE, (int64_t)0x7fffffc0);
   const dec::DecParams p = {reinterpret_cast<const __nv_bfloat16*>(q), ldq,
                             static_cast<const uint8_t*>(kv) + attn_layer * layer_bytes, pages, page_bytes, tables,
                             table_stride, kv_entry, (int)most, lengths, b, kv_heads, group, dim,
                             scale * 1.4426950408889634f, reinterpret_cast<const __nv_bfloat16*>(pr), ldpr,
-                            reinterpret_cast<__nv_bfloat16*>(y), ldy, scratch};
+                            reinterpret_cast<__nv_bfloat16*>(y), ldy,
+                            reinterpret_cast<unsigned long long*>(scratch), dec::dec_tag(), scratch + 4 * dec::SHARES};
   const cudaStream_t st = (cudaStream_t)stream;
   return dim == 64 ? dec::dec_launch<64>(p, st) : dim == 128 ? dec::dec_launch<128>(p, st) : dec::dec_launch<256>(p, st);
 }
 
 extern "C" int jb_decode_attention_scratch(int heads, int kv_heads, int dim) {
   return kv_heads > 0 && heads >= kv_heads && heads / kv_heads <= 16 && dim > 0 && dim <= 256
-             ? 2 * jb::dec::SHARES * (heads / kv_heads) * (dim + 2)
+             ? (int)jb::dec::dec_scratch(heads / kv_heads, dim)
              : 0;
 }

@@ -105,9 +105,9 @@ def test_bad_arguments_are_refused_before_any_launch(lib, call, over, says) -> N
 
 
 def test_scratch_sizes(lib) -> None:
-    """Two cut rows' parts a share; a state and its decay for each of a long row's segments, which all run at once, and
+    """Two cut rows' flags and parts a share; a state and its decay for each of a long row's segments, which all run at once, and
     none for rows that stay whole."""
-    assert lib.jb_decode_attention_scratch(8, 2, 256) == 2 * 148 * 4 * 258
+    assert lib.jb_decode_attention_scratch(8, 2, 256) == 2 * 148 * (2 + 4 * 258)
     assert lib.jb_decode_attention_scratch(34, 2, 256) == lib.jb_decode_attention_scratch(8, 0, 256) == 0
     for b, heads, n in ((1, 16, 1000), (2, 16, 8192), (1, 1, 100000), (100, 1, 4096)):
         floats = lib.jb_linear_scan_scratch(b, heads, n)

@@ -396,6 +396,31 @@ def test_decode_attention_bad_pages_and_lengths() -> None:
     close(got, want, tol)
 
 
+def test_decode_attention_scratch_holds_anything() -> None:
+    """The scratch needs no zeroing: NaN, ones in every bit, what other calls of the same and of other shapes left; a
+    captured call replayed on it again and again gives the same bits."""
+    g = gen(30)
+    lengths = [1000, 3, 2500]
+    kv, tables, dense = cache(g, lengths, 1, 0, 2, 256, entry=0)
+    q, n = normal(g, 3, 8, 256), i32(lengths)
+    scratch = torch.full((kernels._decode_scratch(16, 1, 256),), math.nan, device="cuda")
+    want = kernels.decode_attention(q, kv, tables, 0, n, 0)
+    close(want, *plain_decode(q, dense, 1 / 16))
+    wide = normal(g, 3, 12, 256)
+    for fill in (None, -1, 0, None, 2 ** 31 - 1):
+        if fill is not None:
+            scratch.view(torch.int32).fill_(fill)
+        kernels.decode_attention(wide, kv, tables, 0, n, 0, scratch=scratch)
+        assert torch.equal(kernels.decode_attention(q, kv, tables, 0, n, 0, scratch=scratch), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = kernels.decode_attention(q, kv, tables, 0, n, 0, scratch=scratch)
+    for _ in range(5):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
+
+
 def test_decode_attention_far_pages() -> None:
     """A cache whose bytes pass 32 bits, its last page among those read."""
     g = gen(12)
