@@ -58,12 +58,22 @@ struct Args {
 // One CTA per (row, head); warp w holds key rows [16 w, 16 w + 16) of the state in registers, lane l value columns
 // [4 l, 4 l + 4): 16-byte accesses, 512 contiguous bytes a warp and instruction, all 16 of a thread in flight.
 
+// S = e S + k v (one key row, four columns), and c += q S
+__device__ __forceinline__ void advance(float4& S, float e, float k, const float4& v, float q, float4& c) {
+  S.x = S.x * e + k * v.x;
+  S.y = S.y * e + k * v.y;
+  S.z = S.z * e + k * v.z;
+  S.w = S.w * e + k * v.w;
+  c.x += S.x * q;
+  c.y += S.y * q;
+  c.z += S.z * q;
+  c.w += S.w * q;
+}
 __device__ __forceinline__ float4 ld_bf4(const __nv_bfloat16* p) {
   const uint2 u = *reinterpret_cast<const uint2*>(p);
   return make_float4(bf_lo(u.x), bf_hi(u.x), bf_lo(u.y), bf_hi(u.y));
 }
 
-template <bool DELTA>
 __global__ void __launch_bounds__(256) recurrent_kernel(const Args a) {
   pdl_begin();
   __shared__ float sk[D], sq[D];
@@ -80,50 +90,12 @@ __global__ void __launch_bounds__(256) recurrent_kernel(const Args a) {
   for (int t = 0; t < stop; ++t) {
     if (threadIdx.x < D) sk[threadIdx.x] = bf2f(a.k[row * a.k_row + t * a.k_tok + h * D + threadIdx.x]);
     else sq[threadIdx.x - D] = bf2f(a.q[row * a.q_row + t * a.q_tok + h * D + threadIdx.x - D]);
-    float4 v = ld_bf4(a.v + row * a.v_row + t * a.v_tok + h * D + 4 * lane);
+    const float4 v = ld_bf4(a.v + row * a.v_row + t * a.v_tok + h * D + 4 * lane);
     const float e = expf(a.g[row * a.g_row + t * a.g_tok + h]);
     __syncthreads();
     float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (DELTA) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float kk = sk[warp * 16 + i];
-        c.x += S[i].x * kk;
-        c.y += S[i].y * kk;
-        c.z += S[i].z * kk;
-        c.w += S[i].w * kk;
-      }
-      part[warp][lane] = c;
-      __syncthreads();
-      c = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        const float4 x = part[w][lane];
-        c.x += x.x;
-        c.y += x.y;
-        c.z += x.z;
-        c.w += x.w;
-      }
-      const float b = bf2f(a.beta[(int64_t)row * a.heads + h]);
-      v.x = b * (v.x - e * c.x);
-      v.y = b * (v.y - e * c.y);
-      v.z = b * (v.z - e * c.z);
-      v.w = b * (v.w - e * c.w);
-      c = make_float4(0.f, 0.f, 0.f, 0.f);
-      __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float kk = sk[warp * 16 + i], qq = sq[warp * 16 + i];
-      S[i].x = S[i].x * e + kk * v.x;
-      S[i].y = S[i].y * e + kk * v.y;
-      S[i].z = S[i].z * e + kk * v.z;
-      S[i].w = S[i].w * e + kk * v.w;
-      c.x += S[i].x * qq;
-      c.y += S[i].y * qq;
-      c.z += S[i].z * qq;
-      c.w += S[i].w * qq;
-    }
+    for (int i = 0; i < 16; ++i) advance(S[i], e, sk[warp * 16 + i], v, sq[warp * 16 + i], c);
     part[warp][lane] = c;
     __syncthreads();
     if (threadIdx.x < D) {
@@ -140,6 +112,83 @@ __global__ void __launch_bounds__(256) recurrent_kernel(const Args a) {
   if (out)
 #pragma unroll
     for (int i = 0; i < 16; ++i) reinterpret_cast<float4*>(out + (warp * 16 + i) * D)[lane] = S[i];
+}
+
+// ------------------------------------------------------------------ one token
+//
+// Reads and writes each state once (128 KB a head): bound by HBM, and for one row by its chain of reads. The columns of a
+// state are independent, so a CTA takes 32 of them: 64 CTAs for one row's 16 heads, and no CTA with more than 16 KB to
+// wait for. 8 lanes cover a key row's 32 columns, a warp instruction four rows; a thread's eight rows stay in registers.
+
+template <bool DELTA>
+__global__ void __launch_bounds__(128) step_kernel(const Args a) {
+  pdl_begin();
+  __shared__ float4 part[2][4][8];
+  const int pair = blockIdx.x >> 2, row = pair / a.heads, h = pair % a.heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane >> 3, col = (blockIdx.x & 3) * 32 + (lane & 7) * 4;
+  const float* in = state_in(a.pool, row, h);
+  float4 S[8];   // key rows 32 warp + 4 i + sub
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    S[i] = in ? *reinterpret_cast<const float4*>(in + (32 * warp + 4 * i + sub) * D + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+  float kk[8], qq[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    kk[i] = bf2f(a.k[row * a.k_row + h * D + 32 * warp + 4 * i + sub]);
+    qq[i] = bf2f(a.q[row * a.q_row + h * D + 32 * warp + 4 * i + sub]);
+  }
+  float4 v = ld_bf4(a.v + row * a.v_row + h * D + col);
+  const float e = expf(a.g[row * a.g_row + h]);
+  // the sum over all key rows: the lanes of a column, then the four warps
+  auto total = [&](float4 c, int buf) {
+#pragma unroll
+    for (int o = 8; o < 32; o <<= 1) {
+      c.x += __shfl_xor_sync(0xffffffffu, c.x, o);
+      c.y += __shfl_xor_sync(0xffffffffu, c.y, o);
+      c.z += __shfl_xor_sync(0xffffffffu, c.z, o);
+      c.w += __shfl_xor_sync(0xffffffffu, c.w, o);
+    }
+    if (sub == 0) part[buf][warp][lane & 7] = c;
+    __syncthreads();
+    c = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float4 x = part[buf][w][lane & 7];
+      c.x += x.x;
+      c.y += x.y;
+      c.z += x.z;
+      c.w += x.w;
+    }
+    return c;
+  };
+  if (DELTA) {
+    float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      c.x += S[i].x * kk[i];
+      c.y += S[i].y * kk[i];
+      c.z += S[i].z * kk[i];
+      c.w += S[i].w * kk[i];
+    }
+    c = total(c, 0);
+    const float b = bf2f(a.beta[(int64_t)row * a.heads + h]);
+    v.x = b * (v.x - e * c.x);
+    v.y = b * (v.y - e * c.y);
+    v.z = b * (v.z - e * c.z);
+    v.w = b * (v.w - e * c.w);
+  }
+  float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
+  float* out = state_out(a.pool, row, h);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    advance(S[i], e, kk[i], v, qq[i], c);
+    if (out) *reinterpret_cast<float4*>(out + (32 * warp + 4 * i + sub) * D + col) = S[i];
+  }
+  c = total(c, 1);
+  const float scale = rsqrtf((float)D);
+  if (threadIdx.x < 8)
+    *reinterpret_cast<uint2*>(a.o + row * a.o_row + h * D + col) =
+        make_uint2(pack_bf2(c.x * scale, c.y * scale), pack_bf2(c.z * scale, c.w * scale));
 }
 
 inline bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }

@@ -36,7 +36,7 @@ extern "C" int jb_linear_scan(const uint16_t* q, int64_t q_row, int64_t q_tok, c
                (long long)need);
     return lintc::scan(a, b, scratch, (cudaStream_t)stream);
   }
-  launch_pdl(lin::recurrent_kernel<false>, b * heads, 256, 0, (cudaStream_t)stream, a);
+  launch_pdl(lin::recurrent_kernel, b * heads, 256, 0, (cudaStream_t)stream, a);
   return check_launch("linear recurrent_kernel");
 }
 
@@ -59,7 +59,7 @@ extern "C" int jb_linear_step(const uint16_t* q, int64_t q_row, const uint16_t* 
                         table_stride, out_tables, out_stride}};
   if (int st = lin::check("jb_linear_step", a, b)) return st;
   JB_REQUIRE(out_tables, "jb_linear_step: null pointer (out_tables: where the new states go)");
-  if (beta) launch_pdl(lin::recurrent_kernel<true>, b * heads, 256, 0, (cudaStream_t)stream, a);
-  else launch_pdl(lin::recurrent_kernel<false>, b * heads, 256, 0, (cudaStream_t)stream, a);
-  return check_launch("linear recurrent_kernel");
+  JB_REQUIRE((int64_t)b * heads <= 0x1fffffff, "jb_linear_step: %d rows of %d heads", b, heads);
+  launch_pdl(beta ? lin::step_kernel<true> : lin::step_kernel<false>, 4 * b * heads, 128, 0, (cudaStream_t)stream, a);
+  return check_launch("linear step_kernel");
 }
