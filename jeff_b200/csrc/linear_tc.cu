@@ -19,8 +19,7 @@
 // is zero, one a product of two vectors, two need exponentials), and the outputs leave while MMA4 runs; the next tiles
 // are fetched as soon as theirs have been read. A (row, head) is one CTA, or, where those are fewer than the CTAs that
 // fit, is cut into segments of whole chunks: a first launch leaves each segment's own contribution to the state in
-// scratch (no Q, no outputs; from the last chunk to the first, Kd = e^{decay to the segment's end} K, so that the sum
-// in tensor memory is never touched), a second turns these into the state ahead of each segment and the final one, the
+// scratch (states_kernel), a second turns these into the state ahead of each segment and the final one, the
 // third computes the outputs. Three bounds were measured on the way: the tensor core needs 65 cycles for an M128 N128
 // K16 product and 49 for N64, 1500 a chunk with outputs and 780 without, against HBM's 2800 and 1400; a batch of
 // products waited for costs another 540 cycles, the gates' chain of sums and exponentials 1200, so what bounds a chunk is
@@ -134,13 +133,15 @@ __device__ __forceinline__ float exp2_fast(float x) {   // ex2.approx: 2 ulp
   return y;
 }
 
-// One of two warps' half of a chunk's gates; a, b: the log-decays of tokens lane and lane + 32, in: the decay (base 2)
-// already in `carry`, which grows by the chunk's. ONLY_END: `to_end` alone, and to `carry`'s end.
+// a log-decay in base 2, -inf as a number whose exponential is 0
+__device__ __forceinline__ double log_decay(float g) { return (g < -1e4f ? -1e4f : g) * 1.4426950408889634; }
+
+// One of two warps' half of a chunk's gates; a, b: the log-decays of tokens lane and lane + 32. ONLY_END: `to_end` alone,
+// to the segment's end, `left` being the decay (base 2) from the chunk's first token on; it shrinks by the chunk's.
 template <bool ONLY_END>
 __device__ __forceinline__ void form_gates(Gates& g, int half, float a, float b, int lane, volatile float* whole,
-                                           double& carry) {
-  constexpr double L2E = 1.4426950408889634;
-  double x = (a < -1e4f ? -1e4f : a) * L2E, y = (b < -1e4f ? -1e4f : b) * L2E;
+                                           double& left) {
+  double x = log_decay(a), y = log_decay(b);
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const double yx = __shfl_up_sync(0xffffffffu, x, off), yy = __shfl_up_sync(0xffffffffu, y, off);
@@ -154,7 +155,7 @@ __device__ __forceinline__ void form_gates(Gates& g, int half, float a, float b,
   const double all = __shfl_sync(0xffffffffu, y, 31);
   const double z = half ? y : x;
   const int t = lane + 32 * half;
-  const float f = exp2_fast((float)(ONLY_END ? carry + (all - z) : all - z));
+  const float f = exp2_fast((float)((ONLY_END ? left : all) - z));
   g.to_end[t] = f;
   if (!ONLY_END) {
     const float hi = (float)z;
@@ -166,7 +167,7 @@ __device__ __forceinline__ void form_gates(Gates& g, int half, float a, float b,
     g.cross[t] = exp2_fast((float)(half ? z - mid : mid - z));
     if (lane == 0 && half == 0) *whole = exp2_fast((float)all);
   }
-  carry += all;
+  left -= all;
 }
 
 // eight bf16 values x times f = f0 + f1 in two bf16 parts, on bf16 pairs: x f0 = p + r exactly (16 bits in two bf16
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     g0 = i < chunks && t < work ? gp[t * a.g_tok] : 0.f;
     g1 = i < chunks && t + 32 < work ? gp[(t + 32) * a.g_tok] : 0.f;
   };
-  double carry = 0.0;         // the same warps: log-decays so far
+  double unused = 0.0;
   if (qd == 0) gates_of(0);
   // the state ahead of the segment: one copy over Kd's and V's places, which nothing needs yet
   const float* in = MODE == WHOLE ? lin::state_in(a.pool, row, h)
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     __syncwarp();
   }
   if (qd == 0) {
-    form_gates<false>(gates[0], ch, g0, g1, lane, whole, carry);
+    form_gates<false>(gates[0], ch, g0, g1, lane, whole, unused);
     gates_of(1);
   }
   __syncthreads();
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
     // ---- warps 0 and 4: the next chunk's gates, and the decays of the one after it
     if (qd == 0 && more) {
-      form_gates<false>(gates[set ^ 1], ch, g0, g1, lane, whole + (set ^ 1), carry);
+      form_gates<false>(gates[set ^ 1], ch, g0, g1, lane, whole + (set ^ 1), unused);
       gates_of(c + 2);
     }
     // values past the row's end may be anything: zeros, so that a zero weight keeps them out
@@ -614,16 +615,19 @@ __global__ void __launch_bounds__(THREADS, 2)
   }
 }
 
-// A segment's own contribution to the state, and its decay: S^T += V^T Kd over its chunks from the last to the first, Kd
-// with the decay to the segment's end, so that the sum in tensor memory is only added to. Kd's first part and its two
-// small ones go to accumulators of their own: the tensor core's sums truncate, and the small parts would make the large
-// sum truncate three times as often. Warps 0-7 form Kd, warp 8 fetches the tiles and issues the products, warp 9 forms
+// A segment's own contribution to the state, and its decay: S^T += V^T Kd over its chunks, Kd with the decay to the
+// segment's end (whose whole log-decay is summed first), so that the sum in tensor memory is only added to. The tensor
+// core's sums truncate: the state's error at 5 rows of 3,276 tokens was 1.3e-6 from the last chunk to the first, the
+// large terms at the bottom of the sum. Kd's first part and its two small ones go to accumulators of their own, since
+// the small parts would make the large sum truncate three times as often. Warps 0-7 form Kd, warp 8 fetches the tiles and issues the products, warp 9 forms
 // the gates a chunk ahead; two halves of a chunk in turn, one's Kd formed while the other's products run. They meet at
 // mbarriers only.
 constexpr int ST_THREADS = 320;
 constexpr int ST_K = 0;                // K tile of chunk i: atoms 16384 apart at 8192 (i % 2); Kd's first part over it
 constexpr int ST_V = 32768;            // V tile: TILE (i % 2)
 constexpr int ST_K1 = ST_V + 2 * TILE, ST_K2 = ST_K1 + TILE;   // Kd's other parts (atoms 8192 apart)
+constexpr int ST_TOTALS = ST_K2 + TILE;
+static_assert(ST_TOTALS + ST_THREADS / 32 * 8 <= OFF_G, "the sums fit ahead of the gates");
 
 __global__ void __launch_bounds__(ST_THREADS, 2)
     states_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Args a,
@@ -639,6 +643,7 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
   uint64_t* g_read = done + 10;                                   // [2] that they have been read: eight warps
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + OFF_MISC + 96);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + OFF_MISC + 100);
+  double* totals = reinterpret_cast<double*>(sm + ST_TOTALS);      // [10] the warps' sums of log-decays
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (smem_u32(sm) & 1023) {         // the swizzled tiles' base
@@ -659,9 +664,18 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
   const int stop = a.real ? min(max(a.real[row], 0), a.n) : a.n;
   const int begin = part * seg.chunks * C, work = min(min(begin + seg.chunks * C, a.n), stop);
   const int chunks = begin < work ? (work - begin + C - 1) / C : 0;
-  auto start_of = [&](int i) { return begin + (chunks - 1 - i) * C; };   // the first token of the i-th chunk
+  auto start_of = [&](int i) { return begin + i * C; };   // the first token of chunk i
   auto k_place = [&](int i) { return sm + ST_K + (i & 1) * 8192; };
   auto v_place = [&](int i) { return sm + ST_V + (i & 1) * TILE; };
+  // the segment's whole log-decay
+  const float* gp = a.g + row * a.g_row + h;
+  {
+    double sum = 0.0;
+    for (int t = begin + tid; t < work; t += ST_THREADS) sum += log_decay(gp[t * a.g_tok]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) totals[warp] = sum;
+  }
   auto odd = [](int i) { return (uint32_t)i & 1; };          // a barrier that every chunk uses: chunk i's phase
   auto odd2 = [](int i) { return (uint32_t)(i >> 1) & 1; };  // one that every other chunk uses
   tc_fence_before();
@@ -783,22 +797,23 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
       }
     }
   } else {
-    const float* gp = a.g + row * a.g_row + h;
     auto gate = [&](int i, int t) { return i < chunks && t < work ? gp[t * a.g_tok] : 0.f; };   // 0 past the row's end
-    double carry = 0.0;
+    double left = 0.0;
+#pragma unroll
+    for (int w = 0; w < ST_THREADS / 32; ++w) left += totals[w];
+    if (lane == 0) seg.decay[(int64_t)pair * seg.count + part] = exp2_fast((float)left);
     float g0 = gate(0, start_of(0) + lane), g1 = gate(0, start_of(0) + 32 + lane);
     for (int c = 0; c < chunks && !*abort_flag; ++c) {
       const float x0 = g0, x1 = g1;
       g0 = gate(c + 1, start_of(c + 1) + lane);
       g1 = gate(c + 1, start_of(c + 1) + 32 + lane);
       if (c > 1) mbar_wait(g_read + (c & 1), odd2(c - 2), abort_flag, err, 66);
-      double before = carry;
-      form_gates<true>(gates[c & 1], 0, x0, x1, lane, nullptr, before);
-      form_gates<true>(gates[c & 1], 1, x0, x1, lane, nullptr, carry);
+      double same = left;
+      form_gates<true>(gates[c & 1], 0, x0, x1, lane, nullptr, same);
+      form_gates<true>(gates[c & 1], 1, x0, x1, lane, nullptr, left);
       __syncwarp();
       if (lane == 0) mbar_arrive(g_bar + (c & 1));
     }
-    if (lane == 0) seg.decay[(int64_t)pair * seg.count + part] = exp2_fast((float)carry);
   }
   if (chunks > 0) {
     mbar_wait(done, odd(chunks - 1), abort_flag, err, 61);
