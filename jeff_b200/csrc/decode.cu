@@ -18,7 +18,8 @@ constexpr int PAGE = 32;   // tokens of a key/value page
 // Bound by latency: two dependent reads (the lengths, then the tables and the free list). So one launch, in which
 // every CTA repeats the two sums over all rows (8 bytes a row out of L2) instead of waiting for another's, and then
 // writes its own share: a slice of the tokens and every gridDim-th group of rows. An entry that is read (held before
-// the call) is never one that is written, so the CTAs need no order.
+// the call) is never one that is written, so the CTAs need no order. Measured on a B200: 64 rows with one more token each
+// 4.8 us, 256 fresh prompts of 16,384 tokens with their 50 fixed pages 6.0 us.
 
 constexpr int TAB_THREADS = 256, TAB_ROWS = 1024, TAB_PER = TAB_ROWS / TAB_THREADS;
 
@@ -359,6 +360,10 @@ __global__ void __launch_bounds__(128, 3) prep_tokens_kernel(const PrepParams p)
 // the warps' sums are joined in shared memory. Scores and output are taken transposed, S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16: the 16
 // rows of the tile are keys (then 16 of the head's dimensions), the 8 columns the query heads, so 4 query heads cost
 // half of what a 16-row query tile would. (tcgen05 has no use here: its 128-row tile would be filled with 4 rows.)
+// Measured on a B200, launch included: 64 ragged rows of 1 to 8,192 tokens (8 / 2 heads of 256, 537 MB) 116 us, 71% of
+// the copy rate; 33 rows of 100 to 4,096 (32 / 8 heads of 128, 283 MB) 68 us, 64%; one row of 1,000 12.4 us, latency.
+// Without the arithmetic the first takes 99 us and without the page lookups 92, so what is left is the streaming of half
+// tiles by eight warps an SM (7.2 TB/s when nothing else is done) and the ends of rows.
 // The weights are held as two bf16 parts, p = hi + lo to 2^-17: with at most 4 query heads the lo parts ride in
 // columns 4-7, which would be empty, against the queries repeated there; with more they take a second product.
 

@@ -55,8 +55,10 @@ struct Args {
 
 // ------------------------------------------------------------------ token by token
 //
-// One CTA per (row, head); warp w holds key rows [16 w, 16 w + 16) of the state in registers, lane l value columns
-// [4 l, 4 l + 4): 16-byte accesses, 512 contiguous bytes a warp and instruction, all 16 of a thread in flight.
+// The prompts of a few tokens: the state is read and written once (bound by HBM for many rows: 64 rows of 2 tokens 30 us),
+// every token after the first adds its chain of two barriers (0.6 us for one row). One CTA per (row, head); warp w holds
+// key rows [16 w, 16 w + 16) of the state in registers, lane l value columns [4 l, 4 l + 4): 16-byte accesses, 512
+// contiguous bytes a warp and instruction, all 16 of a thread in flight.
 
 // S = e S + k v (one key row, four columns), and c += q S
 __device__ __forceinline__ void advance(float4& S, float e, float k, const float4& v, float q, float4& c) {
@@ -119,6 +121,8 @@ __global__ void __launch_bounds__(256) recurrent_kernel(const Args a) {
 // Reads and writes each state once (128 KB a head): bound by HBM, and for one row by its chain of reads. The columns of a
 // state are independent, so a CTA takes 32 of them: 64 CTAs for one row's 16 heads, and no CTA with more than 16 KB to
 // wait for. 8 lanes cover a key row's 32 columns, a warp instruction four rows; a thread's eight rows stay in registers.
+// Measured on a B200 with the delta rule: 64 rows 21.3 us (135 MB: 97% of the copy rate; 24.6 with a CTA a state), one
+// row 3.9 us (5.4).
 
 template <bool DELTA>
 __global__ void __launch_bounds__(128) step_kernel(const Args a) {

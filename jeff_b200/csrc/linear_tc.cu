@@ -19,13 +19,18 @@
 // is zero, one a product of two vectors, two need exponentials), and the outputs leave while MMA4 runs; the next tiles
 // are fetched as soon as theirs have been read. A (row, head) is one CTA, or, where those are fewer than the CTAs that
 // fit, is cut into segments of whole chunks: a first launch leaves each segment's own contribution to the state in
-// scratch (states_kernel), a second turns these into the state ahead of each segment and the final one, the
-// third computes the outputs. Three bounds were measured on the way: the tensor core needs 65 cycles for an M128 N128
-// K16 product and 49 for N64, 1500 a chunk with outputs and 780 without, against HBM's 2800 and 1400; a batch of
-// products waited for costs another 540 cycles, the gates' chain of sums and exponentials 1200, so what bounds a chunk is
-// its chain of phases.
-// Waits are bounded (%globaltimer, 2 s): on expiry the CTA records JB_DEV_TIMEOUT | 50.. in the device status
-// word and returns.
+// scratch (states_kernel), a second turns these into the state ahead of each segment and the final one, the third
+// computes the outputs.
+//
+// What bounds it: a chunk's chain of phases (a batch of products waited for costs 540 cycles beside its 65 for an M128
+// N128 K16 product and 49 for N64, the gates' sums and exponentials 1200; 5100 in all with outputs, so 2550 an SM) and,
+// close behind, shared memory, which the operands (8 KB a product), the copies and Kd keep busy for 2300 cycles a chunk
+// with outputs and 1540 without; HBM would need 2000. Measured on a B200: 64 rows of 128 tokens 65.5 us (231 MB with the
+// states, 54% of the copy rate), two rows of 8,192 120 us (272 MB, 35%; 44 states, 8 joining, 68 outputs), one row of
+// 1,001 21 us on the device.
+//
+// Waits are bounded (%globaltimer, 2 s): on expiry the CTA records JB_DEV_TIMEOUT | 50.. in the device status word and
+// returns.
 
 namespace jb {
 namespace lintc {
