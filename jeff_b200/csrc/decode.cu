@@ -355,15 +355,18 @@ __global__ void __launch_bounds__(128, 3) prep_tokens_kernel(const PrepParams p)
 // and weight in scratch, and the CTA that leaves the last of them adds the row's parts, in share order whoever it is
 // (one launch instead of a second one of 5 to 7 us for the sums).
 //
-// In a CTA each warp takes one tile (16 or 32 tokens) of a step, with a ring of its own in shared memory (cp.async of a tile's
-// keys, then its values, tokens past the row's end as zeros) and no barrier with the other warps until a row ends, when
-// the warps' sums are joined in shared memory. Scores and output are taken transposed, S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16: the 16
-// rows of the tile are keys (then 16 of the head's dimensions), the 8 columns the query heads, so 4 query heads cost
-// half of what a 16-row query tile would. (tcgen05 has no use here: its 128-row tile would be filled with 4 rows.)
+// In a CTA each warp takes one tile (16 or 32 tokens) of a step, with a ring of its own in shared memory (cp.async of a
+// tile's keys, then its values, tokens past the row's end as zeros) and no barrier with the other warps until a row
+// ends, when the warps' sums are joined in shared memory. Scores and output are taken transposed, S^T = K Q^T and
+// O^T = V^T P^T on mma.sync m16n8k16: the 16 rows of the tile are keys (then 16 of the head's dimensions), the 8 columns
+// the query heads, so 4 query heads cost half of what a 16-row query tile would. (tcgen05 has no use here: its 128-row
+// tile would be filled with 4 rows.)
 // Measured on a B200, launch included: 64 ragged rows of 1 to 8,192 tokens (8 / 2 heads of 256, 537 MB) 116 us, 71% of
 // the copy rate; 33 rows of 100 to 4,096 (32 / 8 heads of 128, 283 MB) 68 us, 64%; one row of 1,000 12.4 us, latency.
 // Without the arithmetic the first takes 99 us and without the page lookups 92, so what is left is the streaming of half
-// tiles by eight warps an SM (7.2 TB/s when nothing else is done) and the ends of rows.
+// tiles by eight warps an SM (7.2 TB/s when nothing else is done) and the ends of rows. Steps of all heads of fewer
+// tokens, so that a page is read as one contiguous piece, took 121 and 71.
+//
 // The weights are held as two bf16 parts, p = hi + lo to 2^-17: with at most 4 query heads the lo parts ride in
 // columns 4-7, which would be empty, against the queries repeated there; with more they take a second product.
 
@@ -521,7 +524,8 @@ __device__ void dec_join(const DecParams& p, int row, int kv_head, int c0, int c
     mx = ew::warp_max(mx);
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
-      const float w = m[j] == -INFINITY && l[j] == 0.f ? 0.f : exp2f(m[j] - finite(mx));
+      // a part without keys counts nothing; one whose scores were all NaN has that as its sum, and no maximum
+      const float w = l[j] != l[j] ? l[j] : m[j] == -INFINITY ? 0.f : exp2f(m[j] - finite(mx));
       if (w != 0.f) sum += w * l[j];
       if (lane + 32 * j < SHARES) s_w[h * (SHARES + 1) + lane + 32 * j] = w;
     }
@@ -542,8 +546,8 @@ __device__ void dec_join(const DecParams& p, int row, int kv_head, int c0, int c
         x[i] = __ldcg(reinterpret_cast<const float4*>(part(min(i0 + i, count - 1))) + i4);
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
-        const float f = i0 + i < count ? w[i0 + i] : 0.f;
-        if (f == 0.f) continue;   // a part without keys may hold anything
+        if (i0 + i >= count) continue;
+        const float f = w[i0 + i];
         v[0] += f * x[i].x;
         v[1] += f * x[i].y;
         v[2] += f * x[i].z;

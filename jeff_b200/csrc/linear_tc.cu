@@ -623,10 +623,10 @@ __global__ void __launch_bounds__(THREADS, 2)
 // A segment's own contribution to the state, and its decay: S^T += V^T Kd over its chunks, Kd with the decay to the
 // segment's end (whose whole log-decay is summed first), so that the sum in tensor memory is only added to. The tensor
 // core's sums truncate: the state's error at 5 rows of 3,276 tokens was 1.3e-6 from the last chunk to the first, the
-// large terms at the bottom of the sum. Kd's first part and its two small ones go to accumulators of their own, since
-// the small parts would make the large sum truncate three times as often. Warps 0-7 form Kd, warp 8 fetches the tiles and issues the products, warp 9 forms
-// the gates a chunk ahead; two halves of a chunk in turn, one's Kd formed while the other's products run. They meet at
-// mbarriers only.
+// large terms at the bottom of the sum, and is 1.2e-7 so. Kd's first part and its two small ones go to accumulators of
+// their own, since the small parts would make the large sum truncate three times as often. Warps 0-7 form Kd, warp 8
+// fetches the tiles and issues the products, warp 9 forms the gates a chunk ahead; two halves of a chunk in turn, one's
+// Kd formed while the other's products run. They meet at mbarriers only.
 constexpr int ST_THREADS = 320;
 constexpr int ST_K = 0;                // K tile of chunk i: atoms 16384 apart at 8192 (i % 2); Kd's first part over it
 constexpr int ST_V = 32768;            // V tile: TILE (i % 2)

@@ -316,6 +316,11 @@ def plain_decode(q, dense, scale, pr=None):
     ([64] * 200, 8, 2, 256, False),           # more rows than SMs
     ([1] * 700, 14, 2, 64, True),
     ([20000], 2, 2, 128, False),
+    ([77, 0, 3000, 16], 8, 8, 128, True),     # eight key/value heads side by side
+    ([333, 48, 47], 40, 8, 64, False),
+    ([15, 700, 130], 24, 6, 256, True),
+    ([513, 90], 16, 16, 256, False),
+    ([5, 40] * 600, 2, 1, 64, False),         # more rows than a CTA holds the lengths of
 ])
 def test_decode_attention(lengths, heads, kv_heads, dim, gated) -> None:
     g = gen(sum(lengths) + heads)
@@ -370,6 +375,25 @@ def test_decode_attention_large_scores() -> None:
     got = kernels.decode_attention(q, kv, tables, 0, i32(lengths), 0)
     want, tol = plain_decode(q, dense, 1 / 16)
     close(got, want, tol)
+
+
+@pytest.mark.parametrize(("heads", "kv_heads", "dim"), [(8, 2, 256), (9, 3, 128), (16, 1, 64)])
+def test_decode_attention_passes_nan_on(heads, kv_heads, dim) -> None:
+    """A NaN in a query, a key or a value makes NaN of what the formula makes NaN of, in short rows as in cut ones, and
+    of nothing else."""
+    g = gen(12)
+    lengths = [9000, 40, 9000, 40, 9000]
+    kv, tables, dense = cache(g, lengths, 1, 0, kv_heads, dim, entry=0)
+    q = normal(g, 5, heads, dim)
+    q[0, 1, 3] = q[1, 0, 0] = math.nan
+    for r, part, j in ((2, 0, 8000), (3, 0, 39), (4, 1, 17)):
+        dense[r][part, j, kv_heads - 1, 5] = math.nan
+        kv[tables[r, j // 32], 0, part, j % 32, kv_heads - 1, 5] = math.nan
+    want, tol = plain_decode(q, dense, dim ** -0.5)
+    got = kernels.decode_attention(q, kv, tables, 0, i32(lengths), 0)
+    bad = want.isnan()
+    assert bad.any(-1).sum() == 2 + 3 * (heads // kv_heads) and torch.equal(got.isnan(), bad)
+    close(got[~bad], want[~bad], tol[~bad])
 
 
 def test_decode_attention_bad_pages_and_lengths() -> None:
