@@ -361,11 +361,13 @@ __global__ void __launch_bounds__(128, 3) prep_tokens_kernel(const PrepParams p)
 // O^T = V^T P^T on mma.sync m16n8k16: the 16 rows of the tile are keys (then 16 of the head's dimensions), the 8 columns
 // the query heads, so 4 query heads cost half of what a 16-row query tile would. (tcgen05 has no use here: its 128-row
 // tile would be filled with 4 rows.)
-// Measured on a B200, launch included: 64 ragged rows of 1 to 8,192 tokens (8 / 2 heads of 256, 537 MB) 116 us, 71% of
-// the copy rate; 33 rows of 100 to 4,096 (32 / 8 heads of 128, 283 MB) 68 us, 64%; one row of 1,000 12.4 us, latency.
-// Without the arithmetic the first takes 99 us and without the page lookups 92, so what is left is the streaming of half
-// tiles by eight warps an SM (7.2 TB/s when nothing else is done) and the ends of rows. Steps of all heads of fewer
-// tokens, so that a page is read as one contiguous piece, took 121 and 71.
+// Measured on a B200, launch included: 64 ragged rows of 1 to 8,192 tokens (8 / 2 heads of 256, 537 MB) 113 us, 73% of
+// the copy rate; 33 rows of 100 to 4,096 (32 / 8 heads of 128, 283 MB) 68 us, 64%; one row of 1,000 11.7 us, latency.
+// What bounds it is how its pages lie: a ring of copies alone, without lookups, arithmetic and ends of rows, takes 94 us
+// for 537 MB in pages of six layers of which it reads one (5.7 TB/s), 82 us where the pages hold that layer alone. The
+// rest is the start (lengths, then tables, then keys) and the ends of rows. Not kept: steps of all heads of fewer
+// tokens, so that a page is read as one contiguous piece (121 us, 71), flags of parts left and looked at without the
+// block's barriers (113, 69).
 //
 // The weights are held as two bf16 parts, p = hi + lo to 2^-17: with at most 4 query heads the lo parts ride in
 // columns 4-7, which would be empty, against the queries repeated there; with more they take a second product.

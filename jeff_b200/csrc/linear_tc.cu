@@ -27,7 +27,7 @@
 // close behind, shared memory, which the operands (8 KB a product), the copies and Kd keep busy for 2300 cycles a chunk
 // with outputs and 1540 without; HBM would need 2000. Measured on a B200: 64 rows of 128 tokens 65.5 us (231 MB with the
 // states, 54% of the copy rate), two rows of 8,192 120 us (272 MB, 35%; 44 states, 8 joining, 68 outputs), one row of
-// 1,001 21 us on the device.
+// 1,001 23 us on the device.
 //
 // Waits are bounded (%globaltimer, 2 s): on expiry the CTA records JB_DEV_TIMEOUT | 50.. in the device status word and
 // returns.
