@@ -257,7 +257,8 @@ int jb_kv_scatter(const uint16_t* kn, const uint16_t* vn, int b, int n, const in
  * What a continuation token by token needs beside the decision pass. These entry points have no counterpart in the
  * reference, which only answers prefill passes. Key/value pages are given as the pool's data, its pages and their
  * stride in bytes; an entry of a block table outside [0, pages) is taken for no page (its tokens are left out of the
- * attention, a state in it reads as zeros), and nothing is written outside the pool. */
+ * attention, a state in it reads as zeros), and nothing is written outside the pool. Outputs must not overlap inputs
+ * (but for states and tables updated in place), and calls that may run at the same time need scratches of their own. */
 
 /* Block tables and slot maps from the requests' lengths, on the device. Row r of b holds lengths[r] tokens and adds
  * added[r] (negative counts as 0). It takes the pages its new tokens need, off the free list in row order (free_pages,
@@ -287,7 +288,7 @@ int jb_attn_prep_axes(const uint16_t* pr, int64_t ldpr, int t, const float* q_w1
  * tokens is 0. dim 64, 128 or 256; heads a multiple of kv_heads, at most 16 to one. pr (nullable): y is multiplied by
  * sigmoid(pr[r, 2 dim h + dim + d]), the gate of jb_gate_mul. fp32 with one rounding to bf16. The keys of all rows
  * are cut into equal shares over the GPU and rows that were cut are joined from `scratch`
- * (at least jb_decode_attention_scratch floats, overwritten) in a fixed order. */
+ * (at least jb_decode_attention_scratch floats, 16-byte aligned, overwritten, whatever it held) in a fixed order. */
 int jb_decode_attention(const uint16_t* q, int64_t ldq, const void* kv, int64_t pages, int64_t page_bytes,
                         int attn_layer, int attn_layers, const int32_t* tables, int table_stride, int width,
                         int kv_entry, const int32_t* lengths, int b, int heads, int kv_heads, int dim, float scale,

@@ -361,13 +361,14 @@ __global__ void __launch_bounds__(128, 3) prep_tokens_kernel(const PrepParams p)
 // O^T = V^T P^T on mma.sync m16n8k16: the 16 rows of the tile are keys (then 16 of the head's dimensions), the 8 columns
 // the query heads, so 4 query heads cost half of what a 16-row query tile would. (tcgen05 has no use here: its 128-row
 // tile would be filled with 4 rows.)
-// Measured on a B200, launch included: 64 ragged rows of 1 to 8,192 tokens (8 / 2 heads of 256, 537 MB) 113 us, 73% of
-// the copy rate; 33 rows of 100 to 4,096 (32 / 8 heads of 128, 283 MB) 68 us, 64%; one row of 1,000 11.7 us, latency.
+// Measured on a B200, launch included: 64 ragged rows of 1 to 8,192 tokens (8 / 2 heads of 256, 537 MB) 105 us, 78% of
+// the copy rate; 33 rows of 100 to 4,096 (32 / 8 heads of 128, 283 MB) 61 us, 71%; one row of 1,000 10.2 us, latency.
 // What bounds it is how its pages lie: a ring of copies alone, without lookups, arithmetic and ends of rows, takes 94 us
 // for 537 MB in pages of six layers of which it reads one (5.7 TB/s), 82 us where the pages hold that layer alone. The
-// rest is the start (lengths, then tables, then keys) and the ends of rows. Not kept: steps of all heads of fewer
-// tokens, so that a page is read as one contiguous piece (121 us, 71), flags of parts left and looked at without the
-// block's barriers (113, 69).
+// rest is the start (lengths, then tables, then keys), the ends of rows (1 us each; 3.3 with a thread a value) and SMs
+// that stream slower than others. Not kept: steps of all heads of fewer tokens, so that a page is read as one contiguous
+// piece (3% slower), two CTAs of four warps an SM (6%), shares in three waves (18%) or claimed by the CTAs that are done
+// with theirs (21%: every share ends a row, and its start waits for lengths and tables again).
 //
 // The weights are held as two bf16 parts, p = hi + lo to 2^-17: with at most 4 query heads the lo parts ride in
 // columns 4-7, which would be empty, against the queries repeated there; with more they take a second product.
@@ -576,7 +577,7 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
   constexpr int KS = D / 16, CH = D / 8;   // 16-wide k steps, 16-byte chunks of a key
   constexpr int TILE = L::TILE, MT = TILE / 16, CHAINS = 4 / MT;
   extern __shared__ __align__(16) uint8_t sm[];
-  __shared__ float s_m[L::WARPS][16], s_l[L::WARPS][16];
+  __shared__ float s_m[L::WARPS][16], s_l[L::WARPS][16], s_f[16][L::WARPS], s_all[16][2];
   __shared__ float s_w[WEIGHTS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, tq = lane & 3;
   // the rows' lengths are asked for again and again: from shared memory where they fit there
@@ -812,27 +813,52 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
       __syncthreads();
       const bool whole = first_step == 0 && c.step + 1 == c.steps;
       float* part = p.parts + (2 * (int64_t)blockIdx.x + (from_start ? 0 : 1)) * dec_part(p.group, D);
-      for (int i = threadIdx.x; i < p.group * D; i += L::WARPS * 32) {
-        const int h = i / D, d = i % D;
-        float mx = -INFINITY;
+      // each head's factors, maximum and sum over the warps: eight lanes a head
+      if (threadIdx.x < 8 * NT * L::WARPS) {
+        const int w = threadIdx.x % L::WARPS, h = threadIdx.x / L::WARPS;
+        const float mw = s_m[w][h];
+        float mx = mw;
 #pragma unroll
-        for (int w = 0; w < L::WARPS; ++w) mx = fmaxf(mx, s_m[w][h]);
-        float sum = 0.f, v = 0.f;
+        for (int off = 1; off < L::WARPS; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        const float f = mw == -INFINITY ? 0.f : exp2f(mw - mx);   // 0: a warp without keys of this row
+        float sum = f * s_l[w][h];
+#pragma unroll
+        for (int off = 1; off < L::WARPS; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        s_f[h][w] = f;
+        if (w == 0) {
+          s_all[h][0] = mx;
+          s_all[h][1] = sum;
+        }
+      }
+      __syncthreads();
+      for (int i4 = threadIdx.x; i4 < p.group * D / 4; i4 += L::WARPS * 32) {
+        const int h = i4 * 4 / D, d = i4 * 4 % D, head = c.head * p.group + h;
+        uint2 gate = make_uint2(0, 0);
+        if (whole && p.pr) gate = *reinterpret_cast<const uint2*>(p.pr + c.row * p.ldpr + ((int64_t)2 * head + 1) * D + d);
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < L::WARPS; ++w) {
-          if (s_m[w][h] == -INFINITY && s_l[w][h] == 0.f) continue;   // a warp without keys of this row
-          const float a = exp2f(s_m[w][h] - finite(mx));
-          sum += a * s_l[w][h];
-          v += a * reinterpret_cast<const float*>(sm + (w * L::HALVES + (h < 8 ? vslot : slot)) * L::SLOT)[
-                       (h & 7) * D + (d ^ ((h >> 1 & 3) * 8))];
+          const float f = s_f[h][w];
+          const float4 x = *reinterpret_cast<const float4*>(
+              sm + (w * L::HALVES + (h < 8 ? vslot : slot)) * L::SLOT +
+              ((h & 7) * D + (d ^ ((h >> 1 & 3) * 8))) * 4);
+          v[0] += f * x.x;
+          v[1] += f * x.y;
+          v[2] += f * x.z;
+          v[3] += f * x.w;
         }
+        const float mx = s_all[h][0], sum = s_all[h][1];
         if (whole) {
-          const int head = c.head * p.group + h;
-          v = mx == -INFINITY && sum == 0.f ? 0.f : v / sum;
-          if (p.pr) v *= ew::sigmoid(bf2f(p.pr[c.row * p.ldpr + ((int64_t)2 * head + 1) * D + d]));
-          p.y[c.row * p.ldy + (int64_t)head * D + d] = f2bf(v);
+          const float g[4] = {bf_lo(gate.x), bf_hi(gate.x), bf_lo(gate.y), bf_hi(gate.y)};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = sum == 0.f ? 0.f : v[e] / sum;   // no keys: zeros
+            if (p.pr) v[e] *= ew::sigmoid(g[e]);
+          }
+          *reinterpret_cast<uint2*>(p.y + c.row * p.ldy + (int64_t)head * D + d) =
+              make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
         } else {
-          part[i] = v;
+          reinterpret_cast<float4*>(part)[i4] = make_float4(v[0], v[1], v[2], v[3]);
           if (d == 0) {
             part[p.group * D + h] = mx;
             part[p.group * (D + 1) + h] = sum;

@@ -321,6 +321,9 @@ def plain_decode(q, dense, scale, pr=None):
     ([15, 700, 130], 24, 6, 256, True),
     ([513, 90], 16, 16, 256, False),
     ([5, 40] * 600, 2, 1, 64, False),         # more rows than a CTA holds the lengths of
+    ([5000, 7, 9000, 6000, 0, 12000, 6700], 8, 8, 64, True),   # many steps a share
+    ([20000, 30000, 1, 27001], 8, 2, 256, True),
+    ([3000, 2000] * 20, 32, 4, 128, False),
 ])
 def test_decode_attention(lengths, heads, kv_heads, dim, gated) -> None:
     g = gen(sum(lengths) + heads)
