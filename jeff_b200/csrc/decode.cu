@@ -865,35 +865,34 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
           }
         }
       }
-      if (!whole) {
-        // the row's units a .. z and their shares c0 .. c1 (unit u's: the last c with total * c / shares <= u)
-        const long long a = u - c.step, z = a + c.steps - 1;
-        const int c0 = (int)(((a + 1) * shares - 1) / total), c1 = (int)(((z + 1) * shares - 1) / total);
-        const int count = c1 - c0 + 1;
-        const bool first = total * c0 / shares == a;
-        auto slot_of = [&](int i) { return 2 * (c0 + i) + (i == 0 && !first ? 1 : 0); };
-        // the part, then its flag, then the others' flags: of the CTAs whose fences come in this order, the last sees
-        // all of them (a second one may, and then joins the same parts to the same values)
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-          p.flags[slot_of(blockIdx.x - c0)] = p.tag;
-          __threadfence();
-        }
-        __syncthreads();
-        bool there = true;
-        for (int i = threadIdx.x; i < count; i += L::WARPS * 32) there &= p.flags[slot_of(i)] == p.tag;
-        if (__syncthreads_and(there)) {
-          __threadfence();
-          dec_join<D>(p, c.row, c.head, c0, count, first, s_w);
-          __syncthreads();
-          for (int i = threadIdx.x; i < count; i += L::WARPS * 32) p.flags[slot_of(i)] = 0;
-        }
-      }
-      __syncthreads();
+      __syncthreads();   // the slots are free again, the part is written
     }
     if (ends) fetch();
     fetch();
+    if (ends && !(first_step == 0 && c.step + 1 == c.steps)) {
+      // a part of a row whose units are a .. z and whose shares c0 .. c1 (unit u's: the last c with total * c / shares <=
+      // u): its flag, then the others' flags: of the CTAs whose fences come in this order, the last sees all of them (a
+      // second one may, and then joins the same parts to the same values)
+      const long long a = u - c.step, z = a + c.steps - 1;
+      const int c0 = (int)(((a + 1) * shares - 1) / total), c1 = (int)(((z + 1) * shares - 1) / total);
+      const int count = c1 - c0 + 1;
+      const bool first = total * c0 / shares == a;
+      auto slot_of = [&](int i) { return 2 * (c0 + i) + (i == 0 && !first ? 1 : 0); };
+      if (threadIdx.x == 0) {
+        __threadfence();
+        p.flags[slot_of(blockIdx.x - c0)] = p.tag;
+        __threadfence();
+      }
+      __syncthreads();
+      bool there = true;
+      for (int i = threadIdx.x; i < count; i += L::WARPS * 32) there &= p.flags[slot_of(i)] == p.tag;
+      if (__syncthreads_and(there)) {
+        __threadfence();
+        dec_join<D>(p, c.row, c.head, c0, count, first, s_w);
+        __syncthreads();
+        for (int i = threadIdx.x; i < count; i += L::WARPS * 32) p.flags[slot_of(i)] = 0;
+      }
+    }
     slot = vslot + 1 == L::HALVES ? 0 : vslot + 1;
     if (u + 1 < u1) {
       dec_next<L::STEP>(p, length, c);
