@@ -175,7 +175,8 @@ __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* map) {
 //
 // Every kernel of the library starts with pdl_begin(): it waits until the grids it depends on have completed and
 // their memory is visible (a no-op for a launch without the attribute), then lets the stream's next launch start its
-// own launch and CTA dispatch while this grid runs. Nothing of a kernel touches global memory before that wait, so
+// own launch and CTA dispatch while this grid runs. Nothing of a kernel touches global memory before that wait (but the
+// later launches of linear_tc.cu, for what was there before the first of them; their comments say why they may), so
 // launching with the attribute (launch_pdl) overlaps only launch latency, dispatch and the previous grid's tail with
 // the next grid's start; the order of every memory access is what a plain launch gives.
 __device__ __forceinline__ void pdl_begin() {

@@ -25,9 +25,9 @@
 // What bounds it: a chunk's chain of phases (a batch of products waited for costs 540 cycles beside its 65 for an M128
 // N128 K16 product and 49 for N64, the gates' sums and exponentials 1200; 5100 in all with outputs, so 2550 an SM) and,
 // close behind, shared memory, which the operands (8 KB a product), the copies and Kd keep busy for 2300 cycles a chunk
-// with outputs and 1540 without; HBM would need 2000. Measured on a B200: 64 rows of 128 tokens 65.5 us (231 MB with the
-// states, 54% of the copy rate), two rows of 8,192 120 us (272 MB, 35%; 44 states, 8 joining, 68 outputs), one row of
-// 1,001 23 us on the device.
+// with outputs and 1540 without; two CTAs an SM take 8600 each. HBM would need 2000. Measured on a B200: 64 rows of 128 tokens 65.5 us (231 MB with the
+// states, 54% of the copy rate), two rows of 8,192 108 us on the device (272 MB, 38%; 42 states, 8 joining, 66
+// outputs), one row of 1,001 22 us (23 where the second and third launch read nothing ahead of their waits).
 //
 // Waits are bounded (%globaltimer, 2 s): on expiry the CTA records JB_DEV_TIMEOUT | 50.. in the device status word and
 // returns.
@@ -227,7 +227,9 @@ __global__ void __launch_bounds__(THREADS, 2)
     scan_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o, const Args a,
                 const Seg seg, int* err) {
-  pdl_begin();
+  // The outputs' launch is let go by join_kernel's CTAs once they have seen the states' launch end, and that one began
+  // when everything before it had ended: the inputs are there. Only the segments' states are waited for.
+  if (MODE == WHOLE) pdl_begin();
   constexpr int PARTS = MODE == OUTPUTS ? 2 : 3;   // of Kd
   extern __shared__ __align__(1024) uint8_t sm[];
   uint8_t* kq = sm + OFF_KQ;
@@ -305,22 +307,22 @@ __global__ void __launch_bounds__(THREADS, 2)
   const float* in = MODE == WHOLE ? lin::state_in(a.pool, row, h)
                                   : seg.states + ((int64_t)pair * seg.count + part) * STATE;
   float* state = reinterpret_cast<float*>(sm + OFF_K0);
-  if (warp == 0) {
+  if (warp == 0 && chunks) {
     const bool me = elect_one();
-    if (in && me) {
-      mbar_arrive_expect_tx(s_bar, STATE * 4);
-      bulk_load(state, in, STATE * 4, s_bar);
-    }
-    if (chunks) {
-      load_k(0, me);
-      load_q(0, me);
-    }
+    load_k(0, me);
+    load_q(0, me);
     __syncwarp();
+  }
+  if (MODE == OUTPUTS && warp == 2) pdl_begin();
+  if (warp == 2 && in && elect_one()) {
+    mbar_arrive_expect_tx(s_bar, STATE * 4);
+    bulk_load(state, in, STATE * 4, s_bar);
   }
   if (qd == 0) {
     form_gates<false>(gates[0], ch, g0, g1, lane, whole, unused);
     gates_of(1);
   }
+  if (MODE == OUTPUTS && warp != 2) pdl_begin();
   __syncthreads();
   // lane = value column, columns = key rows: into tensor memory, scaled for the first chunk, and its bf16 copy
   auto put_state = [&](int half, uint32_t (&x)[32], float el) {
@@ -862,11 +864,12 @@ __global__ void __launch_bounds__(ST_THREADS, 2)
 // The segments' contributions of a (row, head) -> the state ahead of each, in place, and the final state. Thread = four
 // neighbouring values of the state.
 __global__ void __launch_bounds__(256) join_kernel(const Args a, const Seg seg) {
-  pdl_begin();
   const int pair = blockIdx.x, row = pair / a.heads, h = pair % a.heads;
   const int i = blockIdx.y * 256 + threadIdx.x;
   const float* in = lin::state_in(a.pool, row, h);
+  // (written before the states' launch began, and that has let this one go)
   float4 s = in ? reinterpret_cast<const float4*>(in)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+  pdl_begin();
   float4* parts = reinterpret_cast<float4*>(seg.states + (int64_t)pair * seg.count * STATE) + i;
   const float* decay = seg.decay + (int64_t)pair * seg.count;
   constexpr int AHEAD = 8;   // segments read before the first of them is overwritten
@@ -900,7 +903,7 @@ int tile_map(CUtensorMap* map, const void* base, const Args& a, int b, int64_t t
 // Segments of a (row, head). Measured on a B200, in us: one segment takes 4 + 3.5 a chunk; segments of `per` chunks, all
 // of them at once, 9 + 4.7 per + 0.045 for each segment of the call, whose states are written, joined, and read again.
 // So 8 rows of 256 tokens stay whole (20.8 us, 30.5 in two segments a head), one row of 1,001 takes segments of two
-// chunks (21.2; 24.8 of one, 66 whole), one of 8,192 as many as run at once.
+// chunks (21.7; 66 whole), one of 8,192 as many as run at once.
 inline Seg segments(int b, int heads, int n) {
   const int chunks = (n + C - 1) / C;
   const int64_t pairs = (int64_t)b * heads;
