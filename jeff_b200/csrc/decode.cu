@@ -367,8 +367,8 @@ __global__ void __launch_bounds__(128, 3) prep_tokens_kernel(const PrepParams p)
 // for 537 MB in pages of six layers of which it reads one (5.7 TB/s), 82 us where the pages hold that layer alone. The
 // rest is the start (lengths, then tables, then keys), the ends of rows (1 us each; 3.3 with a thread a value) and SMs
 // that stream slower than others. Not kept: steps of all heads of fewer tokens, so that a page is read as one contiguous
-// piece (3% slower), two CTAs of four warps an SM (6%), shares in three waves (18%) or claimed by the CTAs that are done
-// with theirs (21%: every share ends a row, and its start waits for lengths and tables again).
+// piece (2% slower), two CTAs of four warps an SM (7%), shares in three waves (13%) or claimed by the CTAs that are done
+// with theirs (21%): every share ends a row, and in waves its start waits for lengths and tables again.
 //
 // The weights are held as two bf16 parts, p = hi + lo to 2^-17: with at most 4 query heads the lo parts ride in
 // columns 4-7, which would be empty, against the queries repeated there; with more they take a second product.

@@ -25,9 +25,11 @@
 // What bounds it: a chunk's chain of phases (a batch of products waited for costs 540 cycles beside its 65 for an M128
 // N128 K16 product and 49 for N64, the gates' sums and exponentials 1200; 5100 in all with outputs, so 2550 an SM) and,
 // close behind, shared memory, which the operands (8 KB a product), the copies and Kd keep busy for 2300 cycles a chunk
-// with outputs and 1540 without; two CTAs an SM take 8600 each. HBM would need 2000. Measured on a B200: 64 rows of 128 tokens 65.5 us (231 MB with the
-// states, 54% of the copy rate), two rows of 8,192 108 us on the device (272 MB, 38%; 42 states, 8 joining, 66
-// outputs), one row of 1,001 22 us (23 where the second and third launch read nothing ahead of their waits).
+// with outputs and 1540 without; two CTAs an SM take 8600 each. HBM would need 2000. Measured on a B200: 64 rows of 128
+// tokens 65 us (231 MB with the states, 54% of the copy rate), two rows of 8,192 108 us (272 MB, 38%; 42 the states, 8
+// the join, 66 the outputs, whose starts overlap), one row of 1,001 22 us (23 where the second and third launch read
+// nothing ahead of their waits). Not kept: MMA2 into D as soon as the outputs have left it, P formed under MMA1 (a chunk
+// shorter by the state's update on paper, 6% slower: Q and K are then needed sooner than they come).
 //
 // Waits are bounded (%globaltimer, 2 s): on expiry the CTA records JB_DEV_TIMEOUT | 50.. in the device status word and
 // returns.
