@@ -797,3 +797,60 @@ def test_on_a_stream_of_its_own() -> None:
             got.append(kernels.decode_attention(q, kv, tables, 0, n, 0))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_operators_at_once_on_three_streams() -> None:
+    """Scans in segments and whole, steps and decode attention at once give what each gives alone."""
+    g = gen(22)
+    long, short = linear_case(1, 1, 1001, 16, 6, 0, "tokens"), linear_case(2, 40, 128, 16, 6, 0, "tokens")
+    lengths = [5000, 1, 3000, 64]
+    kv, tables, _ = cache(g, lengths, 2, 1, 2, 256, entry=0)
+    q, n = normal(g, 4, 8, 256), i32(lengths)
+
+    def scan(case):
+        q, k, v, decay, state, ids, out_ids, _ = case
+        return kernels.linear_scan(q, k, v, decay, state, ids, 0, out_tables=out_ids)
+
+    work = [lambda: scan(long), lambda: scan(short), lambda: kernels.decode_attention(q, kv, tables, 1, n, 0)]
+    want = [f() for f in work]
+    torch.cuda.synchronize()
+    finals = [case[4].clone() for case in (long, short)]
+    streams = [torch.cuda.Stream() for _ in work]
+    got = []
+    for _ in range(10):
+        for f, stream in zip(work, streams):
+            with torch.cuda.stream(stream):
+                got.append(f())
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert torch.equal(x, want[i % 3])
+    assert all(torch.equal(a, b[4]) for a, b in zip(finals, (long, short)))
+
+
+def test_scans_in_a_row_in_place() -> None:
+    """Scans that each go on from the state that the one before left in the same pages, launched without a wait in
+    between and replayed as a graph, give what they give one at a time."""
+    q, k, v, decay, state, ids, _, _ = linear_case(3, 1, 1001, 16, 6, 1, "tokens")
+    start = state.clone()
+    cut = [300, 1001, 700]
+
+    def run(wait: bool) -> list[torch.Tensor]:
+        state.copy_(start)
+        outs = []
+        for n in cut:
+            outs.append(kernels.linear_scan(q[:, :n], k[:, :n], v[:, :n], decay[:, :n], state, ids, 1, out_tables=ids))
+            outs.append(kernels.linear_step(q[:, n - 1], k[:, n - 1], v[:, n - 1], decay[:, n - 1], state, ids, 1))
+            if wait:
+                torch.cuda.synchronize()
+        return outs + [state.clone()]
+
+    want = run(True)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(run(False), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(False)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
