@@ -440,8 +440,7 @@ def block_tables(lengths: torch.Tensor, new: torch.Tensor, free: torch.Tensor, t
     _rows_of(free, "free", torch.int32, tuple(free.shape), 1, dev)
     _tables_of(tables, "tables", b, kv_entry + 1, dev)
     if out is None:
-        parts = torch.empty(4 * tokens + 2 * (b + 1), dtype=torch.int32, device=dev).split(
-            (2 * tokens, tokens, tokens, b + 1, b + 1))
+        parts = lengths.new_empty(4 * tokens + 2 * (b + 1)).split((2 * tokens, tokens, tokens, b + 1, b + 1))
         out = SlotMap(parts[0].view(torch.int64), *parts[1:])
     else:
         for name, dtype, size in (("slots", torch.int64, tokens), ("rows", torch.int32, tokens),
@@ -506,7 +505,7 @@ def attn_prep_axes(pr: torch.Tensor, q_w1: torch.Tensor, k_w1: torch.Tensor, inv
     if kv is not None and _cache_of(kv, attn_layer, dev)[4:] != (C.NKV, C.HD):
         raise ValueError(f"kv: expected pages of {C.NKV} heads of {C.HD}, got {tuple(kv.shape)}")
     if out is None:
-        out = torch.empty(t, C.NQ, C.HD, dtype=DT, device=dev)
+        out = pr.new_empty((t, C.NQ, C.HD))
     else:
         _rows_of(out, "out", DT, (t, C.NQ, C.HD), 3, dev)
     pages = (None, 0, 0, attn_layer, 0) if kv is None else (kv.data_ptr(), kv.shape[0], 2 * kv.stride(0), attn_layer,
@@ -549,11 +548,11 @@ def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, at
         _rows_of(pr, "pr", DT, (b, pr.shape[1]), 1, dev)
         shape = (b, heads * dim)
     if out is None:
-        out = torch.empty(shape, dtype=DT, device=dev)
+        out = q.new_empty(shape)
     else:
         _rows_of(out, "out", DT, shape, len(shape) - 1, dev)
     if scratch is None:
-        scratch = torch.empty(_decode_scratch(heads, kv_heads, dim), dtype=torch.float32, device=dev)
+        scratch = q.new_empty(_decode_scratch(heads, kv_heads, dim), dtype=torch.float32)
     else:
         _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), dev)
     _on(dev, "jb_decode_attention", q.data_ptr(), q.stride(0), kv.data_ptr(), pages, 2 * kv.stride(0), attn_layer,
@@ -626,7 +625,7 @@ def linear_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
         _rows_of(real, "real", torch.int32, (b,), 1, q.device)
     need = _scan_scratch(b, heads, n)
     if scratch is None:
-        scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
+        scratch = q.new_empty(need, dtype=torch.float32) if need else None
     else:
         _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), q.device)
     steps = (0, 0) if g.dim() == 1 else g.stride()[:2]
