@@ -118,7 +118,8 @@ __global__ void __launch_bounds__(TAB_THREADS) tables_kernel(const TabParams p) 
     }
     __syncthreads();
     // this CTA's tokens that belong to these rows: the row by bisection of the sums
-    const int lo = (int)max((long long)t0, base_add), hi = (int)min((long long)t1, ta);
+    // (the sums may pass 32 bits, and are cut to the share ahead of that)
+    const int lo = (int)min(max((long long)t0, base_add), (long long)t1), hi = (int)min((long long)t1, ta);
     for (int t = lo + tid; t < hi; t += TAB_THREADS) {
       int l = 0, h = count - 1;   // the last row whose tokens start at or before t; rows that add none share a start
       while (l < h) {

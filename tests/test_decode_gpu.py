@@ -130,6 +130,45 @@ def test_block_tables_give_the_pools_own_order() -> None:
     assert int(got.taken[-1]) == 400 - 2 - pool.free_page_count()
 
 
+@pytest.mark.parametrize("giants", [1, 2])
+def test_block_tables_counts_past_the_type(giants) -> None:
+    """More rows than one round of the sums holds, and counts whose sum passes 31 and 32 bits in the first round: the
+    tokens that fit are listed as ever, and nothing is written around them."""
+    b, tokens, top = 1500, 2000, 2 ** 31 - 1
+    new = [1] * b
+    new[10:10 + giants] = [top] * giants
+    wide = torch.full((5, tokens + 4096), -9, dtype=torch.int64, device="cuda")
+
+    def inside(i: int, size: int, dtype: torch.dtype) -> torch.Tensor:
+        return wide[i].view(dtype)[2048:2048 + size]
+
+    out = kernels.SlotMap(inside(0, tokens, torch.int64), *(inside(1 + i, size, torch.int32) for i, size in
+                                                            enumerate((tokens, tokens, b + 1, b + 1))))
+    tables = torch.zeros(b, 4, dtype=torch.int32, device="cuda")
+    guard = wide.clone()
+    free = [3 + i for i in range(4 * b)]
+    kernels.block_tables(i32([0] * b), i32(new), i32(free), tables, 0, tokens, out=out)
+    assert sum(new[:1024]) in (2 ** 31 + 1022, 2 ** 32 + 1020)
+    take = [min(-(-n // 32), 4) for n in new]
+    want_tables, at = [], 0
+    for n in take:
+        want_tables.append(free[at:at + n] + [0] * (4 - n))
+        at += n
+    assert tables.tolist() == want_tables
+    where = [(r, 0) for r in range(10)] + [(10, p) for p in range(tokens - 10)]
+    assert out.rows.tolist() == [r for r, _ in where] and out.positions.tolist() == [p for _, p in where]
+    assert out.slots.tolist() == [want_tables[r][p // 32] * 32 + p % 32 if p < 128 else -1 for r, p in where]
+    sums = [0]
+    for n in new:
+        sums.append(sums[-1] + n)
+    assert out.starts.tolist() == [min(s, top) for s in sums]
+    assert out.taken.tolist() == [sum(take[:r]) for r in range(b + 1)]
+    for i, (size, dtype) in enumerate(((tokens, torch.int64), (tokens, torch.int32), (tokens, torch.int32),
+                                       (b + 1, torch.int32), (b + 1, torch.int32))):
+        guard[i].view(dtype)[2048:2048 + size] = wide[i].view(dtype)[2048:2048 + size]
+    assert torch.equal(wide, guard)
+
+
 # ---------------------------------------------------------------- attention input side
 
 
