@@ -268,7 +268,8 @@ int jb_kv_scatter(const uint16_t* kn, const uint16_t* vn, int b, int n, const in
  * slots[t] = page * page_tokens + place in the page, rows[t] and positions[t]; -1, -1 and 0 past the last one. starts
  * (b + 1) is each row's first token, taken (b + 1) the pages that the rows before it take. taken[b] > free_count: the
  * list was too short; the entries past it are 0 (the sink) and their tokens' slots -1. A token past the table's last
- * entry (width) takes no page and has slot -1; tokens past `tokens` are not listed. */
+ * entry (width) takes no page and has slot -1; tokens past `tokens` are not listed. b and
+ * tokens: at most 0x7f000000. */
 int jb_block_tables(const int32_t* lengths, const int32_t* added, int b, const int32_t* free_pages, int free_count,
                     int32_t* tables, int table_stride, int width, int kv_entry, int page_tokens, int fixed, int tokens,
                     int64_t* slots, int32_t* rows, int32_t* positions, int32_t* starts, int32_t* taken, void* stream);

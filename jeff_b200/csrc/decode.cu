@@ -934,7 +934,8 @@ extern "C" int jb_block_tables(const int32_t* lengths, const int32_t* added, int
   using namespace jb;
   JB_REQUIRE(lengths && added && tables && slots && rows && positions && starts && taken,
              "jb_block_tables: null pointer");
-  JB_REQUIRE(b > 0 && tokens > 0, "jb_block_tables: %d rows, %d tokens", b, tokens);
+  // (the kernel's indices step past the last row and token by a round of rows, a block's threads, a CTA's share)
+  JB_REQUIRE(b > 0 && b <= 0x7f000000 && tokens > 0 && tokens <= 0x7f000000, "jb_block_tables: %d rows, %d tokens", b, tokens);
   JB_REQUIRE(free_count >= 0 && (free_pages || free_count == 0), "jb_block_tables: a free list of %d pages", free_count);
   JB_REQUIRE(kv_entry >= 0 && kv_entry < width && width <= table_stride && page_tokens > 0,
              "jb_block_tables: key/value entry %d of tables %d wide (stride %d), pages of %d tokens", kv_entry, width,

@@ -104,6 +104,14 @@ def test_bad_arguments_are_refused_before_any_launch(lib, call, over, says) -> N
     assert says in lib.jb_last_error()
 
 
+def test_block_tables_refuses_more_than_its_indices_hold(lib) -> None:
+    for count in (2 ** 31 - 1, 0x7f000001):
+        assert _tables(lib, tokens=count) == -1
+        assert b"%d tokens" % count in lib.jb_last_error()
+        assert _tables(lib, b=count) == -1
+        assert b"%d rows" % count in lib.jb_last_error()
+
+
 def test_scratch_sizes(lib) -> None:
     """Two cut rows' flags and parts a share; a state and its decay for each of a long row's segments, which all run at once, and
     none for rows that stay whole."""
