@@ -286,7 +286,8 @@ int jb_attn_prep_axes(const uint16_t* pr, int64_t ldpr, int t, const float* q_w1
 
 /* Attention of one new token per row over its cached keys: y (b, heads, dim) = softmax(scale q . k_j) v_j over the
  * tokens j < lengths[r] of pages tables[r][kv_entry + j / 32] (at most what the table's width holds); a row without
- * tokens is 0. dim 64, 128 or 256; heads a multiple of kv_heads, at most 16 to one. pr (nullable): y is multiplied by
+ * tokens is 0. dim 64, 128 or 256; heads a multiple of kv_heads, at most 16 to one; heads * dim at
+ * most 2^24, tables of at most 0x7f000000 tokens and 2^38 / kv_heads. pr (nullable): y is multiplied by
  * sigmoid(pr[r, 2 dim h + dim + d]), the gate of jb_gate_mul. fp32 with one rounding to bf16. The keys of all rows
  * are cut into equal shares over the GPU and rows that were cut are joined from `scratch`
  * (at least jb_decode_attention_scratch floats, 16-byte aligned, overwritten, whatever it held) in a fixed order. */

@@ -996,6 +996,12 @@ extern "C" int jb_decode_attention(const uint16_t* q, int64_t ldq, const void* k
              (long long)page_bytes);
   JB_REQUIRE(kv_entry >= 0 && kv_entry <= width && width <= table_stride,
              "jb_decode_attention: key/value entry %d of tables %d wide (stride %d)", kv_entry, width, table_stride);
+  // the kernel counts a row's tokens, its steps of 128 over all heads, and a page's values in 32 bits
+  const int64_t most = (int64_t)(width - kv_entry) * dec::PAGE;
+  JB_REQUIRE(most <= 0x7f000000 && (most + 127) / 128 * kv_heads <= 0x7fffffff,
+             "jb_decode_attention: tables of %lld tokens, %d key/value heads", (long long)most, kv_heads);
+  JB_REQUIRE((int64_t)heads * dim <= 1 << 24 && b <= 0x7f000000, "jb_decode_attention: %d rows of %d heads of %d", b,
+             heads, dim);
   JB_REQUIRE(ldq >= heads * dim && ldq % 8 == 0 && ldy >= heads * dim && ldy % 8 == 0 &&
                  (!pr || (ldpr >= 2 * heads * dim && ldpr % 8 == 0)),
              "jb_decode_attention: row strides %lld, %lld, %lld", (long long)ldq, (long long)ldy, (long long)ldpr);
@@ -1006,7 +1012,6 @@ extern "C" int jb_decode_attention(const uint16_t* q, int64_t ldq, const void* k
   JB_REQUIRE(scratch && scratch_floats >= dec::dec_scratch(group, dim) && dec::aligned16(scratch),
              "jb_decode_attention: a scratch of %lld floats (16-byte aligned), %lld are needed",
              (long long)scratch_floats, (long long)dec::dec_scratch(group, dim));
-  const int64_t most = min((int64_t)(width - kv_entry) * dec::PAGE, (int64_t)0x7fffffc0);
   const dec::DecParams p = {reinterpret_cast<const __nv_bfloat16*>(q), ldq,
                             static_cast<const uint8_t*>(kv) + attn_layer * layer_bytes, pages, page_bytes, tables,
                             table_stride, kv_entry, (int)most, lengths, b, kv_heads, group, dim,

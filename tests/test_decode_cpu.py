@@ -112,6 +112,19 @@ def test_block_tables_refuses_more_than_its_indices_hold(lib) -> None:
         assert b"%d rows" % count in lib.jb_last_error()
 
 
+@pytest.mark.parametrize(("over", "says"), [
+    ({"width": 2 ** 26, "stride": 2 ** 26, "entry": 0}, b"tables of 2147483648 tokens"),
+    ({"width": 0x3f80002, "stride": 0x3f80002, "entry": 1}, b"tables of 2130706464 tokens"),
+    ({"width": 0x3f80000, "stride": 0x3f80000, "entry": 0, "heads": 512, "kv_heads": 256, "dim": 64,
+      "page_bytes": 2 ** 24, "ldq": 2 ** 15, "ldy": 2 ** 15}, b"256 key/value heads"),
+    ({"heads": 2 ** 23, "kv_heads": 2 ** 20, "page_bytes": 2 ** 50}, b"2 rows of 8388608 heads of 256"),
+    ({"b": 0x7f000001, "heads": 1, "kv_heads": 1}, b"2130706433 rows"),
+])
+def test_decode_attention_refuses_more_than_its_indices_hold(lib, over, says) -> None:
+    assert _decode(lib, **over) == -1
+    assert says in lib.jb_last_error()
+
+
 def test_scratch_sizes(lib) -> None:
     """Two cut rows' flags and parts a share; a state and its decay for each of a long row's segments, which all run at once, and
     none for rows that stay whole."""
