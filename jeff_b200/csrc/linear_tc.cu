@@ -581,9 +581,9 @@ __global__ void __launch_bounds__(THREADS, 2)
   const bool ok = *abort_flag == 0;
   {   // chunks that hold padding only
     const int first = max(begin, (work + C - 1) / C * C);
-    for (int i = first * 16 + tid; i < end * 16; i += THREADS)
-      reinterpret_cast<uint4*>(a.o + row * a.o_row + (int64_t)(i >> 4) * a.o_tok + h * D)[i & 15] =
-          make_uint4(0, 0, 0, 0);
+    uint4* o = reinterpret_cast<uint4*>(a.o + row * a.o_row + h * D);
+    for (int64_t i = (int64_t)first * 16 + tid; i < (int64_t)end * 16; i += THREADS)
+      o[(i >> 4) * (a.o_tok / 8) + (i & 15)] = make_uint4(0, 0, 0, 0);
   }
   float* out = MODE == WHOLE ? lin::state_out(a.pool, row, h) : nullptr;
   if (ok && out) {   // through shared memory, Kd's and V's places again, as one copy

@@ -720,6 +720,21 @@ def test_linear_refusals() -> None:
         kernels.linear_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], state, tables, 0, beta=g[:, 0])
 
 
+def test_linear_scan_padding_past_32_bits() -> None:
+    """A row so long that its padding's 16-byte pieces pass 31 bits: zeros out past its end, and nothing around them."""
+    n, real = 2 ** 27 + 4096, 2 ** 27 + 1000
+    x = torch.zeros(1, n, 1, 128, dtype=torch.bfloat16, device="cuda")
+    out = torch.ones(n + 128, 1, 128, dtype=torch.bfloat16, device="cuda")
+    state = torch.full((4, 1, 128, 128), 2.0, device="cuda")
+    kernels.linear_scan(x, x, x, torch.zeros(1, device="cuda"), state, i32([[2]]), 0, real=i32([real]),
+                        out_tables=i32([[3]]), out=out[64:64 + n][None])
+    assert bool((out[:64] == 1).all()) and bool((out[64 + n:] == 1).all())
+    assert not out[64 + real - 3000:64 + n].any() and not out[64:10064].any()
+    assert torch.equal(state[3], state[2])
+    del x, out
+    torch.cuda.empty_cache()   # 69 GB
+
+
 # ---------------------------------------------------------------- together
 
 
