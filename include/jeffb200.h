@@ -256,8 +256,9 @@ int jb_kv_scatter(const uint16_t* kn, const uint16_t* vn, int b, int n, const in
  *
  * What a continuation token by token needs beside the decision pass. These entry points have no counterpart in the
  * reference, which only answers prefill passes. Key/value pages are given as the pool's data, its pages and their
- * stride in bytes; an entry of a block table outside [0, pages) is taken for no page (its tokens are left out of the
- * attention, a state in it reads as zeros), and nothing is written outside the pool. Outputs must not overlap inputs
+ * stride in bytes; an entry of a block table that is 0 (the sink) or outside [0, pages) is taken for no page (its tokens
+ * have no slot and are left out of the attention, a state outside [0, pages) reads as zeros), and nothing is written
+ * outside the pool. Outputs must not overlap inputs
  * (but for states and tables updated in place), and calls that may run at the same time need scratches of their own. */
 
 /* Block tables and slot maps from the requests' lengths, on the device. Row r of b holds lengths[r] tokens and adds
@@ -267,9 +268,9 @@ int jb_kv_scatter(const uint16_t* kn, const uint16_t* vn, int b, int n, const in
  * and convolution pages). All other entries stay. The new tokens are packed row after row: for token t of `tokens`
  * slots[t] = page * page_tokens + place in the page, rows[t] and positions[t]; -1, -1 and 0 past the last one. starts
  * (b + 1) is each row's first token, taken (b + 1) the pages that the rows before it take. taken[b] > free_count: the
- * list was too short; the entries past it are 0 (the sink) and their tokens' slots -1. A token past the table's last
- * entry (width) takes no page and has slot -1; tokens past `tokens` are not listed. b and
- * tokens: at most 0x7f000000. */
+ * list was too short; the entries past it are 0 (the sink) and their tokens' slots -1, in this call and in later ones
+ * (such an entry counts as held). A token past the table's last entry (width) takes no page and has slot -1; tokens past
+ * `tokens` are not listed. b and tokens: at most 0x7f000000. */
 int jb_block_tables(const int32_t* lengths, const int32_t* added, int b, const int32_t* free_pages, int free_count,
                     int32_t* tables, int table_stride, int width, int kv_entry, int page_tokens, int fixed, int tokens,
                     int64_t* slots, int32_t* rows, int32_t* positions, int32_t* starts, int32_t* taken, void* stream);

@@ -7,6 +7,9 @@ namespace jb {
 namespace dec {
 
 constexpr int PAGE = 32;   // tokens of a key/value page
+// The pool's page 0 takes what belongs nowhere, and a table names it where no page was to be had: as an entry of a table
+// it is no page, so that nothing that other rows left there is attended to and no two tokens get one slot.
+constexpr int SINK = 0;
 
 // ------------------------------------------------------------------ block tables and slot maps
 //
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(TAB_THREADS) tables_kernel(const TabParams p) 
         const long long at = s_take[l] + row.head + j - row.held;
         if (at < p.free_count) page = p.free_pages[at];
       }
-      p.slots[t] = page < 0 ? -1 : (int64_t)page * p.page + pos % p.page;
+      p.slots[t] = page <= SINK ? -1 : (int64_t)page * p.page + pos % p.page;
       p.rows[t] = r0 + l;
       p.positions[t] = pos;
     }
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(TAB_THREADS) tables_kernel(const TabParams p) 
       }
       int* dst = p.tables + (int64_t)(r0 + j) * p.table_stride;
       for (int i = lane; i < row.take; i += 32)
-        dst[i < row.head ? i : p.kv_entry + row.held + i - row.head] = at + i < p.free_count ? p.free_pages[at + i] : 0;
+        dst[i < row.head ? i : p.kv_entry + row.held + i - row.head] = at + i < p.free_count ? p.free_pages[at + i] : SINK;
     }
     base_add = ta;
     base_take = tk;
@@ -606,7 +609,7 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
     const int j = x.step * L::STEP + warp * TILE;
     if (j >= x.len) return -1;
     const int page = p.tables[(int64_t)x.row * p.table_stride + p.kv_entry + j / PAGE];
-    return page >= 0 && page < p.pages ? page : -1;
+    return page > SINK && page < p.pages ? page : -1;
   };
   // the fetches' cursor, half a tile at a time: the unit, its page (loaded one unit ahead, so that its load never stands
   // in a fetch's way), keys or values, and the slot; `valid` has a bit for each tile fetched and not yet used

@@ -429,8 +429,9 @@ def block_tables(lengths: torch.Tensor, new: torch.Tensor, free: torch.Tensor, t
     are written behind the row's own in `tables`, in place; fixed: a row that holds no token yet first takes kv_entry
     pages into its entries [0, kv_entry) (a prefix's state and convolution pages, PrefixPool.reserve's order). Every
     other entry stays as it was. `tokens` is the pass's capacity. taken[-1] > len(free) says that the free list was too
-    short: the entries it leaves without a page name the sink (0), and their tokens' slots are -1, as are those of
-    tokens past the table's width."""
+    short: the entries it leaves without a page name the sink (0), and their tokens' slots are -1, also those of later
+    calls on these entries, as are those of tokens past the table's width. Page 0 is never a page to take: `free` must
+    not list it."""
     dev = lengths.device
     b = lengths.shape[0] if lengths.dim() == 1 else -1
     _rows_of(lengths, "lengths", torch.int32, (b,), 1, dev)
@@ -525,12 +526,12 @@ def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, at
                      kv_entry: int, *, scale: float | None = None, pr: torch.Tensor | None = None,
                      out: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of one new token per row, q (b, heads, dim), over the row's lengths[r] cached tokens (its own among
-    them, once attn_prep_axes has written it) in the pages tables[r][kv_entry + j // 32] of kv; heads of 64, 128 or
-    256, up to 16 query heads to a key/value head, scale 1 / sqrt(dim) unless given. A row without tokens is zeros.
-    With pr (the q_proj output, query and gate interleaved per head): times sigmoid(gate), as (b, heads * dim), the
-    o_proj's input; without, (b, heads, dim). fp32 with one rounding. All rows' keys are cut into equal shares over
-    the SMs, whatever the lengths; scratch (fp32, jb_decode_attention_scratch of them, overwritten by every call; calls
-    that may run at the same time need their own) holds the cut rows' parts and is allocated unless given."""
+    them, once attn_prep_axes has written it) in the pages tables[r][kv_entry + j // 32] of kv (an entry that is 0, the
+    sink, or outside kv is no page: its tokens are left out); heads of 64, 128 or 256, up to 16 query heads to a
+    key/value head, scale 1 / sqrt(dim) unless given. A row without tokens is zeros. With pr (the q_proj output, query
+    and gate interleaved per head): times sigmoid(gate), as (b, heads * dim), the o_proj's input; without, (b, heads,
+    dim). fp32 with one rounding. All rows' keys are cut into equal shares over the SMs, whatever the lengths; scratch
+    (fp32, jb_decode_attention_scratch of them, overwritten by every call; calls that may run at the same time need their own) holds the cut rows' parts and is allocated unless given."""
     dev = q.device
     shape = q.shape
     if len(shape) != 3:

@@ -503,6 +503,26 @@ def test_decode_attention_far_pages() -> None:
     close(got, *plain_decode(q, [rows], 1 / 16))
 
 
+def test_rows_left_short_of_pages_stay_without_them() -> None:
+    """A row that found the free list empty holds the sink in its table: its later tokens on that page have no slot either,
+    and its attention leaves the page out, whatever the sink holds."""
+    g = gen(40)
+    tables = torch.zeros(3, 6, dtype=torch.int32, device="cuda")
+    tables[:, :3] = i32([[9, 9, 5], [9, 9, 6], [9, 9, 8]])
+    lengths, new = i32([32, 32, 5]), i32([1, 1, 1])
+    got = kernels.block_tables(lengths, new, i32([7]), tables, 2, 3)
+    assert got.slots.tolist() == [7 * 32, -1, 8 * 32 + 5] and got.taken.tolist() == [0, 1, 2, 2]
+    lengths += new
+    got = kernels.block_tables(lengths, new, i32([]), tables, 2, 3)   # takes no page, so nothing else reports it
+    assert got.slots.tolist() == [7 * 32 + 1, -1, 8 * 32 + 6] and got.taken.tolist() == [0, 0, 0, 0]
+    assert got.positions.tolist() == [33, 33, 6] and tables[:, 2:].tolist() == [[5, 7, 0, 0], [6, 0, 0, 0], [8, 0, 0, 0]]
+    kv = normal(g, 10, 2, 2, 32, 2, 256)
+    q = normal(g, 3, 8, 256)
+    y = kernels.decode_attention(q, kv, tables, 1, i32([34, 34, 7]), 2)
+    dense = [torch.cat([kv[5, 1], kv[7, 1, :, :2]], 1), kv[6, 1], kv[8, 1, :, :7]]
+    close(y, *plain_decode(q, dense, 1 / 16))
+
+
 # ---------------------------------------------------------------- linear attention
 
 
