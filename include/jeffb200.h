@@ -256,10 +256,10 @@ int jb_kv_scatter(const uint16_t* kn, const uint16_t* vn, int b, int n, const in
  *
  * What a continuation token by token needs beside the decision pass. These entry points have no counterpart in the
  * reference, which only answers prefill passes. Key/value pages are given as the pool's data, its pages and their
- * stride in bytes; an entry of a block table that is 0 (the sink) or outside [0, pages) is taken for no page (its tokens
- * have no slot and are left out of the attention, a state outside [0, pages) reads as zeros), and nothing is written
- * outside the pool. Outputs must not overlap inputs
- * (but for states and tables updated in place), and calls that may run at the same time need scratches of their own. */
+ * stride in bytes; an entry of a block table that is 0 (the sink) or outside [0, pages) is taken for no page (its
+ * tokens have no slot and are left out of the attention, a state in it reads as zeros), and nothing is written outside
+ * the pool. Outputs must not overlap inputs (but for states and tables updated in place), and calls that may run at
+ * the same time need scratches of their own. */
 
 /* Block tables and slot maps from the requests' lengths, on the device. Row r of b holds lengths[r] tokens and adds
  * added[r] (negative counts as 0). It takes the pages its new tokens need, off the free list in row order (free_pages,
@@ -318,8 +318,9 @@ int jb_linear_scan(const uint16_t* q, int64_t q_row, int64_t q_tok, const uint16
 int jb_linear_scan_scratch(int b, int heads, int n);
 
 /* jb_linear_scan's recurrence for one token per row (q, k, v (b, heads, 128), g (b, heads) or one decay for each head,
- * o (b, heads, 128)), the new states written to out_tables' pages (the same tables: in place). beta (nullable, bf16
- * (b, heads)): the gated delta rule of jb_gdn_scan, v replaced by beta (v - (e^g S)^T k). */
+ * o (b, heads, 128)), the new states written to out_tables' pages (the same tables: in place; never to the reserved
+ * pages). beta (nullable, bf16 (b, heads)): the gated delta rule of jb_gdn_scan, v replaced by
+ * beta (v - (e^g S)^T k). */
 int jb_linear_step(const uint16_t* q, int64_t q_row, const uint16_t* k, int64_t k_row, const uint16_t* v,
                    int64_t v_row, const float* g, int64_t g_row, const uint16_t* beta, uint16_t* o, int b, int heads,
                    void* state, int64_t pages, int64_t page_bytes, int heads_per_page, int first_head,

@@ -4,14 +4,15 @@
 // beta is the gated delta rule (v_t replaced by beta_t (v_t - (e^{g_t} S_{t-1})^T k_t)).
 //
 // A state is at slot (flat head % heads_per_page) of page tables[r][flat head / heads_per_page], as in gdn.cu. A page
-// outside the pool reads as zeros; nothing is written to such a page or to the reserved pages (the sink, the zeros).
+// outside the pool reads as zeros, and so does the sink, which a table names where no page was to be had and which holds
+// what others left there; nothing is written to such pages or to the page of zeros.
 
 namespace jb {
 namespace lin {
 
 constexpr int D = 128;
 constexpr int64_t STATE_BYTES = (int64_t)D * D * 4;
-constexpr int RESERVED = 2;
+constexpr int SINK = 0, RESERVED = 2;
 
 struct Pool {
   uint8_t* base;
@@ -26,7 +27,7 @@ struct Pool {
 __device__ __forceinline__ const float* state_in(const Pool& p, int row, int h) {
   const int flat = p.first_head + h;
   const int page = p.tables[(int64_t)row * p.table_stride + flat / p.heads_per_page];
-  if (page < 0 || page >= p.pages) return nullptr;
+  if (page <= SINK || page >= p.pages) return nullptr;
   return reinterpret_cast<const float*>(p.base + page * p.page_bytes + (flat % p.heads_per_page) * STATE_BYTES);
 }
 __device__ __forceinline__ float* state_out(const Pool& p, int row, int h) {

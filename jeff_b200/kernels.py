@@ -531,7 +531,8 @@ def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, at
     key/value head, scale 1 / sqrt(dim) unless given. A row without tokens is zeros. With pr (the q_proj output, query
     and gate interleaved per head): times sigmoid(gate), as (b, heads * dim), the o_proj's input; without, (b, heads,
     dim). fp32 with one rounding. All rows' keys are cut into equal shares over the SMs, whatever the lengths; scratch
-    (fp32, jb_decode_attention_scratch of them, overwritten by every call; calls that may run at the same time need their own) holds the cut rows' parts and is allocated unless given."""
+    (fp32, jb_decode_attention_scratch of them, overwritten by every call; calls that may run at the same time need
+    their own) holds the cut rows' parts and is allocated unless given."""
     dev = q.device
     shape = q.shape
     if len(shape) != 3:
@@ -611,13 +612,14 @@ def linear_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
                 tables: torch.Tensor, layer: int, *, real: torch.Tensor | None = None,
                 out_tables: torch.Tensor | None = None, out: torch.Tensor | None = None,
                 scratch: torch.Tensor | None = None) -> torch.Tensor:
-    """Linear attention with a decay for each head over q, k, v (b, n, heads, 128): S_t = e^g S_(t-1) + k_t v_t^T,
-    o_t = S_t^T q_t / sqrt(128), each row from its state in the pages `state` (PrefixPool.state; head h of `layer` is
-    flat head layer * heads + h) that its row of tables names. g: log-decays (b, n, heads) fp32, or (heads,), one for
-    each head; -inf forgets. real (b,) int32: row r has real[r] tokens, its outputs past them are zeros. out_tables:
-    the rows' final states are written to these pages (the reserved pages 0 and 1 never are); rows must not share
-    them, nor write pages that another row reads. scratch (fp32, jb_linear_scan_scratch of them, one for each of the
-    calls that may run at the same time) is allocated unless given. out must not overlap q, k or v."""
+    """Linear attention with a decay for each head over q, k, v (b, n, heads, 128): S_t = e^g S_(t-1) + k_t v_t^T, o_t =
+    S_t^T q_t / sqrt(128), each row from its state in the pages `state` (PrefixPool.state; head h of `layer` is flat
+    head layer * heads + h) that its row of tables names. g: log-decays (b, n, heads) fp32, or (heads,), one for each
+    head; -inf forgets. real (b,) int32: row r has real[r] tokens, its outputs past them are zeros. out_tables: the
+    rows' final states are written to these pages (the reserved pages 0 and 1 never are); rows must not share them, nor
+    write pages that another row reads. A state on page 0, the sink, or outside `state` reads as zeros. scratch (fp32,
+    jb_linear_scan_scratch of them, one for each of the calls that may run at the same time) is allocated unless given.
+    out must not overlap q, k or v."""
     if q.dim() != 4:
         raise ValueError(f"q: expected (rows, tokens, heads, {C.DK}), got {tuple(q.shape)}")
     b, n, heads = q.shape[:3]
@@ -643,8 +645,8 @@ def linear_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
                 out_tables: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """linear_scan's recurrence for one token per row, q, k, v (b, heads, 128), g (b, heads) or (heads,): o (b, heads,
     128), the new states written in place, or to out_tables' pages (rows must not share them, nor write pages that
-    another row reads). beta (b, heads) bf16: the gated delta rule of gdn_scan, v replaced by beta (v - (e^g S)^T k).
-    out must not overlap q, k or v."""
+    another row reads; the new state of a row whose page is 0 or 1, reserved, is dropped). beta (b, heads) bf16: the
+    gated delta rule of gdn_scan, v replaced by beta (v - (e^g S)^T k). out must not overlap q, k or v."""
     if q.dim() != 3:
         raise ValueError(f"q: expected (rows, heads, {C.DK}), got {tuple(q.shape)}")
     b, heads = q.shape[:2]

@@ -755,6 +755,23 @@ def test_linear_scan_padding_past_32_bits() -> None:
     torch.cuda.empty_cache()   # 69 GB
 
 
+@pytest.mark.parametrize("n", [1, 5, 40, 700])
+def test_linear_states_in_the_sink_read_as_zeros(n) -> None:
+    """A fresh row that found no page for its state starts from zeros, whatever the sink holds; other rows are as ever."""
+    q, k, v, g, state, tables, outs, begin = linear_case(16, 2, n, 6, 6, 0, "mixed")
+    tables[0, 0] = 0
+    state[0] = math.nan
+    begin[0] = 0
+    o, mag, s, m = plain_linear(q, k, v, g, begin, i32([n] * 2))
+    got = kernels.linear_scan(q, k, v, g, state, tables, 0, out_tables=outs)
+    close(got, o, HALF * o.abs() + (HALF + 2.0 ** -13) * mag)
+    page, slot = spots(outs, 0, 6, 6)
+    close(state[page, slot], s, (2.0 ** -20 + (n / 4 + 64) * ULP) * m + 1e-30)
+    if n == 1:
+        got = kernels.linear_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], state, tables, 0, out_tables=outs)
+        close(got, o[:, 0], HALF * o[:, 0].abs() + (300 * ULP + 2.0 ** -21) * mag[:, 0])
+
+
 # ---------------------------------------------------------------- together
 
 
