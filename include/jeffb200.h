@@ -307,7 +307,8 @@ int jb_decode_attention_scratch(int heads, int kv_heads, int dim);
  * log-decay at g[row * g_row + token * g_tok + h] (strides 0, 0: one decay for each head). real (nullable): row r has
  * real[r] tokens; outputs past them are 0 and the state stays. out_tables (nullable): the final states' pages; the
  * reserved pages 0 and 1 are never written. scratch: at least jb_linear_scan_scratch floats, 16-byte aligned,
- * overwritten (a few long rows are computed in segments, whose states it holds). */
+ * overwritten (a few long rows are computed in segments, whose states it holds). What is not finite spoils what the
+ * recurrence spoils, no earlier output and no other head; where that gives an infinity it may be NaN. */
 int jb_linear_scan(const uint16_t* q, int64_t q_row, int64_t q_tok, const uint16_t* k, int64_t k_row, int64_t k_tok,
                    const uint16_t* v, int64_t v_row, int64_t v_tok, const float* g, int64_t g_row, int64_t g_tok,
                    const int32_t* real, uint16_t* o, int b, int n, int heads, void* state, int64_t pages,

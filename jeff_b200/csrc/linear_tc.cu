@@ -11,7 +11,8 @@
 // Ahead of an output's own rounding its terms are rounded once, by P for the tokens of its chunk, by the state's bf16
 // copy for those before (where the state itself is another launch's, two parts of Kd, 16 bits, serve that copy). Sums
 // of decays are fp64, their differences rounded to fp32 once, so that a strong decay early in a chunk takes no accuracy
-// from the tokens behind it (-inf is held as -10000, whose exponential is 0).
+// from the tokens behind it (-inf is held as -10000, whose exponential is 0). A value that is not finite would reach earlier
+// tokens of its chunk through the zeros of P: where an output is not finite it is formed again without them.
 //
 // Tensor memory, 256 columns: S^T 0-127, its bf16 copy 128-191 (E once MMA1 has read it), D 192-255. Shared memory 108
 // KB: two CTAs per SM, whose phases (TMA, tensor core, CUDA cores) fill each other's waits. Within a chunk Kd and the
@@ -224,11 +225,50 @@ struct Bool {
   static constexpr bool value = B;
 };
 
+// A warp's outputs of a chunk again (32 channels of 32 tokens, in the output tile already), where MMA3 met a value that is
+// not finite: above P's diagonal 0 * NaN and 0 * inf are NaN, which spoils the tokens ahead of that value. Here a token's
+// sum ends at the token, P and the values from shared and global memory, and a value that is not finite goes by the
+// recurrence, through each product with its key. Finding such outputs costs 1% of a long row's time (two rows of 8,192
+// tokens 106.9 -> 108.1 us) and nothing of a short one's (64 rows of 128 tokens 65.0 -> 63.8).
+__device__ __noinline__ void outputs_again(const Args& a, uint8_t* ot, uint8_t* pt, const Gates& gt, uint32_t ta,
+                                           int row, int h, int start, int live, int qd, int ch) {
+  const int lane = threadIdx.x & 31;
+  const __nv_bfloat16* q = a.q + row * a.q_row + start * a.q_tok + h * D;
+  const __nv_bfloat16* k = a.k + row * a.k_row + start * a.k_tok + h * D;
+  const __nv_bfloat16* v = a.v + row * a.v_row + start * a.v_tok + h * D;
+  const float scale = rsqrtf((float)D);
+  for (int hf = 0; hf < 2; ++hf) {
+    uint32_t d[16], e[16];
+    tmem_ld_frag(ta + ((uint32_t)(16 * hf) << 16) + TM_D, d);
+    tmem_ld_frag(ta + ((uint32_t)(16 * hf) << 16) + TM_B, e);
+    tc_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int t = 32 * ch + 8 * (j >> 2) + 2 * (lane & 3) + (j & 1);
+      const int x = 32 * qd + 16 * hf + 8 * (j >> 1 & 1) + (lane >> 2);
+      const float before = gt.from_start[t] * __uint_as_float(d[j]);
+      if (t >= live || isfinite(__uint_as_float(e[j])) || !isfinite(before)) continue;
+      float sum = before;
+      for (int s = 0; s <= t; ++s) {
+        const float vs = bf2f(v[s * a.v_tok + x]);
+        if (isfinite(vs)) {
+          sum += bf2f(reinterpret_cast<const __nv_bfloat16*>(swz(pt, t, s >> 3))[s & 7]) * vs;
+        } else {
+          float w = 0.f;
+          for (int i = 0; i < D; ++i) w += bf2f(q[t * a.q_tok + i]) * (bf2f(k[s * a.k_tok + i]) * vs);
+          sum += w * exp2_fast((gt.hi[t] - gt.hi[s]) + (gt.lo[t] - gt.lo[s]));
+        }
+      }
+      reinterpret_cast<__nv_bfloat16*>(swz(ot + (x >> 6) * 8192, t, (x & 63) >> 3))[x & 7] = f2bf(sum * scale);
+    }
+  }
+}
+
 template <int MODE>
 __global__ void __launch_bounds__(THREADS, 2)
     scan_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o, const Args a,
-                const Seg seg, int* err) {
+                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
+                const __grid_constant__ Args a, const Seg seg, int* err) {
   // The outputs' launch is let go by join_kernel's CTAs once they have seen the states' launch end, and that one began
   // when everything before it had ended: the inputs are there. Only the segments' states are waited for.
   if (MODE == WHOLE) pdl_begin();
@@ -521,6 +561,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     const float scale = rsqrtf((float)D);
     const int tq = lane & 3;
     uint32_t pk[4][4];   // 8 tokens each: the warp's four groups of 8 channels
+    uint32_t zero = 0;   // the outputs times 0: NaN where one is not finite
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       uint32_t d[16], e[16];
@@ -538,6 +579,7 @@ __global__ void __launch_bounds__(THREADS, 2)
           const float y =
               fmaf(f.y, __uint_as_float(d[4 * i + 2 * g8 + 1]), __uint_as_float(e[4 * i + 2 * g8 + 1])) * scale;
           pk[i][2 * hf + g8] = pack_bf2(t < live ? x : 0.f, t + 1 < live ? y : 0.f);
+          asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(zero) : "r"(pk[i][2 * hf + g8]), "r"(0));
         }
       }
     }
@@ -546,6 +588,10 @@ __global__ void __launch_bounds__(THREADS, 2)
     for (int i = 0; i < 4; ++i)
       st_frags_trans(smem_u32(swz(ot + (x >> 6) * 8192, 32 * ch + 8 * i + (lane & 7), (x & 63) >> 3)), pk[i][0],
                      pk[i][1], pk[i][2], pk[i][3]);
+    if (__any_sync(0xffffffffu, zero & 0x7fff7fffu)) {
+      __syncwarp();
+      outputs_again(a, ot, pt, gt, tmem + lane_bits + 32 * ch, row, h, start_of(c), live, qd, ch);
+    }
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();

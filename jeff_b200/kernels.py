@@ -619,7 +619,8 @@ def linear_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     rows' final states are written to these pages (the reserved pages 0 and 1 never are); rows must not share them, nor
     write pages that another row reads. A state on page 0, the sink, or outside `state` reads as zeros. scratch (fp32,
     jb_linear_scan_scratch of them, one for each of the calls that may run at the same time) is allocated unless given.
-    out must not overlap q, k or v."""
+    What is not finite in q, k, v, g or a state spoils what the recurrence spoils, no earlier output and no other head;
+    where that gives an infinity it may be NaN. out must not overlap q, k or v."""
     if q.dim() != 4:
         raise ValueError(f"q: expected (rows, tokens, heads, {C.DK}), got {tuple(q.shape)}")
     b, n, heads = q.shape[:3]

@@ -772,6 +772,41 @@ def test_linear_states_in_the_sink_read_as_zeros(n) -> None:
         close(got, o[:, 0], HALF * o[:, 0].abs() + (300 * ULP + 2.0 ** -21) * mag[:, 0])
 
 
+@pytest.mark.parametrize("real", [False, True])
+@pytest.mark.parametrize(("b", "n", "heads"), [(2, 5, 16), (2, 100, 3), (20, 130, 16), (1, 700, 16), (2, 1001, 2)])
+def test_linear_scan_passes_what_is_not_finite_on(b, n, heads, real) -> None:
+    """A value, key, query or decay that is not finite spoils what the recurrence spoils, the outputs from its token on
+    and its entries of the state, and no earlier token's output, other column or head."""
+    q, k, v, g, state, tables, outs, begin = linear_case(17, b, n, heads, 6, 0, "mixed")
+    last = n - 2 if real else n
+    at = n // 2 + 1   # the middle of a chunk
+    h = heads - 1
+    v[0, at, 0, 7] = math.nan
+    v[b - 1, at + 1, 1, 100] = math.inf
+    v[0, last - 1, 1, 127] = -math.inf
+    q[0, at - 1, 0, 3] = math.nan
+    if heads > 2:
+        k[0, at, 2, 9] = math.nan
+        k[b - 1, last - 1, 2, 60] = math.inf
+    if heads > 5:
+        g[0, at, h] = math.nan
+        k[0, 3, h - 1, 100] = -math.inf
+        v[b - 1, n // 3:n // 3 + 2, h - 2, :64] = -math.inf
+    lengths = i32([last] * b)
+    o, _, s, _ = plain_linear(q, k, v, g, begin, lengths)
+    clean = [torch.where(x.isfinite(), x, 1) for x in (q, k, v, g)]
+    _, mag, _, m = plain_linear(*clean, begin, lengths)
+    got = kernels.linear_scan(q, k, v, g, state, tables, 0, real=lengths if real else None, out_tables=outs)
+    page, slot = spots(outs, 0, heads, 6)
+    ends = state[page, slot]
+    assert not o.isfinite().all() and not s.isfinite().all()
+    assert torch.equal(got.isfinite(), o.isfinite()) and torch.equal(ends.isfinite(), s.isfinite())
+    fine = o.isfinite()
+    close(got[fine], o[fine], (HALF * o.abs() + (HALF + 2.0 ** -13) * mag)[fine])
+    fine = s.isfinite()
+    close(ends[fine], s[fine], ((2.0 ** -20 + (n / 4 + 64) * ULP) * m + 1e-30)[fine])
+
+
 # ---------------------------------------------------------------- together
 
 
