@@ -259,7 +259,8 @@ int jb_kv_scatter(const uint16_t* kn, const uint16_t* vn, int b, int n, const in
  * stride in bytes; an entry of a block table that is 0 (the sink) or outside [0, pages) is taken for no page (its
  * tokens have no slot and are left out of the attention, a state in it reads as zeros), and nothing is written outside
  * the pool. Outputs must not overlap inputs (but for states and tables updated in place), and calls that may run at
- * the same time need scratches of their own. */
+ * the same time need scratches of their own. The row stride of bf16 inputs and outputs of one row, and the token stride
+ * of one token, may be anything. */
 
 /* Block tables and slot maps from the requests' lengths, on the device. Row r of b holds lengths[r] tokens and adds
  * added[r] (negative counts as 0). It takes the pages its new tokens need, off the free list in row order (free_pages,

@@ -956,6 +956,7 @@ extern "C" int jb_attn_prep_axes(const uint16_t* pr, int64_t ldpr, int t, const 
                                  int attn_layer, int attn_layers, const int64_t* slots, void* stream) {
   using namespace jb;
   JB_REQUIRE(pr && q_w1 && k_w1 && inv_freq && positions && q, "jb_attn_prep_axes: null pointer");
+  if (t == 1) ldpr = dec::NQ * 2 * dec::HD + 2 * dec::NKV * dec::HD;   // a single row's stride says nothing
   JB_REQUIRE(t > 0 && ldpr >= dec::NQ * 2 * dec::HD + 2 * dec::NKV * dec::HD && ldpr % 8 == 0 && axis_stride >= 0,
              "jb_attn_prep_axes: t %d, ldpr %lld, axis stride %lld", t, (long long)ldpr, (long long)axis_stride);
   JB_REQUIRE((kn != nullptr) == (vn != nullptr) && (kv != nullptr) == (slots != nullptr) && (kn || kv),
@@ -1005,6 +1006,10 @@ extern "C" int jb_decode_attention(const uint16_t* q, int64_t ldq, const void* k
              "jb_decode_attention: tables of %lld tokens, %d key/value heads", (long long)most, kv_heads);
   JB_REQUIRE((int64_t)heads * dim <= 1 << 24 && b <= 0x7f000000, "jb_decode_attention: %d rows of %d heads of %d", b,
              heads, dim);
+  if (b == 1) {   // a single row's strides say nothing
+    ldq = ldy = heads * dim;
+    ldpr = 2 * heads * dim;
+  }
   JB_REQUIRE(ldq >= heads * dim && ldq % 8 == 0 && ldy >= heads * dim && ldy % 8 == 0 &&
                  (!pr || (ldpr >= 2 * heads * dim && ldpr % 8 == 0)),
              "jb_decode_attention: row strides %lld, %lld, %lld", (long long)ldq, (long long)ldy, (long long)ldpr);

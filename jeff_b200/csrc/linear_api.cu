@@ -22,6 +22,8 @@ extern "C" int jb_linear_scan(const uint16_t* q, int64_t q_row, int64_t q_tok, c
                               const int32_t* tables, int table_stride, const int32_t* out_tables, int out_stride,
                               float* scratch, int64_t scratch_floats, void* stream) {
   using namespace jb;
+  if (n == 1) q_tok = k_tok = v_tok = (int64_t)heads * lin::D;   // a single token's strides say nothing, nor a single row's
+  if (b == 1) q_row = k_row = v_row = (int64_t)n * heads * lin::D;
   const lin::Args a = {reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<const __nv_bfloat16*>(k),
                        reinterpret_cast<const __nv_bfloat16*>(v), q_row, k_row, v_row, q_tok, k_tok, v_tok, g, g_row,
                        g_tok, nullptr, real, reinterpret_cast<__nv_bfloat16*>(o), (int64_t)n * heads * lin::D,
@@ -51,6 +53,7 @@ extern "C" int jb_linear_step(const uint16_t* q, int64_t q_row, const uint16_t* 
                               int first_head, const int32_t* tables, int table_stride, const int32_t* out_tables,
                               int out_stride, void* stream) {
   using namespace jb;
+  if (b == 1) q_row = k_row = v_row = (int64_t)heads * lin::D;
   const lin::Args a = {reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<const __nv_bfloat16*>(k),
                        reinterpret_cast<const __nv_bfloat16*>(v), q_row, k_row, v_row, 0, 0, 0, g, g_row, 0,
                        reinterpret_cast<const __nv_bfloat16*>(beta), nullptr, reinterpret_cast<__nv_bfloat16*>(o),

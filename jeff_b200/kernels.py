@@ -379,11 +379,16 @@ def _rows_of(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, .
         step *= size
 
 
+def _apart(t: torch.Tensor) -> int:
+    """Elements from one row (page, table) of `t` to the next; of a single one, whose stride may be anything, its own."""
+    return t.stride(0) if t.shape[0] > 1 else t.numel()
+
+
 def _tables_of(tables: torch.Tensor, name: str, rows: int, width: int, device: torch.device) -> None:
     """Block tables of at least `rows` rows and `width` entries, packed or with their rows apart."""
     shape = tables.shape
     if len(shape) != 2 or shape[0] < rows or shape[1] < width or tables.dtype is not torch.int32 or \
-            not (tables.is_contiguous() or tables.stride(1) == 1):
+            not (tables.is_contiguous() or tables.stride(1) == 1 or shape[1] == 1):
         raise ValueError(f"{name}: expected int32 (rows >= {rows}, width >= {width}) with packed rows, got "
                          f"{tuple(shape)} {tables.dtype}, strides {tables.stride()}")
     if tables.device != device:
@@ -450,7 +455,7 @@ def block_tables(lengths: torch.Tensor, new: torch.Tensor, free: torch.Tensor, t
             _rows_of(getattr(out, name), name, dtype, (size,), 1, dev)
     slots, rows, positions, starts, taken = out
     _on(dev, "jb_block_tables", lengths.data_ptr(), new.data_ptr(), b, free.data_ptr(), free.shape[0],
-        tables.data_ptr(), tables.stride(0), tables.shape[1], kv_entry, page_tokens, 1 if fixed else 0, tokens,
+        tables.data_ptr(), _apart(tables), tables.shape[1], kv_entry, page_tokens, 1 if fixed else 0, tokens,
         slots.data_ptr(), rows.data_ptr(), positions.data_ptr(), starts.data_ptr(), taken.data_ptr())
     return out
 
@@ -509,7 +514,7 @@ def attn_prep_axes(pr: torch.Tensor, q_w1: torch.Tensor, k_w1: torch.Tensor, inv
         out = pr.new_empty((t, C.NQ, C.HD))
     else:
         _rows_of(out, "out", DT, (t, C.NQ, C.HD), 3, dev)
-    pages = (None, 0, 0, attn_layer, 0) if kv is None else (kv.data_ptr(), kv.shape[0], 2 * kv.stride(0), attn_layer,
+    pages = (None, 0, 0, attn_layer, 0) if kv is None else (kv.data_ptr(), kv.shape[0], 2 * _apart(kv), attn_layer,
                                                             kv.shape[1])
     _on(dev, "jb_attn_prep_axes", pr.data_ptr(), pr.stride(0), t, q_w1.data_ptr(), k_w1.data_ptr(),
         inv_freq.data_ptr(), positions.data_ptr(), positions.stride(0), axes - (1 << 64) if axes >> 63 else axes,
@@ -557,8 +562,8 @@ def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, at
         scratch = q.new_empty(_decode_scratch(heads, kv_heads, dim), dtype=torch.float32)
     else:
         _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), dev)
-    _on(dev, "jb_decode_attention", q.data_ptr(), q.stride(0), kv.data_ptr(), pages, 2 * kv.stride(0), attn_layer,
-        layers, tables.data_ptr(), tables.stride(0), tables.shape[1], kv_entry, lengths.data_ptr(), b, heads,
+    _on(dev, "jb_decode_attention", q.data_ptr(), q.stride(0), kv.data_ptr(), pages, 2 * _apart(kv), attn_layer,
+        layers, tables.data_ptr(), _apart(tables), tables.shape[1], kv_entry, lengths.data_ptr(), b, heads,
         kv_heads, dim, dim ** -0.5 if scale is None else scale, ptr(pr), 0 if pr is None else pr.stride(0),
         out.data_ptr(), out.stride(0), scratch.data_ptr(), scratch.numel())
     return out
@@ -598,9 +603,8 @@ def _linear_of(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
         out = torch.empty_like(v, memory_format=torch.contiguous_format)
     else:
         _rows_of(out, "out", DT, shape, len(shape), dev)
-    return out, (state.data_ptr(), held[0], 4 * state.stride(0), held[1], layer * heads,
-                 tables.data_ptr(), tables.stride(0), ptr(out_tables),
-                 0 if out_tables is None else out_tables.stride(0))
+    return out, (state.data_ptr(), held[0], 4 * _apart(state), held[1], layer * heads, tables.data_ptr(),
+                 _apart(tables), ptr(out_tables), 0 if out_tables is None else _apart(out_tables))
 
 
 @functools.lru_cache(maxsize=256)

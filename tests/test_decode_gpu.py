@@ -807,6 +807,58 @@ def test_linear_scan_passes_what_is_not_finite_on(b, n, heads, real) -> None:
     close(ends[fine], s[fine], ((2.0 ** -20 + (n / 4 + 64) * ULP) * m + 1e-30)[fine])
 
 
+def one_row(t: torch.Tensor, stride: int) -> torch.Tensor:
+    """`t`, one row long, with `stride` between its rows: what a transposed or narrowed tensor may bring."""
+    return torch.as_strided(t, t.shape, (stride, *t.stride()[1:]), t.storage_offset())
+
+
+def test_one_row_with_any_stride() -> None:
+    """The stride of a dimension of one says nothing: a single row, page, token or table is taken as it stands."""
+    g = gen(41)
+    kv, tables, dense = cache(g, [70], 2, 1, 2, 256, entry=1)
+    q, pr, n = normal(g, 8, 1, 256).transpose(0, 1), normal(g, 1, 4096 + 8), i32([70])
+    assert q.is_contiguous() and q.stride(0) == 256
+    want, tol = plain_decode(q, dense, 1 / 16, pr)
+    for stride in (0, 1, 5):
+        out = one_row(torch.empty(1, 2048, dtype=torch.bfloat16, device="cuda"), stride)
+        kernels.decode_attention(q, kv, one_row(tables, stride), 1, n, 1, pr=one_row(pr, stride), out=out)
+        close(out.view(1, 8, 256), want, tol)
+        close(kernels.decode_attention(one_row(q, stride), one_row(kv[2:3], stride), tables * 0 + 5, 1, n, 1), want * 0,
+              tol * 0)   # a pool of one page, which the table does not name
+
+        w, f = torch.ones(256, device="cuda"), torch.ones(32, device="cuda")
+        x = normal(g, 1, C.ATTN_PROJ)
+        pages = [torch.zeros(1, 2, 2, 32, 2, 256, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        slot, axes = torch.tensor([3], device="cuda"), kernels.rope_axes((32,))
+        a = kernels.attn_prep_axes(x, w, w, f, i32([[9]]), axes, kv=pages[0], slots=slot)
+        b = kernels.attn_prep_axes(one_row(x, stride), w, w, f, one_row(i32([[9]]), stride), axes,
+                                   kv=one_row(pages[1], stride), slots=slot)
+        assert torch.equal(a, b) and torch.equal(*pages)
+
+        table = i32([[1, 2, 3, 0]])
+        made = kernels.block_tables(i32([33]), i32([40]), i32([8]), one_row(table, stride), 1, 40)
+        assert table.tolist() == [[1, 2, 3, 8]] and made.slots.tolist() == [3 * 32 + i for i in range(1, 32)] + [
+            8 * 32 + i for i in range(9)]
+
+        for tokens in (1, 4, 70, 1001):
+            lq, lk, lv, decay, state, ids, outs, _ = linear_case(18, 1, tokens, 6, 6, 0, "mixed")
+            page = int(outs[0, 0])
+            o = kernels.linear_scan(lq, lk, lv, decay, state, ids, 0, out_tables=outs)
+            end = state[page].clone()
+            o2 = kernels.linear_scan(*(one_row(y, stride) for y in (lq, lk, lv, decay)), state, one_row(ids, stride), 0,
+                                     out_tables=one_row(outs, stride))
+            assert torch.equal(o, o2) and torch.equal(state[page], end)
+        token = [y[:, 0] for y in (lq, lk, lv, decay)]
+        o = kernels.linear_step(*token, state, ids, 0, out_tables=outs)
+        o2 = kernels.linear_step(*(one_row(y, stride) for y in token), state, one_row(ids, stride), 0,
+                                 out_tables=one_row(outs, stride))
+        assert torch.equal(o, o2)
+        one = [y.unsqueeze(1) for y in token]   # one token of one row, both strides free
+        o3 = kernels.linear_scan(*(torch.as_strided(y, y.shape, (stride, 3, *y.stride()[2:]), y.storage_offset())
+                                   for y in one), state, ids, 0)
+        close(o3[:, 0], o.double(), 2 * HALF * o.double().abs() + 1e-5)
+
+
 # ---------------------------------------------------------------- together
 
 
