@@ -632,6 +632,8 @@ def linear_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     if real is not None:
         _rows_of(real, "real", torch.int32, (b,), 1, q.device)
     need = _scan_scratch(b, heads, n)
+    if need and not all(x.stride(1) > 0 and (b == 1 or x.stride(0) > 0) for x in (q, k, v)):
+        need = 0   # one token or row that stands for all goes token by token, in one launch
     if scratch is None:
         scratch = q.new_empty(need, dtype=torch.float32) if need else None
     else:

@@ -859,6 +859,27 @@ def test_one_row_with_any_stride() -> None:
         close(o3[:, 0], o.double(), 2 * HALF * o.double().abs() + 1e-5)
 
 
+def test_linear_scan_counts_its_launches() -> None:
+    """Rows in segments are three launches and need a scratch; inputs that go token by token, one key, value or query
+    standing for all, are one and need none."""
+    q, k, v, g, state, tables, _, _ = linear_case(19, 1, 700, 4, 4, 0, "mixed")
+    two = linear_case(20, 2, 700, 4, 4, 0, "mixed")
+
+    def made(*args, **kw) -> int:
+        before = _lib.launches
+        kernels.linear_scan(*args, 0, **kw)
+        return _lib.launches - before
+
+    none = torch.empty(0, device="cuda")
+    assert made(q, k, v, g, state, tables) == 3
+    assert made(q, k[:, :1].expand(-1, 700, -1, -1), v, g, state, tables, scratch=none) == 1
+    assert made(two[0], two[1], two[2][:1].expand(2, -1, -1, -1), *two[3:6], scratch=none) == 1
+    assert made(q[:, :7], k[:, :7], v[:, :7], g[:, :7], state, tables, scratch=none) == 1
+    assert made(q.expand(1, -1, -1, -1), k, v, g, state, tables) == 3
+    with pytest.raises(ValueError, match="a scratch of 0 floats"):
+        made(q, k, v, g, state, tables, scratch=none)
+
+
 # ---------------------------------------------------------------- together
 
 
