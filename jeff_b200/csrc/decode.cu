@@ -1031,7 +1031,8 @@ extern "C" int jb_decode_attention(const uint16_t* q, int64_t ldq, const void* k
 }
 
 extern "C" int jb_decode_attention_scratch(int heads, int kv_heads, int dim) {
-  return kv_heads > 0 && heads >= kv_heads && heads / kv_heads <= 16 && dim > 0 && dim <= 256
+  return kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= 16 &&
+                 (dim == 64 || dim == 128 || dim == 256)
              ? (int)jb::dec::dec_scratch(heads / kv_heads, dim)
              : 0;
 }

@@ -138,6 +138,14 @@ def test_scratch_sizes(lib) -> None:
         assert lib.jb_linear_scan_scratch(b, heads, n) == 0
 
 
+def test_no_scratch_size_for_heads_that_are_refused(lib) -> None:
+    for heads, kv_heads, dim in ((9, 2, 256), (8, 2, 96), (8, 2, 32), (0, 2, 64), (1, 2, 64), (17, 1, 64)):
+        assert lib.jb_decode_attention_scratch(heads, kv_heads, dim) == 0
+        assert _decode(lib, heads=heads, kv_heads=kv_heads, dim=dim) == -1
+    for dim in (64, 128, 256):
+        assert lib.jb_decode_attention_scratch(16, 1, dim) > lib.jb_decode_attention_scratch(4, 2, dim) > 0
+
+
 def test_rope_axes() -> None:
     def of(axes: int) -> list[int]:
         return [axes >> 2 * i & 3 for i in range(32)]
