@@ -60,7 +60,7 @@ __device__ __forceinline__ TabRow tab_row(const TabParams& p, int r) {
 
 __global__ void __launch_bounds__(TAB_THREADS) tables_kernel(const TabParams p) {
   pdl_begin();
-  __shared__ long long s_add[TAB_ROWS + 1], s_take[TAB_ROWS + 1];
+  __shared__ long long s_add[TAB_ROWS], s_take[TAB_ROWS];
   __shared__ long long w_add[TAB_THREADS / 32], w_take[TAB_THREADS / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int per = (p.tokens + gridDim.x - 1) / gridDim.x;
@@ -114,10 +114,6 @@ __global__ void __launch_bounds__(TAB_THREADS) tables_kernel(const TabParams p) 
       }
       ea += mine[i].add;
       ek += mine[i].take;
-    }
-    if (tid == TAB_THREADS - 1) {
-      s_add[TAB_ROWS] = ta;
-      s_take[TAB_ROWS] = tk;
     }
     __syncthreads();
     // this CTA's tokens that belong to these rows: the row by bisection of the sums
@@ -415,7 +411,7 @@ struct DecParams {
   const int* tables;
   int table_stride, kv_entry, most;   // tokens the table holds
   const int* lengths;
-  int b, kv_heads, group, dim;
+  int b, kv_heads, group;
   float scale_log2;
   const __nv_bfloat16* pr;
   int64_t ldpr;
@@ -431,31 +427,21 @@ struct DecParams {
 
 __device__ __forceinline__ int dec_length(const DecParams& p, int r) { return min(max(p.lengths[r], 0), p.most); }
 
-// Units (steps of one key/value head) of the rows before `row`, and of all; warp-collective.
+// Units (steps of one key/value head) of all rows; warp-collective.
 template <int STEP, class Len>
-__device__ void dec_units(const DecParams& p, const Len& len, int row, long long& before, long long& total) {
+__device__ long long dec_units(const DecParams& p, const Len& len) {
   const int lane = threadIdx.x & 31;
-  long long some = 0, all = 0;
+  long long all = 0;
   for (int r0 = 0; r0 < p.b; r0 += 128) {
-    int n[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = r0 + 32 * i + lane;
-      n[i] = r < p.b ? (len(r) + STEP - 1) / STEP : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      all += n[i];
-      if (r0 + 32 * i + lane < row) some += n[i];
+      all += r < p.b ? (len(r) + STEP - 1) / STEP : 0;
     }
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-    some += __shfl_xor_sync(0xffffffffu, some, o);
-  }
-  before = some * p.kv_heads;
-  total = all * p.kv_heads;
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  return all * p.kv_heads;
 }
 
 struct Cursor {   // a unit: a step of a row's head, and the row's tokens
@@ -593,8 +579,7 @@ __global__ void __launch_bounds__(Dec<D>::WARPS * 32, 1) decode_kernel(const Dec
     __syncthreads();
   }
   auto length = [&](int r) { return p.b <= HELD ? s_len[r] : dec_length(p, r); };
-  long long none, total;
-  dec_units<L::STEP>(p, length, 0, none, total);
+  const long long total = dec_units<L::STEP>(p, length);
   for (int r = blockIdx.x; r < p.b; r += gridDim.x)   // rows without tokens
     if (length(r) == 0)
       for (int i = threadIdx.x; i < p.kv_heads * p.group * D; i += L::WARPS * 32) p.y[r * p.ldy + i] = f2bf(0.f);
@@ -1022,7 +1007,7 @@ extern "C" int jb_decode_attention(const uint16_t* q, int64_t ldq, const void* k
              (long long)scratch_floats, (long long)dec::dec_scratch(group, dim));
   const dec::DecParams p = {reinterpret_cast<const __nv_bfloat16*>(q), ldq,
                             static_cast<const uint8_t*>(kv) + attn_layer * layer_bytes, pages, page_bytes, tables,
-                            table_stride, kv_entry, (int)most, lengths, b, kv_heads, group, dim,
+                            table_stride, kv_entry, (int)most, lengths, b, kv_heads, group,
                             scale * 1.4426950408889634f, reinterpret_cast<const __nv_bfloat16*>(pr), ldpr,
                             reinterpret_cast<__nv_bfloat16*>(y), ldy,
                             reinterpret_cast<unsigned long long*>(scratch), dec::dec_tag(), scratch + 4 * dec::SHARES};
