@@ -880,6 +880,25 @@ def test_linear_scan_counts_its_launches() -> None:
         made(q, k, v, g, state, tables, scratch=none)
 
 
+@pytest.mark.parametrize(("b", "n", "heads", "kind"), [(30, 192, 16, "heads"), (2, 2000, 16, "mixed")])
+def test_linear_scan_errors_do_not_lean(b, n, heads, kind) -> None:
+    """The outputs' errors are roundings, which lean to neither side, while a factor that is off by 2^-9 throughout leans.
+    With no negative number anywhere nothing cancels: along a chunk's outputs, the errors' projection has a variance of at
+    most (2^-8)^2 / 3 for each rounding of its terms, of the scores and of the state's copy, at the worst one rounding of
+    each shared by all. The mean over all rows' heads' chunks stays within six deviations, and 2^-13 for sums that cut off."""
+    q, k, v, g, state, tables, _, _ = linear_case(23, b, n, heads, 6, 0, kind)
+    q, k, v = q.abs(), k.abs(), v.abs()
+    state.abs_()
+    page, slot = spots(tables, 0, heads, 6)
+    got = kernels.linear_scan(q, k, v, g, state, tables, 0)
+    o, _, _, _ = plain_linear(q, k, v, g, state[page, slot], i32([n] * b))
+    lean = torch.stack([(x * y).sum((1, 3)) / (y * y).sum((1, 3)) for x, y in zip((got.double() - o).split(64, 1),
+                                                                                  o.split(64, 1))])
+    bound = 6 * HALF * (2 / 3 / lean.numel()) ** 0.5 + 2.0 ** -13
+    assert bound < 2.0 ** -10
+    assert abs(float(lean.mean())) <= bound
+
+
 # ---------------------------------------------------------------- together
 
 
