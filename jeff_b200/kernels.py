@@ -379,13 +379,9 @@ def _rows_of(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, .
         step *= size
 
 
-def _apart(t: torch.Tensor) -> int:
-    """Elements from one row (page, table) of `t` to the next; of a single one, whose stride may be anything, its own."""
-    return t.stride(0) if t.shape[0] > 1 else t.numel()
-
-
 def _tables_of(tables: torch.Tensor, name: str, rows: int, width: int, device: torch.device) -> None:
-    """Block tables of at least `rows` rows and `width` entries, packed or with their rows apart."""
+    """Block tables of at least `rows` rows and `width` entries, packed or with their rows apart. (Where one row, page or
+    token is all there is, its tensor's stride may be anything: the calls below give the packed size instead.)"""
     shape = tables.shape
     if len(shape) != 2 or shape[0] < rows or shape[1] < width or tables.dtype is not torch.int32 or \
             not (tables.is_contiguous() or tables.stride(1) == 1 or shape[1] == 1):
@@ -454,8 +450,9 @@ def block_tables(lengths: torch.Tensor, new: torch.Tensor, free: torch.Tensor, t
                                   ("taken", torch.int32, b + 1)):
             _rows_of(getattr(out, name), name, dtype, (size,), 1, dev)
     slots, rows, positions, starts, taken = out
+    width = tables.shape[1]
     _on(dev, "jb_block_tables", lengths.data_ptr(), new.data_ptr(), b, free.data_ptr(), free.shape[0],
-        tables.data_ptr(), _apart(tables), tables.shape[1], kv_entry, page_tokens, 1 if fixed else 0, tokens,
+        tables.data_ptr(), tables.stride(0) if b > 1 else width, width, kv_entry, page_tokens, 1 if fixed else 0, tokens,
         slots.data_ptr(), rows.data_ptr(), positions.data_ptr(), starts.data_ptr(), taken.data_ptr())
     return out
 
@@ -514,8 +511,8 @@ def attn_prep_axes(pr: torch.Tensor, q_w1: torch.Tensor, k_w1: torch.Tensor, inv
         out = pr.new_empty((t, C.NQ, C.HD))
     else:
         _rows_of(out, "out", DT, (t, C.NQ, C.HD), 3, dev)
-    pages = (None, 0, 0, attn_layer, 0) if kv is None else (kv.data_ptr(), kv.shape[0], 2 * _apart(kv), attn_layer,
-                                                            kv.shape[1])
+    pages = (None, 0, 0, attn_layer, 0) if kv is None else (
+        kv.data_ptr(), kv.shape[0], 2 * (kv.stride(0) if kv.shape[0] > 1 else kv.numel()), attn_layer, kv.shape[1])
     _on(dev, "jb_attn_prep_axes", pr.data_ptr(), pr.stride(0), t, q_w1.data_ptr(), k_w1.data_ptr(),
         inv_freq.data_ptr(), positions.data_ptr(), positions.stride(0), axes - (1 << 64) if axes >> 63 else axes,
         out.data_ptr(), ptr(kn), ptr(vn), *pages, ptr(slots))
@@ -562,9 +559,11 @@ def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, at
         scratch = q.new_empty(_decode_scratch(heads, kv_heads, dim), dtype=torch.float32)
     else:
         _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), dev)
-    _on(dev, "jb_decode_attention", q.data_ptr(), q.stride(0), kv.data_ptr(), pages, 2 * _apart(kv), attn_layer,
-        layers, tables.data_ptr(), _apart(tables), tables.shape[1], kv_entry, lengths.data_ptr(), b, heads,
-        kv_heads, dim, dim ** -0.5 if scale is None else scale, ptr(pr), 0 if pr is None else pr.stride(0),
+    width = tables.shape[1]
+    _on(dev, "jb_decode_attention", q.data_ptr(), q.stride(0), kv.data_ptr(), pages,
+        2 * (kv.stride(0) if pages > 1 else kv.numel()), attn_layer, layers, tables.data_ptr(),
+        tables.stride(0) if b > 1 else width, width, kv_entry, lengths.data_ptr(), b, heads, kv_heads, dim,
+        dim ** -0.5 if scale is None else scale, ptr(pr), 0 if pr is None else pr.stride(0),
         out.data_ptr(), out.stride(0), scratch.data_ptr(), scratch.numel())
     return out
 
@@ -603,8 +602,10 @@ def _linear_of(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
         out = torch.empty_like(v, memory_format=torch.contiguous_format)
     else:
         _rows_of(out, "out", DT, shape, len(shape), dev)
-    return out, (state.data_ptr(), held[0], 4 * _apart(state), held[1], layer * heads, tables.data_ptr(),
-                 _apart(tables), ptr(out_tables), 0 if out_tables is None else _apart(out_tables))
+    one = b == 1
+    return out, (state.data_ptr(), held[0], 4 * (state.stride(0) if held[0] > 1 else state.numel()), held[1],
+                 layer * heads, tables.data_ptr(), width if one else tables.stride(0), ptr(out_tables),
+                 0 if out_tables is None else width if one else out_tables.stride(0))
 
 
 @functools.lru_cache(maxsize=256)
@@ -632,16 +633,16 @@ def linear_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     if real is not None:
         _rows_of(real, "real", torch.int32, (b,), 1, q.device)
     need = _scan_scratch(b, heads, n)
-    if need and not all(x.stride(1) > 0 and (b == 1 or x.stride(0) > 0) for x in (q, k, v)):
+    (q0, q1, _, _), (k0, k1, _, _), (v0, v1, _, _) = q.stride(), k.stride(), v.stride()
+    if need and not (q1 and k1 and v1 and (b == 1 or q0 and k0 and v0)):
         need = 0   # one token or row that stands for all goes token by token, in one launch
     if scratch is None:
         scratch = q.new_empty(need, dtype=torch.float32) if need else None
     else:
         _rows_of(scratch, "scratch", torch.float32, tuple(scratch.shape), scratch.dim(), q.device)
     steps = (0, 0) if g.dim() == 1 else g.stride()[:2]
-    _on(q.device, "jb_linear_scan", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-        v.data_ptr(), v.stride(0), v.stride(1), g.data_ptr(), *steps, ptr(real), o.data_ptr(), b, n, heads, *pool,
-        ptr(scratch), 0 if scratch is None else scratch.numel())
+    _on(q.device, "jb_linear_scan", q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, g.data_ptr(),
+        *steps, ptr(real), o.data_ptr(), b, n, heads, *pool, ptr(scratch), 0 if scratch is None else scratch.numel())
     if need:
         _lib.launches += 2   # in segments: their states, the join, the outputs
     return o
