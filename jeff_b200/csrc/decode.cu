@@ -169,9 +169,10 @@ __global__ void __launch_bounds__(TAB_THREADS) tables_kernel(const TabParams p) 
 // ------------------------------------------------------------------ attention input side, several rotary axes
 //
 // Per token and head: y = x rsqrt(mean(x^2) + eps) w1, then the pair (d, d + 32), d < 32, turned by the angle
-// pos[axis(d)] f_d. Everything stays in fp32 and is rounded to bf16 once, at the end. The angle is formed in fp64 (a
-// position of 31 bits times a 24-bit frequency is exact there) and reduced to a part of one turn before the fp32 sine
-// and cosine, so positions of any size keep full accuracy.
+// pos[axis(d)] f_d. Everything stays in fp32 and is rounded to bf16 once, at the end. The angle is formed in fp64 and
+// reduced to a part of one turn before the fp32 sine and cosine. There a position of up to 29 bits times a 24-bit frequency
+// is exact and past that rounded, as the factor 1 / 2 pi and its product are: in all at most 3 * 2^-53 of the angle, 7e-7 rad
+// at a position of 2^31 and a frequency of 1 (the fp32 sine and cosine themselves: some 1e-7).
 
 constexpr int NQ = 8, NKV = 2, HD = 256, ROT = 64;
 // From this many tokens on a warp takes a whole token; below, a block does, a warp a head. Measured back to back, in us,
@@ -364,9 +365,10 @@ __global__ void __launch_bounds__(128, 3) prep_tokens_kernel(const PrepParams p)
 // the query heads, so 4 query heads cost half of what a 16-row query tile would. (tcgen05 has no use here: its 128-row
 // tile would be filled with 4 rows.)
 // Measured on a B200, launch included: 64 ragged rows of 1 to 8,192 tokens (8 / 2 heads of 256, 537 MB) 105 us, 78% of
-// the copy rate; 33 rows of 100 to 4,096 (32 / 8 heads of 128, 283 MB) 61 us, 71%; one row of 1,000 10.2 us, latency.
-// What bounds it is how its pages lie: a ring of copies alone, without lookups, arithmetic and ends of rows, takes 94 us
-// for 537 MB in pages of six layers of which it reads one (5.7 TB/s), 82 us where the pages hold that layer alone. The
+// the copy rate; 33 rows of 100 to 4,096 (32 / 8 heads of 128, 283 MB) 61 us, 71%; one row of 1,000 9.8 us, latency.
+// What bounds it is how its pages lie: a ring of copies alone, without lookups, arithmetic and ends of rows, takes 95 us
+// for 537 MB in pages of six layers of which it reads one (5.7 TB/s), 83 us where the pages hold that layer alone, and 48
+// us for 277 MB of 8 heads of 128 with one layer a page or two (5.8 TB/s: a head's keys are 256 bytes, 2 KB apart). The
 // rest is the start (lengths, then tables, then keys), the ends of rows (1 us each; 3.3 with a thread a value) and SMs
 // that stream slower than others. Not kept: steps of all heads of fewer tokens, so that a page is read as one contiguous
 // piece (2% slower), two CTAs of four warps an SM (7%), shares in three waves (13%) or claimed by the CTAs that are done
@@ -382,7 +384,8 @@ struct Dec {
   static constexpr int HALVES = D == 64 ? 5 : 3;  // a warp's ring, in tiles' keys or values
   static constexpr int STEP = WARPS * TILE;       // tokens
   // bytes of a key in shared memory, its 16-byte chunk c at c ^ (key % 8): ldmatrix without conflicts, and rows on
-  // 128-byte lines (a 16-byte pad instead costs 11% of the streaming rate: 6.4 against 7.2 TB/s)
+  // 128-byte lines (with keys padded by 16 bytes instead, copies alone take 102 us for 537 MB in pages of six layers, not
+  // 95, and 51 for 277 MB of 128-wide heads, not 48)
   static constexpr int PITCH = D * 2;
   static constexpr int SLOT = TILE * PITCH;       // a tile's keys or its values; eight heads' outputs at a row's end
   static constexpr int SMEM = WARPS * HALVES * SLOT;
