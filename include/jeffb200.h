@@ -288,11 +288,12 @@ int jb_attn_prep_axes(const uint16_t* pr, int64_t ldpr, int t, const float* q_w1
 
 /* Attention of one new token per row over its cached keys: y (b, heads, dim) = softmax(scale q . k_j) v_j over the
  * tokens j < lengths[r] of pages tables[r][kv_entry + j / 32] (at most what the table's width holds); a row without
- * tokens is 0. dim 64, 128 or 256; heads a multiple of kv_heads, at most 16 to one; heads * dim at
- * most 2^24, tables of at most 0x7f000000 tokens and 2^38 / kv_heads. pr (nullable): y is multiplied by
- * sigmoid(pr[r, 2 dim h + dim + d]), the gate of jb_gate_mul. fp32 with one rounding to bf16. The keys of all rows
- * are cut into equal shares over the GPU and rows that were cut are joined from `scratch`
- * (at least jb_decode_attention_scratch floats, 16-byte aligned, overwritten, whatever it held) in a fixed order. */
+ * tokens is 0. dim 64, 128 or 256; heads a multiple of kv_heads, at most 16 to one; heads * dim at most 2^24, tables of
+ * at most 0x7f000000 tokens and 2^38 / kv_heads. pr (nullable): y is multiplied by
+ * sigmoid(pr[r, 2 dim h + dim + d]), the gate of jb_gate_mul. fp32 with one rounding to bf16. What is not finite reaches
+ * what the formula lets it reach, an infinite value perhaps as NaN. The keys of all rows are cut into equal shares over
+ * the GPU and rows that were cut are joined from `scratch` (at least jb_decode_attention_scratch floats, 16-byte
+ * aligned, overwritten, whatever it held) in a fixed order. */
 int jb_decode_attention(const uint16_t* q, int64_t ldq, const void* kv, int64_t pages, int64_t page_bytes,
                         int attn_layer, int attn_layers, const int32_t* tables, int table_stride, int width,
                         int kv_entry, const int32_t* lengths, int b, int heads, int kv_heads, int dim, float scale,

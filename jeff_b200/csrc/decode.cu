@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(128, 3) prep_tokens_kernel(const PrepParams p)
 // the query heads, so 4 query heads cost half of what a 16-row query tile would. (tcgen05 has no use here: its 128-row
 // tile would be filled with 4 rows.)
 // Measured on a B200, launch included: 64 ragged rows of 1 to 8,192 tokens (8 / 2 heads of 256, 537 MB) 105 us, 78% of
-// the copy rate; 33 rows of 100 to 4,096 (32 / 8 heads of 128, 283 MB) 61 us, 71%; one row of 1,000 9.8 us, latency.
+// the copy rate; 33 rows of 100 to 4,096 (32 / 8 heads of 128, 283 MB) 59 us, 73%; one row of 1,000 9.8 us, latency.
 // What bounds it is how its pages lie: a ring of copies alone, without lookups, arithmetic and ends of rows, takes 95 us
 // for 537 MB in pages of six layers of which it reads one (5.7 TB/s), 83 us where the pages hold that layer alone, and 48
 // us for 277 MB of 8 heads of 128 with one layer a page or two (5.8 TB/s: a head's keys are 256 bytes, 2 KB apart). The

@@ -9,9 +9,11 @@
 //   MMA4  S^T += V^T Kd               (Kd = e^{gl - gc} K in bf16 parts, S^T scaled by e^gl beforehand)
 // Rounding: the state is fp32 and what enters it keeps 24 bits (three bf16 parts of a decayed key, the value exact).
 // Ahead of an output's own rounding its terms are rounded once, by P for the tokens of its chunk, by the state's bf16
-// copy for those before (where the state itself is another launch's, two parts of Kd, 16 bits, serve that copy). Sums
-// of decays are fp64, their differences rounded to fp32 once, so that a strong decay early in a chunk takes no accuracy
-// from the tokens behind it (-inf is held as -10000, whose exponential is 0). A value that is not finite would reach earlier
+// copy for those before (where the state itself is another launch's, two parts of Kd, 16 bits, serve that copy): errors
+// of 0.0023 of the outputs' norm, where their own rounding makes 0.0017. A second part of P and of the copy would be 12
+// more products a chunk (some 600 of its cycles by the figures below) and twice their places and stores. Sums of decays
+// are fp64, their differences rounded to fp32 once, so that a strong decay early in a chunk takes no accuracy from the
+// tokens behind it (-inf is held as -10000, whose exponential is 0). A value that is not finite would reach earlier
 // tokens of its chunk through the zeros of P: where an output is not finite it is formed again without them.
 //
 // Tensor memory, 256 columns: S^T 0-127, its bf16 copy 128-191 (E once MMA1 has read it), D 192-255. Shared memory 108
@@ -27,7 +29,7 @@
 // N128 K16 product and 49 for N64, the gates' sums and exponentials 1200; 5100 in all with outputs, so 2550 an SM) and,
 // close behind, shared memory, which the operands (8 KB a product), the copies and Kd keep busy for 2300 cycles a chunk
 // with outputs and 1540 without; two CTAs an SM take 8600 each. HBM would need 2000. Measured on a B200: 64 rows of 128
-// tokens 65 us (231 MB with the states, 54% of the copy rate), two rows of 8,192 108 us (272 MB, 38%; 42 the states, 8
+// tokens 64 us (231 MB with the states, 55% of the copy rate), two rows of 8,192 108 us (272 MB, 38%; 42 the states, 8
 // the join, 66 the outputs, whose starts overlap), one row of 1,001 22 us (23 where the second and third launch read
 // nothing ahead of their waits). Not kept: MMA2 into D as soon as the outputs have left it, P formed under MMA1 (a chunk
 // shorter by the state's update on paper, 6% slower: Q and K are then needed sooner than they come).

@@ -380,8 +380,8 @@ def _rows_of(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, .
 
 
 def _tables_of(tables: torch.Tensor, name: str, rows: int, width: int, device: torch.device) -> None:
-    """Block tables of at least `rows` rows and `width` entries, packed or with their rows apart. (Where one row, page or
-    token is all there is, its tensor's stride may be anything: the calls below give the packed size instead.)"""
+    """Block tables of at least `rows` rows and `width` entries, packed or with their rows apart. (The stride of a single
+    row or page may be anything: the calls below give its packed size instead.)"""
     shape = tables.shape
     if len(shape) != 2 or shape[0] < rows or shape[1] < width or tables.dtype is not torch.int32 or \
             not (tables.is_contiguous() or tables.stride(1) == 1 or shape[1] == 1):
@@ -452,8 +452,8 @@ def block_tables(lengths: torch.Tensor, new: torch.Tensor, free: torch.Tensor, t
     slots, rows, positions, starts, taken = out
     width = tables.shape[1]
     _on(dev, "jb_block_tables", lengths.data_ptr(), new.data_ptr(), b, free.data_ptr(), free.shape[0],
-        tables.data_ptr(), tables.stride(0) if b > 1 else width, width, kv_entry, page_tokens, 1 if fixed else 0, tokens,
-        slots.data_ptr(), rows.data_ptr(), positions.data_ptr(), starts.data_ptr(), taken.data_ptr())
+        tables.data_ptr(), tables.stride(0) if b > 1 else width, width, kv_entry, page_tokens, 1 if fixed else 0,
+        tokens, slots.data_ptr(), rows.data_ptr(), positions.data_ptr(), starts.data_ptr(), taken.data_ptr())
     return out
 
 
@@ -530,11 +530,12 @@ def decode_attention(q: torch.Tensor, kv: torch.Tensor, tables: torch.Tensor, at
     """Attention of one new token per row, q (b, heads, dim), over the row's lengths[r] cached tokens (its own among
     them, once attn_prep_axes has written it) in the pages tables[r][kv_entry + j // 32] of kv (an entry that is 0, the
     sink, or outside kv is no page: its tokens are left out); heads of 64, 128 or 256, up to 16 query heads to a
-    key/value head, scale 1 / sqrt(dim) unless given. A row without tokens is zeros. With pr (the q_proj output, query
-    and gate interleaved per head): times sigmoid(gate), as (b, heads * dim), the o_proj's input; without, (b, heads,
-    dim). fp32 with one rounding. All rows' keys are cut into equal shares over the SMs, whatever the lengths; scratch
-    (fp32, jb_decode_attention_scratch of them, overwritten by every call; calls that may run at the same time need
-    their own) holds the cut rows' parts and is allocated unless given."""
+    key/value head, scale 1 / sqrt(dim) unless given. A row without tokens is zeros. What is not finite reaches what the
+    formula lets it reach, an infinite value perhaps as NaN. With pr (the q_proj output, query and gate interleaved per
+    head): times sigmoid(gate), as (b, heads * dim), the o_proj's input; without, (b, heads, dim). fp32 with one
+    rounding. All rows' keys are cut into equal shares over the SMs, whatever the lengths; scratch (fp32,
+    jb_decode_attention_scratch of them, overwritten by every call; calls that may run at the same time need their own)
+    holds the cut rows' parts and is allocated unless given."""
     dev = q.device
     shape = q.shape
     if len(shape) != 3:
